@@ -10,7 +10,7 @@ OUT=${VAR_OUT:-gym_amd/lib/variants}
 mkdir -p "$OUT"
 name=$1; file=$2; shift 2
 base=$(basename "$file" .hip)
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt "$@" -c "$SRC/$file" -o /tmp/variant_${name}.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c "$SRC/$file" -o /tmp/variant_${name}.o
 objs=""
 for o in gym_amd/lib/obj/*.o; do
   if [ "$(basename "$o" .o)" != "$base" ]; then objs="$objs $o"; fi
