@@ -128,6 +128,18 @@ public sealed unsafe class GpuVectorEnv<TState, TAction, TObs> : IDisposable
                         GxPolicy policy = GxPolicy.Random, IntPtr dActions = default, IntPtr stream = default)
         => Native.Check(Native.gx_vec_rollout_out(_vec.DangerousGetHandle(), kSteps, (int)policy, dActions, (int)output,
                                                   dRewardRows, dDoneRows, dTruncatedRows, stream));
+    /// <summary>One step with actions drawn from a policy's logits on the GPU (gx_vec_step_logits).</summary>
+    public void StepLogits(GxSample sample, IntPtr stream = default)
+    {
+        sample.StructSize = (uint)sizeof(GxSample);
+        Native.Check(Native.gx_vec_step_logits(_vec.DangerousGetHandle(), &sample, stream));
+    }
+    /// <summary>Rows of an embedding table for the current Discrete observations (gx_vec_embed_obs).</summary>
+    public void EmbedObs(GxEmbed embed, IntPtr stream = default)
+    {
+        embed.StructSize = (uint)sizeof(GxEmbed);
+        Native.Check(Native.gx_vec_embed_obs(_vec.DangerousGetHandle(), &embed, stream));
+    }
     public GxStats Stats() { Native.Check(Native.gx_vec_stats(_vec.DangerousGetHandle(), out GxStats s)); return s; }
 
     /// <summary>The SoA state image (gx_vec_get_state): n_real rows of NumEnvs reals, then n_int rows of int32.</summary>

@@ -27,7 +27,10 @@ public enum GxPolicy { DeviceActions = 0, Random = 1 }
 
 public enum GxRolloutOut { Last = 0, All = 1, None = 2 }
 
-public enum GxDType { F32 = 0, F64 = 1, I32 = 2, U8 = 3 }
+public enum GxDType { F32 = 0, F64 = 1, I32 = 2, U8 = 3, F16 = 4, BF16 = 5, I64 = 6 }
+
+[Flags]
+public enum GxOpFlags : uint { None = 0, DefaultStream = 1 }
 
 [StructLayout(LayoutKind.Sequential)]
 public unsafe struct GxDesc
@@ -104,6 +107,36 @@ public struct GxRows
     public IntPtr StateReal, Steps, EpReturn, Actions, Reward, Done, Stats, Error;
 }
 
+// gx_sample: one action a row from a policy's logits (device pointers)
+[StructLayout(LayoutKind.Sequential)]
+public struct GxSample
+{
+    public uint StructSize, OpFlags;
+    public int LogitsDType, NActions;
+    public ulong Rows;
+    public long RowStride, ColStride;
+    public IntPtr Logits, U, Temperature, TopK, TopP, MinP;
+    public float TemperatureAll;
+    public int TopKAll;
+    public float TopPAll, MinPAll;
+    public IntPtr Actions, Logprob, Workspace;
+    public ulong WorkspaceBytes;
+}
+
+// gx_embed: rows of a table by Discrete observations, and the table's gradient (device pointers)
+[StructLayout(LayoutKind.Sequential)]
+public struct GxEmbed
+{
+    public uint StructSize, OpFlags;
+    public int TableDType, RowsDType, IdsDType, Accumulate;
+    public ulong Tokens;
+    public long NStates, Dim, TableStride, RowsStride;
+    public IntPtr Ids, Table, Rows, Workspace;
+    public ulong WorkspaceBytes;
+    public float Scale;
+    public int Reserved;
+}
+
 internal static unsafe partial class Native
 {
     private const string Lib = "gymx"; // resolves libgymx.so on Linux
@@ -134,6 +167,13 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int gx_vec_sample_actions(IntPtr vec, ulong tick, IntPtr dActions, IntPtr stream);
     [LibraryImport(Lib)] internal static partial int gx_vec_tick(IntPtr vec, out ulong tick);
     [LibraryImport(Lib)] internal static partial int gx_vec_stats(IntPtr vec, out GxStats stats);
+    [LibraryImport(Lib)] internal static partial int gx_sample_workspace(IntPtr ctx, GxSample* sample, out ulong bytes);
+    [LibraryImport(Lib)] internal static partial int gx_sample_logits(IntPtr ctx, GxSample* sample, IntPtr stream);
+    [LibraryImport(Lib)] internal static partial int gx_vec_step_logits(IntPtr vec, GxSample* sample, IntPtr stream);
+    [LibraryImport(Lib)] internal static partial int gx_embed_lookup(IntPtr ctx, GxEmbed* embed, IntPtr stream);
+    [LibraryImport(Lib)] internal static partial int gx_embed_grad_workspace(IntPtr ctx, GxEmbed* embed, out ulong bytes);
+    [LibraryImport(Lib)] internal static partial int gx_embed_grad(IntPtr ctx, GxEmbed* embed, IntPtr stream);
+    [LibraryImport(Lib)] internal static partial int gx_vec_embed_obs(IntPtr vec, GxEmbed* embed, IntPtr stream);
     [LibraryImport(Lib)] internal static partial int gx_comm_unique_id(byte* id128);
     [LibraryImport(Lib)] internal static partial int gx_comm_init(IntPtr ctx, byte* id128, int rank, int world, out IntPtr comm);
     [LibraryImport(Lib)] internal static partial int gx_comm_destroy(IntPtr comm);

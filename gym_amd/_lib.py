@@ -18,7 +18,8 @@ MODE_EXACT, MODE_FAST32, MODE_FP64 = 0, 1, 2
 AUTORESET, RECORD_STATS, SLIPPERY, TAXI_FULL, ACROBOT_RK4, BLACKJACK_FULL = 1, 2, 4, 8, 16, 64
 POLICY_DEVICE_ACTIONS, POLICY_RANDOM = 0, 1
 OUT_LAST, OUT_ALL, OUT_NONE = 0, 1, 2
-F32, F64, I32, U8 = range(4)
+F32, F64, I32, U8, F16, BF16, I64 = range(7)
+OP_DEFAULT_STREAM = 1
 
 
 class GxDesc(C.Structure):
@@ -74,6 +75,29 @@ class GxRows(C.Structure):
     ]
 
 
+class GxSample(C.Structure):
+    """gx_sample: one action a row from a policy's logits"""
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("op_flags", C.c_uint32), ("logits_dtype", C.c_int32), ("n_actions", C.c_int32),
+        ("rows", C.c_uint64), ("row_stride", C.c_int64), ("col_stride", C.c_int64), ("logits", C.c_void_p),
+        ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p), ("temperature_all", C.c_float), ("top_k_all", C.c_int32), ("top_p_all", C.c_float),
+        ("min_p_all", C.c_float), ("actions", C.c_void_p), ("logprob", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class GxEmbed(C.Structure):
+    """gx_embed: rows of a table by Discrete observations, and the table's gradient"""
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("op_flags", C.c_uint32), ("table_dtype", C.c_int32), ("rows_dtype", C.c_int32),
+        ("ids_dtype", C.c_int32), ("accumulate", C.c_int32), ("tokens", C.c_uint64), ("n_states", C.c_int64),
+        ("dim", C.c_int64), ("table_stride", C.c_int64), ("rows_stride", C.c_int64), ("ids", C.c_void_p),
+        ("table", C.c_void_p), ("rows", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("scale", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
 ROWS_MAX_ENVS = 1 << 24
 
 
@@ -112,6 +136,13 @@ SIGNATURES = {
     "gx_vec_tick": (_i, [_vp, C.POINTER(_u64)]),
     "gx_vec_stats": (_i, [_vp, C.POINTER(GxStats)]),
     "gx_rows_step": (_i, [_vp, C.POINTER(GxRows), _i, _vp]),
+    "gx_sample_workspace": (_i, [_vp, C.POINTER(GxSample), C.POINTER(_u64)]),
+    "gx_sample_logits": (_i, [_vp, C.POINTER(GxSample), _vp]),
+    "gx_vec_step_logits": (_i, [_vp, C.POINTER(GxSample), _vp]),
+    "gx_embed_lookup": (_i, [_vp, C.POINTER(GxEmbed), _vp]),
+    "gx_embed_grad_workspace": (_i, [_vp, C.POINTER(GxEmbed), C.POINTER(_u64)]),
+    "gx_embed_grad": (_i, [_vp, C.POINTER(GxEmbed), _vp]),
+    "gx_vec_embed_obs": (_i, [_vp, C.POINTER(GxEmbed), _vp]),
     "gx_comm_unique_id": (_i, [_vp]),
     "gx_comm_init": (_i, [_vp, _vp, _i, _i, C.POINTER(_vp)]),
     "gx_comm_destroy": (_i, [_vp]),

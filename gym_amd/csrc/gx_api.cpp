@@ -22,6 +22,7 @@
 #include "../../include/gymx.h"
 #include "gx_device.h"
 #include "gx_launch.h"
+#include "gx_policy.h"
 
 using namespace gx;
 
@@ -1350,6 +1351,189 @@ extern "C" int gx_rows_step(gx_ctx* c, const gx_rows* r, int k_steps, void* stre
   static_assert(sizeof(gx_stats) == 48 && sizeof(gx_stats) <= sizeof(StatSlot), "gx_stats is the head of StatSlot");
   HIP_TRY(hipMemcpyAsync(r->stats, result, sizeof(gx_stats), hipMemcpyDeviceToDevice, stream));
   if (r->error) HIP_TRY(hipMemcpyAsync(r->error, err, 4, hipMemcpyDeviceToDevice, stream));
+  return GX_OK;
+}
+
+// ------------------------------------------ between a policy and a batch ---
+namespace {
+
+// These entry points run on the context's GPU and leave the calling thread's current device as it was: their callers
+// hold tensors of a framework that tracks it.
+struct DeviceScope {
+  int before = -1;
+  hipError_t error = hipSuccess;
+  explicit DeviceScope(int device) {
+    error = hipGetDevice(&before);
+    if (error == hipSuccess && before != device) error = hipSetDevice(device);
+    else before = -1;
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+hipStream_t op_stream(const gx_ctx* c, uint32_t op_flags, void* stream) {
+  return stream || (op_flags & GX_OP_DEFAULT_STREAM) ? (hipStream_t)stream : c->compute;
+}
+
+bool is_float_type(int dt) { return dt == GX_F32 || dt == GX_F16 || dt == GX_BF16; }
+size_t float_type_size(int dt) { return dt == GX_F32 ? 4 : 2; }
+
+// largest element offset a kernel forms, kept far inside int64
+bool span_fits(uint64_t count, int64_t stride, uint64_t inner) {
+  return count == 0 || (unsigned __int128)(count - 1) * (uint64_t)stride + inner < ((unsigned __int128)1 << 60);
+}
+
+int sample_args(const char* who, const gx_sample* s, bool draws, SampleArgs* a) {
+  if (s->struct_size != sizeof(gx_sample)) return fail(GX_ERR_INVALID, "%s: gx_sample.struct_size is %u, expected %zu", who, s->struct_size, sizeof(gx_sample));
+  if (s->op_flags & ~(uint32_t)GX_OP_DEFAULT_STREAM) return fail(GX_ERR_INVALID, "%s: unknown op_flags 0x%x", who, s->op_flags);
+  if (!is_float_type(s->logits_dtype)) return fail(GX_ERR_UNSUPPORTED, "%s: logits of dtype %d (GX_F32, GX_F16, GX_BF16)", who, s->logits_dtype);
+  if (s->n_actions < 1 || s->n_actions > (1 << 24)) return fail(GX_ERR_INVALID, "%s: n_actions %d outside 1..2^24", who, s->n_actions);
+  if (s->rows > (1ull << 40)) return fail(GX_ERR_INVALID, "%s: %llu rows exceed 2^40", who, (unsigned long long)s->rows);
+  if (s->row_stride < 0 || s->col_stride < 0) return fail(GX_ERR_INVALID, "%s: negative stride", who);
+  if (!span_fits((uint64_t)s->n_actions, s->col_stride, 1) ||
+      !span_fits(s->rows, s->row_stride, (uint64_t)(s->n_actions - 1) * (uint64_t)s->col_stride + 1))
+    return fail(GX_ERR_INVALID, "%s: the strides reach past 2^60 elements", who);
+  if (!s->temperature && !(s->temperature_all >= 0.0f)) return fail(GX_ERR_INVALID, "%s: temperature %g must not be negative", who, (double)s->temperature_all);
+  if (!s->top_k && s->top_k_all < 0) return fail(GX_ERR_INVALID, "%s: top_k %d must not be negative", who, s->top_k_all);
+  if (!s->top_p && !(s->top_p_all >= 0.0f && s->top_p_all <= 1.0f)) return fail(GX_ERR_INVALID, "%s: top_p %g outside [0, 1]", who, (double)s->top_p_all);
+  if (!s->min_p && !(s->min_p_all >= 0.0f && s->min_p_all <= 1.0f)) return fail(GX_ERR_INVALID, "%s: min_p %g outside [0, 1]", who, (double)s->min_p_all);
+  if (s->rows) {
+    if (!s->logits || !s->actions) return fail(GX_ERR_INVALID, "%s: null logits or actions", who);
+    if (!s->u && !draws) return fail(GX_ERR_INVALID, "%s: u is null: the random numbers are the caller's", who);
+    if ((uintptr_t)s->logits & (float_type_size(s->logits_dtype) - 1)) return fail(GX_ERR_INVALID, "%s: logits must be aligned to their element", who);
+    const void* ptrs[] = {s->u, s->temperature, s->top_k, s->top_p, s->min_p, s->actions, s->logprob};
+    for (const void* p : ptrs)
+      if ((uintptr_t)p & 3) return fail(GX_ERR_INVALID, "%s: u, the parameters, actions and logprob must be 4-byte aligned", who);
+  }
+  *a = SampleArgs{};
+  a->logits = s->logits; a->rows = s->rows; a->row_stride = s->row_stride; a->col_stride = s->col_stride;
+  a->n = s->n_actions;
+  a->u = s->u; a->temperature = s->temperature; a->top_k = s->top_k; a->top_p = s->top_p; a->min_p = s->min_p;
+  a->temperature_all = s->temperature_all; a->top_k_all = s->top_k_all; a->top_p_all = s->top_p_all; a->min_p_all = s->min_p_all;
+  a->actions = s->actions; a->logprob = s->logprob;
+  return GX_OK;
+}
+
+int check_workspace(const char* who, size_t need, const void* ws, uint64_t bytes) {
+  if (!need) return GX_OK;
+  if (!ws || bytes < need) return fail(GX_ERR_INVALID, "%s: needs a workspace of %zu bytes, got %llu", who, need, ws ? (unsigned long long)bytes : 0ull);
+  if ((uintptr_t)ws & 255) return fail(GX_ERR_INVALID, "%s: the workspace must be 256-byte aligned", who);
+  return GX_OK;
+}
+
+int run_sample(const char* who, gx_ctx* c, const gx_sample* s, const SampleArgs& a, hipStream_t stream) {
+  if (int rc = check_workspace(who, sample_workspace(a, c->num_cus), s->workspace, s->workspace_bytes)) return rc;
+  if (a.rows == 0) return GX_OK;
+  HIP_TRY(launch_sample_logits(a, s->logits_dtype, s->workspace, c->num_cus, stream));
+  return GX_OK;
+}
+
+int embed_args(const char* who, const gx_embed* e, bool own_ids, EmbedArgs* a) {
+  if (e->struct_size != sizeof(gx_embed)) return fail(GX_ERR_INVALID, "%s: gx_embed.struct_size is %u, expected %zu", who, e->struct_size, sizeof(gx_embed));
+  if (e->op_flags & ~(uint32_t)GX_OP_DEFAULT_STREAM) return fail(GX_ERR_INVALID, "%s: unknown op_flags 0x%x", who, e->op_flags);
+  if (!is_float_type(e->table_dtype) || !is_float_type(e->rows_dtype))
+    return fail(GX_ERR_UNSUPPORTED, "%s: table of dtype %d, rows of dtype %d (GX_F32, GX_F16, GX_BF16)", who, e->table_dtype, e->rows_dtype);
+  if (e->ids_dtype != GX_I32 && e->ids_dtype != GX_I64) return fail(GX_ERR_UNSUPPORTED, "%s: ids of dtype %d (GX_I32, GX_I64)", who, e->ids_dtype);
+  if (e->tokens > 0x7FFFFFFFull) return fail(GX_ERR_INVALID, "%s: %llu tokens exceed 2^31-1", who, (unsigned long long)e->tokens);
+  if (e->n_states < 1 || e->n_states > 0x7FFFFFFFll) return fail(GX_ERR_INVALID, "%s: n_states %lld outside 1..2^31-1", who, (long long)e->n_states);
+  if (e->dim < 1 || e->dim > (1 << 24)) return fail(GX_ERR_INVALID, "%s: dim %lld outside 1..2^24", who, (long long)e->dim);
+  if (e->table_stride < e->dim || e->rows_stride < e->dim) return fail(GX_ERR_INVALID, "%s: rows overlap: strides %lld and %lld, dim %lld", who, (long long)e->table_stride, (long long)e->rows_stride, (long long)e->dim);
+  if (!span_fits((uint64_t)e->n_states, e->table_stride, (uint64_t)e->dim) || !span_fits(e->tokens, e->rows_stride, (uint64_t)e->dim))
+    return fail(GX_ERR_INVALID, "%s: the strides reach past 2^60 elements", who);
+  if (!e->table || (e->tokens && !e->rows)) return fail(GX_ERR_INVALID, "%s: null table or rows", who);
+  if (e->tokens && !own_ids && !e->ids) return fail(GX_ERR_INVALID, "%s: null ids", who);
+  if (((uintptr_t)e->table & (float_type_size(e->table_dtype) - 1)) || ((uintptr_t)e->rows & (float_type_size(e->rows_dtype) - 1)) ||
+      ((uintptr_t)e->ids & (e->ids_dtype == GX_I64 ? 7 : 3)))
+    return fail(GX_ERR_INVALID, "%s: table, rows and ids must be aligned to their elements", who);
+  if (!std::isfinite(e->scale)) return fail(GX_ERR_INVALID, "%s: scale %g is not finite", who, (double)e->scale);
+  *a = EmbedArgs{};
+  a->ids = e->ids; a->ids64 = e->ids_dtype == GX_I64; a->accumulate = e->accumulate != 0; a->tokens = e->tokens;
+  a->n_states = e->n_states; a->dim = e->dim; a->table_stride = e->table_stride; a->rows_stride = e->rows_stride;
+  a->table = e->table; a->rows = e->rows; a->scale = e->scale;
+  return GX_OK;
+}
+
+}  // namespace
+
+extern "C" int gx_sample_workspace(gx_ctx* c, const gx_sample* s, uint64_t* bytes) {
+  if (!c || !s || !bytes) return fail(GX_ERR_INVALID, "gx_sample_workspace: null argument");
+  SampleArgs a;
+  if (int rc = sample_args("gx_sample_workspace", s, true, &a)) return rc;
+  *bytes = sample_workspace(a, c->num_cus);
+  return GX_OK;
+}
+
+extern "C" int gx_sample_logits(gx_ctx* c, const gx_sample* s, void* stream) {
+  if (!c || !s) return fail(GX_ERR_INVALID, "gx_sample_logits: null argument");
+  SampleArgs a;
+  if (int rc = sample_args("gx_sample_logits", s, false, &a)) return rc;
+  DeviceScope dev(c->device);
+  HIP_TRY(dev.error);
+  return run_sample("gx_sample_logits", c, s, a, op_stream(c, s->op_flags, stream));
+}
+
+extern "C" int gx_vec_step_logits(gx_vec* v, const gx_sample* s, void* stream_) {
+  if (!v || !s) return fail(GX_ERR_INVALID, "gx_vec_step_logits: null argument");
+  if (v->info.action_dtype != GX_I32) return fail(GX_ERR_UNSUPPORTED, "gx_vec_step_logits: env id %d has Box actions", v->desc.env_id);
+  SampleArgs a;
+  if (int rc = sample_args("gx_vec_step_logits", s, true, &a)) return rc;
+  if (s->rows != v->n) return fail(GX_ERR_INVALID, "gx_vec_step_logits: %llu rows of logits for %llu envs", (unsigned long long)s->rows, (unsigned long long)v->n);
+  if (s->n_actions != v->info.action_n) return fail(GX_ERR_INVALID, "gx_vec_step_logits: %d logits a row, ActionSpace is Discrete(%d)", s->n_actions, v->info.action_n);
+  if ((uintptr_t)s->actions & 15) return fail(GX_ERR_INVALID, "gx_vec_step_logits: actions must be 16-byte aligned");
+  a.seed_lo = (uint32_t)v->desc.seed;
+  a.seed_hi = (uint32_t)(v->desc.seed >> 32);
+  a.tick = v->tick;
+  a.env_index_base = v->desc.env_index_base;
+  DeviceScope dev(v->ctx->device);
+  HIP_TRY(dev.error);
+  const hipStream_t stream = op_stream(v->ctx, s->op_flags, stream_);
+  if (int rc = run_sample("gx_vec_step_logits", v->ctx, s, a, stream)) return rc;
+  return launch_step(v, s->actions, 1, v->stride, GX_POLICY_DEVICE_ACTIONS, stream);
+}
+
+extern "C" int gx_embed_lookup(gx_ctx* c, const gx_embed* e, void* stream) {
+  if (!c || !e) return fail(GX_ERR_INVALID, "gx_embed_lookup: null argument");
+  EmbedArgs a;
+  if (int rc = embed_args("gx_embed_lookup", e, false, &a)) return rc;
+  if (a.tokens == 0) return GX_OK;
+  DeviceScope dev(c->device);
+  HIP_TRY(dev.error);
+  HIP_TRY(launch_embed_lookup(a, e->table_dtype, e->rows_dtype, c->num_cus, op_stream(c, e->op_flags, stream)));
+  return GX_OK;
+}
+
+extern "C" int gx_embed_grad_workspace(gx_ctx* c, const gx_embed* e, uint64_t* bytes) {
+  if (!c || !e || !bytes) return fail(GX_ERR_INVALID, "gx_embed_grad_workspace: null argument");
+  EmbedArgs a;
+  if (int rc = embed_args("gx_embed_grad_workspace", e, true, &a)) return rc;
+  *bytes = embed_grad_workspace(a, c->num_cus);
+  return GX_OK;
+}
+
+extern "C" int gx_embed_grad(gx_ctx* c, const gx_embed* e, void* stream) {
+  if (!c || !e) return fail(GX_ERR_INVALID, "gx_embed_grad: null argument");
+  EmbedArgs a;
+  if (int rc = embed_args("gx_embed_grad", e, false, &a)) return rc;
+  if (int rc = check_workspace("gx_embed_grad", embed_grad_workspace(a, c->num_cus), e->workspace, e->workspace_bytes)) return rc;
+  DeviceScope dev(c->device);
+  HIP_TRY(dev.error);
+  HIP_TRY(launch_embed_grad(a, e->table_dtype, e->rows_dtype, e->workspace, c->num_cus, op_stream(c, e->op_flags, stream)));
+  return GX_OK;
+}
+
+extern "C" int gx_vec_embed_obs(gx_vec* v, const gx_embed* e, void* stream) {
+  if (!v || !e) return fail(GX_ERR_INVALID, "gx_vec_embed_obs: null argument");
+  if (!v->is_tabular) return fail(GX_ERR_UNSUPPORTED, "gx_vec_embed_obs: the observation of env id %d is not Discrete", v->desc.env_id);
+  if (e->ids) return fail(GX_ERR_INVALID, "gx_vec_embed_obs: ids are the batch's own observations and must be null");
+  EmbedArgs a;
+  if (int rc = embed_args("gx_vec_embed_obs", e, true, &a)) return rc;
+  if (e->tokens != v->n) return fail(GX_ERR_INVALID, "gx_vec_embed_obs: %llu tokens for %llu envs", (unsigned long long)e->tokens, (unsigned long long)v->n);
+  a.ids = v->d_int;
+  a.ids64 = 0;
+  DeviceScope dev(v->ctx->device);
+  HIP_TRY(dev.error);
+  HIP_TRY(launch_embed_lookup(a, e->table_dtype, e->rows_dtype, v->ctx->num_cus, op_stream(v->ctx, e->op_flags, stream)));
   return GX_OK;
 }
 

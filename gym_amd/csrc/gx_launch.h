@@ -94,4 +94,16 @@ hipError_t launch_stats_materialize_returns(const StepArgs& a, const int32_t* le
 hipError_t launch_stats_flush_open(const StepArgs& a, int ep_return_is_f64, const int32_t* length_row, dim3 grid,
                                    hipStream_t stream);
 
+// actions from a policy's logits (gx_sample.hip); dtype: the logits' gx_dtype.  Grids and the workspace's layout follow
+// from the arguments and the number of compute units alone.
+struct SampleArgs;
+size_t sample_workspace(const SampleArgs& a, int num_cus);
+hipError_t launch_sample_logits(const SampleArgs& a, int dtype, void* workspace, int num_cus, hipStream_t stream);
+
+// embedding of Discrete observations (gx_embed.hip); the gx_dtypes of the table and of the rows
+struct EmbedArgs;
+hipError_t launch_embed_lookup(const EmbedArgs& a, int table_dtype, int rows_dtype, int num_cus, hipStream_t stream);
+size_t embed_grad_workspace(const EmbedArgs& a, int num_cus);
+hipError_t launch_embed_grad(const EmbedArgs& a, int table_dtype, int rows_dtype, void* workspace, int num_cus, hipStream_t stream);
+
 }  // namespace gx

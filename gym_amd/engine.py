@@ -184,6 +184,22 @@ class DeviceBatch:
     def sample_actions(self, tick, d_actions_ptr, stream=None):
         L.check(L.load().gx_vec_sample_actions(self._h, tick, C.c_void_p(d_actions_ptr), C.c_void_p(stream or 0)))
 
+    # ---- a policy on the GPU (torch tensors, on torch's current stream) ----
+    def step_logits(self, logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One step with actions drawn from a policy's logits [num_envs, n_actions] -> (actions int32 [num_envs],
+        logprob float32 [num_envs]); the arguments are gym_amd.policy.sample_logits', u = None draws from the batch's
+        generator (gx_vec_step_logits)."""
+        from . import policy
+
+        return policy.step_logits(self, logits, u, temperature, top_k, top_p, min_p)
+
+    def embed_obs(self, weight, scale=1.0, dtype=None, out=None):
+        """Rows of an embedding table for the batch's current Discrete observations: gym_amd.policy.embed_lookup with
+        the observation row as ids (gx_vec_embed_obs)."""
+        from . import policy
+
+        return policy.embed_obs(self, weight, scale, dtype, out)
+
     def view(self):
         v = L.GxView()
         L.check(L.load().gx_vec_device_view(self._h, C.byref(v)))

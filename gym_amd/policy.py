@@ -1,0 +1,228 @@
+"""Between a policy on the GPU and a batch of environments: actions drawn from logits, rows of an embedding table for
+Discrete observations and that table's gradient (gx_sample, gx_embed of include/gymx.h), on torch tensors.
+
+torch is used for memory and streams only: every call checks its tensors, launches HIP kernels on the current stream of
+the tensors' device and returns without waiting.  Scratch memory comes from torch's allocator, per call, so calls on
+several streams or in several captured graphs do not share any; what is returned belongs to the caller.  Nothing here
+differentiates by itself: embed_grad is the gradient to put behind embed_lookup.
+"""
+import ctypes as C
+
+from . import _lib as L
+from .envs import default_context
+
+_dtypes = {}
+
+
+def _torch():
+    import torch
+
+    if not _dtypes:
+        _dtypes.update({torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16, torch.int32: L.I32,
+                        torch.int64: L.I64})
+    return torch
+
+
+def _float_type(name, dtype):
+    code = _dtypes.get(dtype)
+    if code not in (L.F32, L.F16, L.BF16):
+        raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, dtype))
+    return code
+
+
+def _on_gpu(name, t, device=None):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor, not %s" % (name, type(t).__name__))
+    if not t.is_cuda:
+        raise ValueError("%s must be on the GPU, not %s" % (name, t.device))
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, device))
+
+
+def _vector(name, t, dtype, n, device):
+    _on_gpu(name, t, device)
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous %s tensor of shape (%d,)" % (name, dtype, n))
+    return t.data_ptr()
+
+
+def _call(fn, handle, desc, device):
+    L.check(fn(handle, C.byref(desc), _torch().cuda.current_stream(device).cuda_stream))
+
+
+def _workspace(torch, fn, ctx, desc, device):
+    need = C.c_uint64()
+    L.check(fn(ctx._h, C.byref(desc), C.byref(need)))
+    if not need.value:
+        return None
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device)  # torch's blocks are 512-byte aligned
+    desc.workspace, desc.workspace_bytes = ws.data_ptr(), need.value
+    return ws
+
+
+def _sample_desc(torch, logits, u, temperature, top_k, top_p, min_p, actions, logprob):
+    rows, n = logits.shape
+    dev = logits.device
+    d = L.GxSample(C.sizeof(L.GxSample), L.OP_DEFAULT_STREAM, _float_type("logits", logits.dtype), n, rows,
+                   logits.stride(0), logits.stride(1), logits.data_ptr())
+    if u is not None:
+        d.u = _vector("u", u, torch.float32, rows, dev)
+    if isinstance(temperature, torch.Tensor):
+        d.temperature = _vector("temperature", temperature, torch.float32, rows, dev)
+    else:
+        d.temperature_all = temperature
+    if isinstance(top_k, torch.Tensor):
+        d.top_k = _vector("top_k", top_k, torch.int32, rows, dev)
+    else:
+        d.top_k_all = min(top_k, 2**31 - 1)  # beyond the number of actions: all of them
+    if isinstance(top_p, torch.Tensor):
+        d.top_p = _vector("top_p", top_p, torch.float32, rows, dev)
+    else:
+        d.top_p_all = top_p
+    if isinstance(min_p, torch.Tensor):
+        d.min_p = _vector("min_p", min_p, torch.float32, rows, dev)
+    else:
+        d.min_p_all = min_p
+    d.actions, d.logprob = actions.data_ptr(), logprob.data_ptr()
+    return d
+
+
+def _logits(logits):
+    _on_gpu("logits", logits)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must have shape (rows, n_actions), not %s" % (tuple(logits.shape),))
+
+
+def _result(torch, name, t, dtype, n, device):
+    """an output: the caller's tensor, checked, or a new one"""
+    if t is None:
+        return torch.empty(n, dtype=dtype, device=device)
+    _vector(name, t, dtype, n, device)
+    return t
+
+
+def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, logprob=None):
+    """One action a row -> (actions int32 [rows], logprob float32 [rows]).
+
+    logits [rows, n_actions], float32 / float16 / bfloat16, any non-negative strides (a transposed [n_actions, rows]
+    included); -inf masks an action, NaN reads as -inf.  u: float32 [rows], the random numbers, in [0, 1).  Each
+    parameter is a number for all rows or a contiguous tensor [rows] (float32; top_k int32): temperature (0: the largest
+    logit, the lowest index among equals), top_k (0: all), top_p, min_p; what they keep and in which order is written at
+    gx_sample.  logprob is the log of the probability the action was drawn with.  A row without an action (all -inf):
+    action -1, logprob -inf.  out / logprob: tensors to write into."""
+    torch = _torch()
+    _logits(logits)
+    if u is None:
+        raise TypeError("u must be a torch tensor of random numbers (DeviceBatch.step_logits can draw its own)")
+    dev = logits.device
+    out = _result(torch, "out", out, torch.int32, logits.shape[0], dev)
+    logprob = _result(torch, "logprob", logprob, torch.float32, logits.shape[0], dev)
+    ctx = default_context(dev.index)
+    d = _sample_desc(torch, logits, u, temperature, top_k, top_p, min_p, out, logprob)
+    ws = _workspace(torch, L.load().gx_sample_workspace, ctx, d, dev)  # noqa: F841  (alive until the launch)
+    _call(L.load().gx_sample_logits, ctx._h, d, dev)
+    return out, logprob
+
+
+def step_logits(batch, logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """DeviceBatch.step_logits"""
+    torch = _torch()
+    _logits(logits)
+    dev = logits.device
+    if dev.index != batch.ctx.device:
+        raise ValueError("logits are on %s, the batch on GPU %d" % (dev, batch.ctx.device))
+    # the step reads whole vectors: the row is as long as the batch's own
+    actions = torch.empty(int(batch.view().stride), dtype=torch.int32, device=dev)
+    logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=dev)
+    d = _sample_desc(torch, logits, u, temperature, top_k, top_p, min_p, actions, logprob)
+    ws = _workspace(torch, L.load().gx_sample_workspace, batch.ctx, d, dev)  # noqa: F841
+    _call(L.load().gx_vec_step_logits, batch._h, d, dev)
+    return actions[:batch.n], logprob
+
+
+def _matrix(name, t, device=None):
+    _on_gpu(name, t, device)
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError("%s must have shape (rows, dim), not %s" % (name, tuple(t.shape)))
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("%s must have contiguous rows that do not overlap, strides are %s" % (name, t.stride()))
+    return max(t.stride(0), t.shape[1])
+
+
+def _ids(ids, device):
+    torch = _torch()
+    _on_gpu("ids", ids, device)
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 1 or not ids.is_contiguous():
+        raise ValueError("ids must be a contiguous int32 or int64 tensor of shape (tokens,)")
+
+
+def _lookup(fn, handle, weight, ids, tokens, scale, dtype, out):
+    torch = _torch()
+    stride = _matrix("weight", weight)
+    dev = weight.device
+    if weight.shape[0] < 1:
+        raise ValueError("weight has no rows")
+    if out is None:
+        out = torch.empty(tokens, weight.shape[1], dtype=dtype or weight.dtype, device=dev)
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError("out is %s, dtype says %s" % (out.dtype, dtype))
+    out_stride = _matrix("out", out, dev)
+    if tuple(out.shape) != (tokens, weight.shape[1]):
+        raise ValueError("out must have shape (%d, %d), not %s" % (tokens, weight.shape[1], tuple(out.shape)))
+    d = L.GxEmbed(C.sizeof(L.GxEmbed), L.OP_DEFAULT_STREAM, _float_type("weight", weight.dtype), _float_type("out", out.dtype),
+                  L.I32 if ids is None else _dtypes[ids.dtype], 0, tokens, weight.shape[0], weight.shape[1], stride, out_stride,
+                  None if ids is None else ids.data_ptr(), weight.data_ptr(), out.data_ptr(), None, 0, scale, 0)
+    _call(fn, handle, d, dev)
+    return out
+
+
+def embed_lookup(weight, ids, scale=1.0, dtype=None, out=None):
+    """out[i, :] = scale * weight[ids[i], :], rounded once to `dtype` (the weight's own by default).
+
+    weight [n_states, dim] and out [tokens, dim]: float32 / float16 / bfloat16 each, contiguous rows, any row stride of
+    at least dim.  ids [tokens], int32 (an observation row of a batch) or int64; an id outside the table gives zeros."""
+    torch = _torch()
+    _on_gpu("weight", weight)
+    _ids(ids, weight.device)
+    return _lookup(L.load().gx_embed_lookup, default_context(weight.device.index)._h, weight, ids, ids.shape[0], scale, dtype, out)
+
+
+def embed_obs(batch, weight, scale=1.0, dtype=None, out=None):
+    """DeviceBatch.embed_obs"""
+    _on_gpu("weight", weight)
+    if weight.device.index != batch.ctx.device:
+        raise ValueError("weight is on %s, the batch on GPU %d" % (weight.device, batch.ctx.device))
+    return _lookup(L.load().gx_vec_embed_obs, batch._h, weight, None, batch.n, scale, dtype, out)
+
+
+def embed_grad(grad, ids, n_states, scale=1.0, dtype=None, out=None, accumulate=False):
+    """embed_lookup's gradient with respect to its weight: table[v, :] = scale * sum of grad[i, :] over ids[i] == v.
+
+    grad [tokens, dim] and the result [n_states, dim]: float32 / float16 / bfloat16 each (`dtype`: float32 by default),
+    contiguous rows.  out: a tensor to write into, accumulate adds to what it holds.  Ids outside the table are left
+    out.  Equal calls give equal bits: the order of the additions depends on the ids alone."""
+    torch = _torch()
+    grad_stride = _matrix("grad", grad)
+    dev = grad.device
+    _ids(ids, dev)
+    if ids.shape[0] != grad.shape[0]:
+        raise ValueError("%d ids for %d rows of grad" % (ids.shape[0], grad.shape[0]))
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        if n_states < 1:
+            raise ValueError("n_states must be positive")
+        out = torch.empty(n_states, grad.shape[1], dtype=dtype or torch.float32, device=dev)
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError("out is %s, dtype says %s" % (out.dtype, dtype))
+    out_stride = _matrix("out", out, dev)
+    if tuple(out.shape) != (n_states, grad.shape[1]):
+        raise ValueError("out must have shape (%d, %d), not %s" % (n_states, grad.shape[1], tuple(out.shape)))
+    ctx = default_context(dev.index)
+    d = L.GxEmbed(C.sizeof(L.GxEmbed), L.OP_DEFAULT_STREAM, _float_type("out", out.dtype), _float_type("grad", grad.dtype),
+                  _dtypes[ids.dtype], 1 if accumulate else 0, ids.shape[0], n_states, grad.shape[1], out_stride, grad_stride,
+                  ids.data_ptr(), out.data_ptr(), grad.data_ptr(), None, 0, scale, 0)
+    ws = _workspace(torch, L.load().gx_embed_grad_workspace, ctx, d, dev)  # noqa: F841
+    _call(L.load().gx_embed_grad, ctx._h, d, dev)
+    return out

@@ -94,7 +94,8 @@ typedef enum gx_policy {
                                    (Spaces.Discrete.cs:18, Spaces.Box.cs:25-33) */
 } gx_policy;
 
-typedef enum gx_dtype { GX_F32 = 0, GX_F64 = 1, GX_I32 = 2, GX_U8 = 3 } gx_dtype;
+/* GX_F16, GX_BF16 and GX_I64 occur in the tensors a policy exchanges with the library (gx_sample, gx_embed) only */
+typedef enum gx_dtype { GX_F32 = 0, GX_F64 = 1, GX_I32 = 2, GX_U8 = 3, GX_F16 = 4, GX_BF16 = 5, GX_I64 = 6 } gx_dtype;
 
 typedef struct gx_ctx gx_ctx;
 typedef struct gx_vec gx_vec;
@@ -352,6 +353,96 @@ typedef struct gx_rows {
 /* All pointers are device pointers, 16-byte aligned.  Padding elements [num_envs, stride) of the
  * rows must be addressable; their values are ignored on input and unspecified on output. */
 int gx_rows_step(gx_ctx* ctx, const gx_rows* rows, int k_steps, void* stream);
+
+/* ---- between a policy on the GPU and a batch ------------------------------ */
+/* No counterpart in the reference, whose agents draw from ActionSpace.Sample() (Spaces.Discrete.cs:18) or on the host.
+ * The two ends of a Discrete interface on device memory the CALLER owns: actions drawn from a policy's logits, and the
+ * rows of an embedding table for Discrete observations, with the table's gradient.  The calls allocate nothing, keep
+ * nothing between calls and only enqueue on `stream`; scratch memory is the caller's (`workspace`), one per call in
+ * flight, so calls on different streams, threads or graphs do not meet.  They leave the calling thread's current device
+ * as they found it.  `stream` NULL is the context's stream, as everywhere else, or HIP's default stream with
+ * GX_OP_DEFAULT_STREAM. */
+typedef enum gx_op_flags { GX_OP_DEFAULT_STREAM = 1u } gx_op_flags;
+
+/* One action a row from logits[r * row_stride + a * col_stride], a = 0 .. n_actions-1, in the order of these steps:
+ *   a NaN logit reads as -inf (never drawn); m = the row's largest logit
+ *   temperature  weight w = exp((x - m) / T).  T = 0: the largest logit alone, the lowest index among equals
+ *   order        logits descending, equal logits by index ascending
+ *   top_k        the first k of the order (0: all)
+ *   top_p        of those, the shortest beginning of the order whose weight reaches p times theirs, at least one
+ *   min_p        of those, the ones with w >= min_p (the largest has w = 1)
+ *   draw         the first action IN INDEX ORDER at which the sum of the weights kept exceeds u times their total
+ * Weights and sums are binary64: the action is the one exact arithmetic gives but where u or p lies within a few 1e-12
+ * (relative) of a border.  A row of logits that are all -inf (every action masked): action -1, log-probability -inf;
+ * with +inf among the logits, those share the probability.  T = +inf is uniform over what is not -inf. */
+typedef struct gx_sample {
+  uint32_t struct_size;      /* sizeof(gx_sample) */
+  uint32_t op_flags;         /* gx_op_flags */
+  int32_t logits_dtype;      /* GX_F32, GX_F16 or GX_BF16 */
+  int32_t n_actions;         /* 1 .. 2^24 */
+  uint64_t rows;             /* 0 .. 2^40; 0: nothing happens */
+  int64_t row_stride;        /* elements, >= 0; {n, 1} is row-major, {1, stride} the layout of the batch's own rows */
+  int64_t col_stride;
+  const void* logits;        /* aligned to its element */
+  const float* u;            /* [rows] in [0, 1): the random numbers (below 0 and NaN read as 0, 1 and above as the
+                                largest below 1).  NULL in gx_vec_step_logits only: see there */
+  const float* temperature;  /* [rows], or NULL: temperature_all for every row; so the next three.  In the per-row forms
+                                T <= 0 and NaN read as 0, k <= 0 as all, p < 0 as 0, p NaN as 1, min_p NaN as 0, above 1
+                                as 1; the common values are checked instead: T >= 0, k >= 0, p and min_p in [0, 1] */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+  int32_t* actions;          /* out [rows] */
+  float* logprob;            /* out [rows], may be NULL: log of the probability the action was drawn with */
+  void* workspace;           /* 256-byte aligned device memory of gx_sample_workspace's size; may be NULL where that is 0 */
+  uint64_t workspace_bytes;
+} gx_sample;
+int gx_sample_workspace(gx_ctx* ctx, const gx_sample* sample, uint64_t* bytes);
+int gx_sample_logits(gx_ctx* ctx, const gx_sample* sample, void* stream);
+/* gx_sample_logits followed by gx_vec_step_device on its actions: one step of a batch whose policy's logits are on the
+ * device.  rows = num_envs, n_actions = gx_info.action_n (Box actions: GX_ERR_UNSUPPORTED), actions [gx_view.stride]
+ * and 16-byte aligned.  u = NULL draws u = w * 2^-32 from the batch's generator, w env i's word of the random policy's
+ * stream at this tick: for the classic-control and frame envs equal logits then give gx_vec_step_random's actions (the
+ * table-driven envs and Blackjack use that step's words inside Step, their random policy's actions are other ones).
+ * A graph that recorded a call replays its tick.  A row without an action (-1) is an action outside the space, treated
+ * as gx_vec_step_device treats one. */
+int gx_vec_step_logits(gx_vec* vec, const gx_sample* sample, void* stream);
+
+/* Embedding of Discrete observations: lookup  rows[i][:] = scale * table[ids[i]][:]
+ *                                     gradient table[v][:] = scale * (sum over the i with ids[i] = v) rows[i][:]
+ * (plus what table[v][:] held, with accumulate).  Arithmetic in binary32 (the gradient's long sums joined in binary64,
+ * always in the same order: equal calls give equal bits), rounded once to the type written.  An id outside
+ * 0 .. n_states-1 reads as a row of zeros and adds to no gradient. */
+typedef struct gx_embed {
+  uint32_t struct_size;      /* sizeof(gx_embed) */
+  uint32_t op_flags;         /* gx_op_flags */
+  int32_t table_dtype;       /* GX_F32, GX_F16 or GX_BF16 */
+  int32_t rows_dtype;        /* the same choice, independent */
+  int32_t ids_dtype;         /* GX_I32 or GX_I64 */
+  int32_t accumulate;        /* gradient only: non-zero adds to the table instead of overwriting all of it */
+  uint64_t tokens;           /* 0 .. 2^31-1 */
+  int64_t n_states;          /* 1 .. 2^31-1 rows of the table */
+  int64_t dim;               /* 1 .. 2^24 elements of a row */
+  int64_t table_stride;      /* elements between rows, >= dim */
+  int64_t rows_stride;
+  const void* ids;           /* [tokens] */
+  void* table;               /* read by the lookup, written by the gradient */
+  void* rows;                /* [tokens] rows: written by the lookup, read by the gradient (the output's gradient) */
+  void* workspace;           /* gradient only: as gx_sample's, of gx_embed_grad_workspace's size */
+  uint64_t workspace_bytes;
+  float scale;
+  int32_t reserved;
+} gx_embed;
+int gx_embed_lookup(gx_ctx* ctx, const gx_embed* embed, void* stream);
+int gx_embed_grad_workspace(gx_ctx* ctx, const gx_embed* embed, uint64_t* bytes);
+int gx_embed_grad(gx_ctx* ctx, const gx_embed* embed, void* stream);
+/* The lookup for the batch's current observations (gx_view.obs, int32): ids must be NULL, tokens = num_envs.
+ * GX_ERR_UNSUPPORTED for envs whose observation is not Discrete. */
+int gx_vec_embed_obs(gx_vec* vec, const gx_embed* embed, void* stream);
 
 /* ---- multi-GPU: episode statistics only -------------------------------- */
 /* unique_id: 128 bytes, produced by rank 0 with gx_comm_unique_id and passed

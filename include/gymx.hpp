@@ -212,6 +212,10 @@ class Batch {
   void Rollout(int k, int policy = GX_POLICY_RANDOM, const void* d_actions = nullptr, void* stream = nullptr) {
     check(gx_vec_rollout(h_, k, policy, d_actions, stream));
   }
+  // a policy on the GPU: a step with actions drawn from its logits, the rows of its embedding table for the current
+  // observations (struct_size is filled in here)
+  void StepLogits(gx_sample s, void* stream = nullptr) { s.struct_size = sizeof s; check(gx_vec_step_logits(h_, &s, stream)); }
+  void EmbedObs(gx_embed e, void* stream = nullptr) { e.struct_size = sizeof e; check(gx_vec_embed_obs(h_, &e, stream)); }
   gx_stats Stats() { gx_stats s{}; check(gx_vec_stats(h_, &s)); return s; }
   void Synchronize() { ctx_->Synchronize(); }
 
