@@ -2,9 +2,6 @@
 // of a policy's tensors, and folds over a wavefront in a fixed order.
 #pragma once
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-
 #include "gx_device.h"
 
 namespace gx {
@@ -40,18 +37,19 @@ struct EmbedArgs {
   float scale;
 };
 
+using f16 = _Float16;
+using bf16 = __bf16;
 __device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+__device__ __forceinline__ float to_f32(f16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return (float)v; }
+// to nearest, ties to even
+template <class T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 // the binary32 value as it stands: the compiler would fold a product before the conversion into v_fma_mixlo_f16, which
 // skips the product's own rounding and with it the agreement with the plain form
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) {
+template <> __device__ __forceinline__ f16 from_f32<f16>(float v) {
   asm("" : "+v"(v));
-  return __float2half(v);
+  return (f16)v;
 }
-template <> __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
 
 // butterfly folds: every lane ends with the same bits, whatever the values
 __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {

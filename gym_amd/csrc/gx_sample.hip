@@ -202,8 +202,8 @@ hipError_t launch_sample_logits(const SampleArgs& a, int dtype, void*, int num_c
   const uint64_t groups = (a.rows + kWavesPerGroup - 1) / kWavesPerGroup;
   const dim3 grid((unsigned)(groups < (uint64_t)num_cus * 64 ? groups : (uint64_t)num_cus * 64));
   if (dtype == GX_F32) hipLaunchKernelGGL(sample_kernel<float>, grid, dim3(64 * kWavesPerGroup), 0, stream, a);
-  else if (dtype == GX_F16) hipLaunchKernelGGL(sample_kernel<__half>, grid, dim3(64 * kWavesPerGroup), 0, stream, a);
-  else hipLaunchKernelGGL(sample_kernel<__hip_bfloat16>, grid, dim3(64 * kWavesPerGroup), 0, stream, a);
+  else if (dtype == GX_F16) hipLaunchKernelGGL(sample_kernel<f16>, grid, dim3(64 * kWavesPerGroup), 0, stream, a);
+  else hipLaunchKernelGGL(sample_kernel<bf16>, grid, dim3(64 * kWavesPerGroup), 0, stream, a);
   return hipGetLastError();
 }
 

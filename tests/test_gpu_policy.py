@@ -299,6 +299,14 @@ def test_grad_few_states_many_tokens():
         assert torch.equal(a, policy.embed_grad(grad, ids, states, scale=2.0))
 
 
+@pytest.mark.parametrize("tokens", [8191, 8192, 8193, 12_289, 70_000])
+def test_grad_sizes_of_the_sort(tokens):
+    """one workgroup's sort and the tiles', one to three digits"""
+    for states, dim in [(31, 5), (1023, 3), (1024, 3), (40_000, 2), (1_500_000, 1)]:
+        _, ids = make_embed(tokens, states, 1, F32, tokens)
+        check_grad(torch.randn(tokens, dim, generator=gen(states), device="cuda"), ids, states)
+
+
 def test_grad_sorted_equal_and_absent_ids():
     grad = torch.randn(4096, 20, generator=gen(1), device="cuda")
     for ids in (torch.arange(4096, device="cuda").int(), torch.arange(4095, -1, -1, device="cuda").int(), torch.full((4096,), 9, device="cuda").int(),
