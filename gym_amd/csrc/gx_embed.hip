@@ -19,54 +19,43 @@ template <class T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const 
 }
 template <class T, int N> __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) { __builtin_memcpy(p, &x, sizeof x); }
 
-// ------------------------------------------------------------------ lookup ---
-// Bound by the rows it writes.  Eight elements a lane (16 or 32 bytes each way); as many lanes a row as the row has
-// such pieces, so a wave takes several rows of a narrow table; kRowsAhead rows a lane, so that many gathers are in flight
-// behind the ids.
-constexpr int kPiece = 8, kRowsAhead = 4;
+// Rows are taken in pieces of kPiece elements, a lane each.  The last piece of a row that is no multiple of kPiece long
+// begins early, so that it is a whole one too; what it shares with the piece before it holds the same values twice in
+// the lookup and is written by the piece before it alone in the gradient.  Rows shorter than a piece go element by element.
+constexpr int kPiece = 8;
 
-template <class T, class R>
+// ------------------------------------------------------------------ lookup ---
+// Bound by the rows it writes.  As many lanes a row as the row has pieces, so a wave takes several rows of a narrow
+// table; kRowsAhead rows a lane, so that many gathers are in flight behind the ids.
+constexpr int kRowsAhead = 4;
+
+template <class T, class R, int N>
 __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_shift) {
   const int lanes = 1 << lanes_shift, rows = kBlock >> lanes_shift;
   const int lane = threadIdx.x & (lanes - 1), row = threadIdx.x >> lanes_shift;
+  const T* table = static_cast<const T*>(a.table);
+  R* out = static_cast<R*>(a.rows);
   for (uint64_t first = (uint64_t)blockIdx.x * (rows * kRowsAhead) + row; first < a.tokens; first += (uint64_t)gridDim.x * (rows * kRowsAhead)) {
-    const T* from[kRowsAhead];
+    int32_t id[kRowsAhead];
 #pragma unroll
     for (int k = 0; k < kRowsAhead; k++) {
       const uint64_t i = first + k * rows;
-      from[k] = nullptr;
-      if (i < a.tokens) {
-        const int64_t v = id_at(a, i);
-        if (v >= 0 && v < a.n_states) from[k] = static_cast<const T*>(a.table) + v * a.table_stride;
-      }
+      const int64_t v = i < a.tokens ? id_at(a, i) : -1;
+      id[k] = v >= 0 && v < a.n_states ? (int32_t)v : -1;
     }
-    for (int64_t c = (int64_t)lane * kPiece; c < a.dim; c += (int64_t)lanes * kPiece) {
-      if (c + kPiece <= a.dim) {
-        Pack<T, kPiece> x[kRowsAhead];
+    for (int64_t at = (int64_t)lane * N; at < a.dim; at += (int64_t)lanes * N) {
+      const int64_t c = at + N <= a.dim ? at : a.dim - N;
+      Pack<T, N> x[kRowsAhead];
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-          if (from[k]) x[k] = load_pack<T, kPiece>(from[k] + c);
-          else
+      for (int k = 0; k < kRowsAhead; k++) x[k] = load_pack<T, N>(table + (id[k] < 0 ? 0 : id[k]) * a.table_stride + c);
 #pragma unroll
-            for (int j = 0; j < kPiece; j++) x[k].v[j] = (T)0.0f;
-        }
+      for (int k = 0; k < kRowsAhead; k++) {
+        const uint64_t i = first + k * rows;
+        if (i >= a.tokens) continue;
+        Pack<R, N> y;
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-          const uint64_t i = first + k * rows;
-          if (i >= a.tokens) continue;
-          Pack<R, kPiece> y;
-#pragma unroll
-          for (int j = 0; j < kPiece; j++) y.v[j] = from_f32<R>(from[k] ? to_f32(x[k].v[j]) * a.scale : 0.0f);
-          store_pack(static_cast<R*>(a.rows) + (int64_t)i * a.rows_stride + c, y);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) {
-          const uint64_t i = first + k * rows;
-          if (i >= a.tokens) continue;
-          R* to = static_cast<R*>(a.rows) + (int64_t)i * a.rows_stride;
-          for (int64_t d = c; d < a.dim; d++) to[d] = from_f32<R>(from[k] ? to_f32(from[k][d]) * a.scale : 0.0f);
-        }
+        for (int j = 0; j < N; j++) y.v[j] = from_f32<R>(id[k] < 0 ? 0.0f : to_f32(x[k].v[j]) * a.scale);
+        store_pack(out + (int64_t)i * a.rows_stride + c, y);
       }
     }
   }
@@ -74,6 +63,7 @@ __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_s
 
 // ---------------------------------------------------------------- gradient ---
 // table[v] = scale * sum of the rows whose id is v, by sorted tokens:
+//   0  few tokens and states: a workgroup a state looks through all ids; nothing is sorted, one launch.
 //   1  the pairs (id, token) are sorted by id, stably, by counting: digits of up to 10 bits, least significant first.
 //      Ids outside the table sort behind everything as n_states.  One workgroup sorts up to kSortOne tokens alone, in
 //      LDS; more are cut into tiles: counts per tile and digit, running sums over the tiles, and the scatter.
@@ -84,25 +74,30 @@ __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_s
 //   3  runs over several chunks are joined from those parts, in order, in binary64.
 // Every addition's place follows from the ids alone: equal calls, equal bits.
 constexpr int kSortOne = 8192, kSortThreads = 1024;  // tokens one workgroup sorts alone
-constexpr int kTile = 4096;                          // tokens a workgroup of kBlock threads sorts, 16 a thread
+constexpr int kTile = 16384;                         // tokens of a tile, 16 a thread
 constexpr int kMaxDigit = 10;
 
+struct __align__(8) Pair { uint32_t key, token; };
+
 struct GradPlan {
+  bool direct;              // nothing is sorted
   int bits, passes, digit;  // of the key, how many digits, bits of each
   bool one;                 // one workgroup sorts
   uint32_t tiles;
   int lanes_shift;          // lanes of a group: 8 columns each
   int64_t col_tiles;        // groups a row takes
   uint32_t chunk, chunks;   // tokens of a chunk, number of chunks
-  size_t keys_a, keys_b, order_a, order_b, counts, totals, parts, bytes;  // offsets into the workspace
+  size_t pairs_a, pairs_b, counts, totals, parts, bytes;  // offsets into the workspace
 };
 
 // a launch has fewer than 2^32 threads: beyond that the workgroups go round
 unsigned capped(uint64_t blocks) { return (unsigned)(blocks < (1u << 22) ? blocks : 1u << 22); }
 
+// lanes of a row, as a power of two: a piece each, or an element each of a row shorter than a piece
 int shift_for(int64_t dim, int most) {
+  const int64_t pieces = dim >= kPiece ? (dim + kPiece - 1) / kPiece : dim;
   int s = 0;
-  while (s < most && ((int64_t)kPiece << s) < dim) s++;
+  while (s < most && (int64_t)1 << s < pieces) s++;
   return s;
 }
 
@@ -111,12 +106,15 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 GradPlan grad_plan(const EmbedArgs& a, int num_cus) {
   GradPlan p{};
   const uint64_t n = a.tokens;
+  // A wave looks at 64 ids a turn; 2^17 turns are a few microseconds of the whole card, three launches less.
+  p.direct = n > 0 && n <= 2048 && (uint64_t)a.n_states * (uint64_t)((a.dim + 63) / 64) * ((n + 63) / 64) <= (1u << 17);
+  if (p.direct) return p;
   p.bits = 64 - __builtin_clzll((unsigned long long)a.n_states);  // 0 .. n_states
   p.passes = (p.bits + kMaxDigit - 1) / kMaxDigit;
   p.digit = (p.bits + p.passes - 1) / p.passes;
   p.one = n <= (uint64_t)kSortOne;
   p.tiles = (uint32_t)((n + kTile - 1) / kTile);
-  const int64_t pieces = (a.dim + kPiece - 1) / kPiece;
+  const int64_t pieces = a.dim >= kPiece ? (a.dim + kPiece - 1) / kPiece : a.dim;
   p.lanes_shift = shift_for(a.dim, 6);
   p.col_tiles = (pieces + (1 << p.lanes_shift) - 1) >> p.lanes_shift;
   // chunks: enough lanes to fill the card (16 waves a compute unit), not fewer than 8 tokens, not more than 512
@@ -127,13 +125,9 @@ GradPlan grad_plan(const EmbedArgs& a, int num_cus) {
   p.chunks = (uint32_t)((n + p.chunk - 1) / p.chunk);
   size_t at = 0;
   auto take = [&](size_t bytes) { size_t o = at; at += up256(bytes); return o; };
-  p.keys_a = take(n * 4);
-  p.order_a = take(n * 4);
+  p.pairs_a = take(n * sizeof(Pair));
   if (!p.one) {
-    if (p.passes > 1) {
-      p.keys_b = take(n * 4);
-      p.order_b = take(n * 4);
-    }
+    if (p.passes > 1) p.pairs_b = take(n * sizeof(Pair));
     p.counts = take((size_t)p.tiles * 4 << p.digit);
     p.totals = take((size_t)4 << p.digit);
   }
@@ -170,7 +164,7 @@ __device__ __forceinline__ void clear_table(const EmbedArgs& a, uint64_t block, 
 }
 
 template <class T>
-__global__ void __launch_bounds__(kBlock) clear_kernel(EmbedArgs a) { clear_table<T>(a, blockIdx.x, gridDim.x); }
+__global__ void __launch_bounds__(kSortThreads) clear_kernel(EmbedArgs a) { clear_table<T>(a, blockIdx.x, gridDim.x); }
 
 // LDS of one wave: its operations are executed in order; this keeps the compiler to that order too
 __device__ __forceinline__ void wave_order() {
@@ -221,92 +215,76 @@ __device__ __forceinline__ void scan_lds(uint32_t* values, int n, uint32_t* sums
 // wave owning a contiguous stretch, so that (digit, wave) order keeps equal ids in the order of their tokens.
 constexpr int kOneBits = 5;
 template <class T>
-__global__ void __launch_bounds__(kSortThreads) sort_one_kernel(EmbedArgs a, int bits, uint32_t* keys_out, uint32_t* order_out) {
+__global__ void __launch_bounds__(kSortThreads) sort_one_kernel(EmbedArgs a, int bits, Pair* out) {
   if (blockIdx.x) {
     clear_table<T>(a, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
-  constexpr int kWaves = kSortThreads / 64, kEach = kSortOne / kSortThreads, kBins = 1 << kOneBits;
-  __shared__ uint32_t keys[kSortOne];
-  __shared__ uint16_t order[kSortOne];
+  constexpr int kWaves = kSortThreads / 64, kMost = kSortOne / kSortThreads, kBins = 1 << kOneBits;
+  __shared__ Pair pairs[kSortOne];
   __shared__ uint32_t counts[kBins * kWaves];  // [digit][wave]
   __shared__ uint32_t sums[kWaves];
+  static_assert(kBins * kWaves <= kSortThreads, "one counter a thread");
   const int n = (int)a.tokens, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t k[kEach], o[kEach];
-  // element e of this lane is token wave * 512 + e * 64 + lane
-  const int base = wave * (64 * kEach) + lane;
+  // element e of this lane is token (wave * each + e) * 64 + lane
+  const int each = (n + kSortThreads - 1) / kSortThreads, base = wave * each * 64 + lane;
+  Pair p[kMost];
 #pragma unroll
-  for (int e = 0; e < kEach; e++) {
+  for (int e = 0; e < kMost; e++) {
     const int i = base + e * 64;
-    k[e] = i < n ? sort_key(a, i) : 0xFFFFFFFFu;
-    o[e] = i;
+    if (e < each && i < n) p[e] = Pair{sort_key(a, i), (uint32_t)i};
   }
   for (int shift = 0; shift < bits; shift += kOneBits) {
     if (threadIdx.x < kBins * kWaves) counts[threadIdx.x] = 0;
-    static_assert(kBins * kWaves <= kSortThreads, "one counter a thread");
     __syncthreads();
-    uint32_t rank[kEach];
+    uint32_t rank[kMost];
 #pragma unroll
-    for (int e = 0; e < kEach; e++) {
+    for (int e = 0; e < kMost; e++) {
+      if (e >= each) break;
       const bool live = base + e * 64 < n;
-      const uint32_t d = (k[e] >> shift) & (kBins - 1);
-      const unsigned long long same = same_digit(d, kOneBits, __ballot(live));
-      uint32_t before = 0;
-      if (live) before = counts[d * kWaves + wave];
+      const uint32_t d = live ? (p[e].key >> shift) & (kBins - 1) : 0;
+      const unsigned long long same = same_digit(d, kOneBits, __ballot(live)), below = same & ((1ull << lane) - 1);
+      const uint32_t before = live ? counts[d * kWaves + wave] : 0;
       wave_order();
-      rank[e] = before + __popcll(same & ((1ull << lane) - 1));
-      if (live && (same & ((1ull << lane) - 1)) == 0) counts[d * kWaves + wave] = before + __popcll(same);
+      rank[e] = before + __popcll(below);
+      if (live && below == 0) counts[d * kWaves + wave] = before + __popcll(same);
       wave_order();
     }
     __syncthreads();
     scan_lds(counts, kBins * kWaves, sums);
 #pragma unroll
-    for (int e = 0; e < kEach; e++)
-      if (base + e * 64 < n) {
-        const uint32_t to = counts[((k[e] >> shift) & (kBins - 1)) * kWaves + wave] + rank[e];
-        keys[to] = k[e];
-        order[to] = (uint16_t)o[e];
-      }
+    for (int e = 0; e < kMost; e++)
+      if (e < each && base + e * 64 < n) pairs[counts[((p[e].key >> shift) & (kBins - 1)) * kWaves + wave] + rank[e]] = p[e];
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kEach; e++) {
-      const int i = base + e * 64;
-      if (i < n) {
-        k[e] = keys[i];
-        o[e] = order[i];
-      }
-    }
+    for (int e = 0; e < kMost; e++)
+      if (e < each && base + e * 64 < n) p[e] = pairs[base + e * 64];
     __syncthreads();
   }
 #pragma unroll
-  for (int e = 0; e < kEach; e++) {
-    const int i = base + e * 64;
-    if (i < n) {
-      keys_out[i] = k[e];
-      order_out[i] = o[e];
-    }
-  }
+  for (int e = 0; e < kMost; e++)
+    if (e < each && base + e * 64 < n) out[base + e * 64] = p[e];
 }
 
 // counts[digit][tile]; the workgroups behind the tiles clear the table
 template <class T>
-__global__ void __launch_bounds__(kBlock) count_kernel(EmbedArgs a, const uint32_t* keys, uint32_t tiles, int shift, int digit, uint32_t* counts) {
+__global__ void __launch_bounds__(kSortThreads) count_kernel(EmbedArgs a, const Pair* pairs, uint32_t tiles, int shift, int digit, uint32_t* counts) {
   if (blockIdx.x >= tiles) {
     clear_table<T>(a, blockIdx.x - tiles, gridDim.x - tiles);
     return;
   }
   __shared__ uint32_t bins[1 << kMaxDigit];
   const int n_bins = 1 << digit;
-  for (int b = threadIdx.x; b < n_bins; b += kBlock) bins[b] = 0;
+  for (int b = threadIdx.x; b < n_bins; b += kSortThreads) bins[b] = 0;
   __syncthreads();
-  const uint64_t first = (uint64_t)blockIdx.x * kTile;
+  const uint64_t first = (uint64_t)blockIdx.x * kTile + threadIdx.x;
 #pragma unroll
-  for (int e = 0; e < kTile / kBlock; e++) {
-    const uint64_t i = first + e * kBlock + threadIdx.x;
-    if (i < a.tokens) atomicAdd(&bins[((keys ? keys[i] : sort_key(a, i)) >> shift) & (n_bins - 1)], 1u);  // counts: order does not matter
+  for (int e = 0; e < kTile / kSortThreads; e++) {
+    const uint64_t i = first + e * kSortThreads;
+    if (i < a.tokens) atomicAdd(&bins[((pairs ? pairs[i].key : sort_key(a, i)) >> shift) & (n_bins - 1)], 1u);  // counts: order does not matter
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < n_bins; b += kBlock) counts[(size_t)b * tiles + blockIdx.x] = bins[b];
+  for (int b = threadIdx.x; b < n_bins; b += kSortThreads) counts[(size_t)b * tiles + blockIdx.x] = bins[b];
 }
 
 // running sums of one digit's counts over the tiles, in place, and the digit's total
@@ -348,48 +326,56 @@ __global__ void __launch_bounds__(kBlock) scan_tiles_kernel(uint32_t* counts, ui
   if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-__global__ void __launch_bounds__(kBlock) scatter_kernel(EmbedArgs a, const uint32_t* keys, const uint32_t* order, uint32_t tiles, int shift,
-                                                         int digit, const uint32_t* counts, const uint32_t* totals, uint32_t* keys_out,
-                                                         uint32_t* order_out) {
-  constexpr int kWaves = kBlock / 64, kEach = kTile / kBlock;
-  __shared__ uint32_t place[1 << kMaxDigit];                // where the digit's next token of this tile goes
-  __shared__ uint16_t seen[kWaves][1 << kMaxDigit];         // tokens of the digit in each wave's stretch
+__global__ void __launch_bounds__(kSortThreads) scatter_kernel(EmbedArgs a, const Pair* pairs, uint32_t tiles, int shift, int digit,
+                                                               const uint32_t* counts, const uint32_t* totals, Pair* out) {
+  constexpr int kWaves = kSortThreads / 64, kEach = kTile / kSortThreads;
+  __shared__ uint32_t place[1 << kMaxDigit];         // where the digit's next token of this tile goes
+  __shared__ uint16_t seen[kWaves][1 << kMaxDigit];  // tokens of the digit in each wave's stretch, then in those before it
   __shared__ uint32_t sums[kWaves];
   const int n_bins = 1 << digit, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int b = threadIdx.x; b < n_bins; b += kBlock) {
+  for (int b = threadIdx.x; b < n_bins; b += kSortThreads) {
     place[b] = totals[b];
 #pragma unroll
     for (int w = 0; w < kWaves; w++) seen[w][b] = 0;
   }
   __syncthreads();
   scan_lds(place, n_bins, sums);
-  for (int b = threadIdx.x; b < n_bins; b += kBlock) place[b] += counts[(size_t)b * tiles + blockIdx.x];
   const uint64_t first = (uint64_t)blockIdx.x * kTile + wave * (64 * kEach) + lane;
-  uint32_t k[kEach], rank[kEach];
+  Pair p[kEach];
+  uint32_t rank[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; e++) {
     const uint64_t i = first + e * 64;
-    const bool live = i < a.tokens;
-    k[e] = live ? (keys ? keys[i] : sort_key(a, i)) : 0;
-    const uint32_t d = (k[e] >> shift) & (n_bins - 1);
-    const unsigned long long same = same_digit(d, digit, __ballot(live));
-    uint32_t before = 0;
-    if (live) before = seen[wave][d];
+    if (i < a.tokens) p[e] = pairs ? pairs[i] : Pair{sort_key(a, i), (uint32_t)i};
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    const bool live = first + e * 64 < a.tokens;
+    const uint32_t d = live ? (p[e].key >> shift) & (n_bins - 1) : 0;
+    const unsigned long long same = same_digit(d, digit, __ballot(live)), below = same & ((1ull << lane) - 1);
+    const uint32_t before = live ? seen[wave][d] : 0;
     wave_order();
-    rank[e] = before + __popcll(same & ((1ull << lane) - 1));
-    if (live && (same & ((1ull << lane) - 1)) == 0) seen[wave][d] = (uint16_t)(before + __popcll(same));
+    rank[e] = before + __popcll(below);
+    if (live && below == 0) seen[wave][d] = (uint16_t)(before + __popcll(same));
     wave_order();
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < n_bins; b += kSortThreads) {
+    place[b] += counts[(size_t)b * tiles + blockIdx.x];
+    uint32_t run = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      const uint32_t here = seen[w][b];
+      seen[w][b] = (uint16_t)run;
+      run += here;
+    }
   }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < kEach; e++) {
-    const uint64_t i = first + e * 64;
-    if (i >= a.tokens) continue;
-    const uint32_t d = (k[e] >> shift) & (n_bins - 1);
-    uint32_t to = place[d] + rank[e];
-    for (int w = 0; w < wave; w++) to += seen[w][d];
-    keys_out[to] = k[e];
-    order_out[to] = order ? order[i] : (uint32_t)i;
+    if (first + e * 64 >= a.tokens) continue;
+    const uint32_t d = (p[e].key >> shift) & (n_bins - 1);
+    out[place[d] + seen[wave][d] + rank[e]] = p[e];
   }
 }
 
@@ -400,84 +386,88 @@ __device__ __forceinline__ void put(const EmbedArgs& a, uint32_t key, int64_t c,
   *to = from_f32<T>((float)(sum * (double)a.scale + old));
 }
 
-template <class T>
-__device__ __forceinline__ void put_piece(const EmbedArgs& a, uint32_t key, int64_t c, int cols, const float* sum) {
-  if (cols < kPiece) {
-    for (int j = 0; j < kPiece; j++)
-      if (j < cols) put<T>(a, key, c + j, (double)sum[j]);
+// columns c .. c + N - 1 of a state, but for the first `skip`, which the piece before holds too
+template <class T, int N>
+__device__ __forceinline__ void put_piece(const EmbedArgs& a, uint32_t key, int64_t c, int skip, const float* sum) {
+  T* to = static_cast<T*>(a.table) + (int64_t)key * a.table_stride + c;
+  if (skip) {
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (j >= skip) put<T>(a, key, c + j, (double)sum[j]);
     return;
   }
-  T* to = static_cast<T*>(a.table) + (int64_t)key * a.table_stride + c;
-  Pack<T, kPiece> y;
-  if (a.accumulate) y = load_pack<T, kPiece>(to);
+  Pack<T, N> y;
+  if (a.accumulate) y = load_pack<T, N>(to);
 #pragma unroll
-  for (int j = 0; j < kPiece; j++)
+  for (int j = 0; j < N; j++)
     y.v[j] = from_f32<T>((float)((double)sum[j] * (double)a.scale + (a.accumulate ? (double)to_f32(y.v[j]) : 0.0)));
   store_pack(to, y);
 }
 
-// One group of lanes a chunk and stretch of columns, eight columns a lane, eight rows in flight.
-template <class T, class R>
+// One group of lanes a chunk and stretch of columns, a piece a lane, eight rows in flight and the next eight's pairs.
+template <class T, class R, int N>
 __global__ void __launch_bounds__(kBlock) sum_kernel(EmbedArgs a, int lanes_shift, int64_t col_tiles, uint32_t chunk, uint32_t chunks,
-                                                     const uint32_t* keys, const uint32_t* order, float* parts) {
+                                                     const Pair* pairs, float* parts) {
   constexpr int kAhead = 8;
   const int lane = threadIdx.x & ((1 << lanes_shift) - 1);
   const uint64_t groups = (uint64_t)chunks * (uint64_t)col_tiles, stride = (uint64_t)gridDim.x * (kBlock >> lanes_shift);
   for (uint64_t group = (uint64_t)blockIdx.x * (kBlock >> lanes_shift) + (threadIdx.x >> lanes_shift); group < groups; group += stride) {
     const uint64_t which = group / (uint64_t)col_tiles;
-    const int64_t c = ((int64_t)(group % (uint64_t)col_tiles) << lanes_shift) * kPiece + (int64_t)lane * kPiece;
-    if (c >= a.dim) continue;
+    const int64_t at_col = ((int64_t)(group % (uint64_t)col_tiles) << lanes_shift) * N + (int64_t)lane * N;
+    if (at_col >= a.dim) continue;
+    const int64_t c = at_col + N <= a.dim ? at_col : a.dim - N;
+    const int skip = (int)(at_col - c);
+    const R* rows = static_cast<const R*>(a.rows) + c;
     const uint32_t first = (uint32_t)which * chunk;
     const uint32_t n = (uint32_t)a.tokens, end = n - first < chunk ? n : first + chunk;
-    const int cols = a.dim - c < kPiece ? (int)(a.dim - c) : kPiece;
-    float sum[kPiece] = {};
-    uint32_t current = keys[first];
+    float sum[N] = {};
+    Pair next[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) next[k] = pairs[first + k < end ? first + k : end - 1];
+    uint32_t current = next[0].key;
     // a part, not a run: entered from the chunk before, or left into the next one
-    bool entered = first > 0 && keys[first - 1] == current;
-    const bool left = end < n && keys[end] == keys[end - 1];
+    bool entered = first > 0 && pairs[first - 1].key == current;
+    const bool left = end < n && pairs[end].key == pairs[end - 1].key;
     auto flush = [&](bool part, int which_part) {
       if (current >= (uint32_t)a.n_states) return;
       if (!part) {
-        put_piece<T>(a, current, c, cols, sum);
+        put_piece<T, N>(a, current, c, skip, sum);
         return;
       }
-      float* to = parts + ((size_t)which * 2 + which_part) * (size_t)a.dim + c;
-      if (cols == kPiece) {
-        Pack<float, kPiece> y;
+      Pack<float, N> y;
 #pragma unroll
-        for (int j = 0; j < kPiece; j++) y.v[j] = sum[j];
-        store_pack(to, y);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kPiece; j++)
-          if (j < cols) to[j] = sum[j];
-      }
+      for (int j = 0; j < N; j++) y.v[j] = sum[j];
+      store_pack(parts + ((size_t)which * 2 + which_part) * (size_t)a.dim + c, y);
     };
     for (uint32_t at = first; at < end; at += kAhead) {
-      uint32_t key[kAhead];
-      Pack<R, kPiece> x[kAhead];
+      Pair p[kAhead];
+      Pack<R, N> x[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; k++) {
-        const uint32_t i = at + k < end ? at + k : end - 1;
-        key[k] = keys[i];
-        const R* from = static_cast<const R*>(a.rows) + (int64_t)order[i] * a.rows_stride + c;
-        if (cols == kPiece) x[k] = load_pack<R, kPiece>(from);
-        else
+        p[k] = next[k];
+        x[k] = load_pack<R, N>(rows + (int64_t)p[k].token * a.rows_stride);
+      }
 #pragma unroll
-          for (int j = 0; j < kPiece; j++) x[k].v[j] = j < cols ? from[j] : (R)0.0f;
+      for (int k = 0; k < kAhead; k++) next[k] = pairs[at + kAhead + k < end ? at + kAhead + k : end - 1];
+      if (at + kAhead <= end && p[kAhead - 1].key == current) {  // sorted: all eight
+#pragma unroll
+        for (int k = 0; k < kAhead; k++)
+#pragma unroll
+          for (int j = 0; j < N; j++) sum[j] += to_f32(x[k].v[j]);
+        continue;
       }
 #pragma unroll
       for (int k = 0; k < kAhead; k++) {
         if (at + k >= end) break;
-        if (key[k] != current) {
+        if (p[k].key != current) {
           flush(entered, 0);
           entered = false;
-          current = key[k];
+          current = p[k].key;
 #pragma unroll
-          for (int j = 0; j < kPiece; j++) sum[j] = 0.0f;
+          for (int j = 0; j < N; j++) sum[j] = 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < kPiece; j++) sum[j] += to_f32(x[k].v[j]);
+        for (int j = 0; j < N; j++) sum[j] += to_f32(x[k].v[j]);
       }
     }
     // the last run: a chunk that a single run enters and leaves has one part, the first
@@ -485,54 +475,123 @@ __global__ void __launch_bounds__(kBlock) sum_kernel(EmbedArgs a, int lanes_shif
   }
 }
 
-// The runs that leave the chunk they begin in: one workgroup each and 64 columns, 16 groups of 16 lanes that take every
-// 16th part, then added in order.
+// The runs that leave the chunk they begin in.  A workgroup looks at kJoinChunks chunks' ends, then takes the runs it
+// found one after the other, 32 columns: 64 groups of 8 lanes add every 64th part, then the groups' sums are added in order.
+constexpr int kJoinThreads = 512, kJoinChunks = 16, kJoinGroups = kJoinThreads / 8;
+
 template <class T>
-__global__ void __launch_bounds__(kBlock) join_kernel(EmbedArgs a, uint32_t chunk, uint32_t chunks, const uint32_t* keys, const float* parts) {
-  const uint32_t n = (uint32_t)a.tokens;
-  const uint64_t col_tiles = (uint64_t)(a.dim + 63) / 64;
-  __shared__ double sums[16][64];
-  const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  // (uniform over the workgroup throughout; the last chunk has nothing to join)
-  for (uint64_t b = blockIdx.x; b < (uint64_t)(chunks - 1) * col_tiles; b += gridDim.x) {
-    const uint32_t c0 = (uint32_t)(b / col_tiles);
-    const int64_t col0 = (int64_t)(b % col_tiles) * 64;
-    const uint32_t end = (c0 + 1) * chunk;
-    const uint32_t key = keys[end - 1];
-    if (keys[end] != key || key >= (uint32_t)a.n_states) continue;
-    if (c0 > 0 && keys[end - chunk - 1] == key) continue;  // began before this chunk
-    // the run's last token: the first place in [end, n) with a larger key, by halving
-    uint32_t lo = end, hi = n;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (keys[mid] == key) lo = mid + 1; else hi = mid;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(EmbedArgs a, uint32_t chunk, uint32_t chunks, const Pair* pairs, const float* parts) {
+  const uint32_t n = (uint32_t)a.tokens, blocks = (chunks - 1 + kJoinChunks - 1) / kJoinChunks;  // the last chunk has nothing to join
+  const uint64_t col_tiles = (uint64_t)(a.dim + 31) / 32;
+  __shared__ double sums[kJoinGroups][32];
+  __shared__ uint32_t found[kJoinChunks];  // the run's last chunk, 0: none begins here
+  const int group = threadIdx.x >> 3, lane = threadIdx.x & 7;
+  for (uint64_t b = blockIdx.x; b < (uint64_t)blocks * col_tiles; b += gridDim.x) {
+    const uint32_t c_first = (uint32_t)(b / col_tiles) * kJoinChunks;
+    const int64_t col0 = (int64_t)(b % col_tiles) * 32;
+    if (threadIdx.x < kJoinChunks) {
+      uint32_t last = 0;
+      const uint32_t c0 = c_first + threadIdx.x;
+      if (c0 < chunks - 1) {
+        const uint32_t end = (c0 + 1) * chunk;
+        const uint32_t key = pairs[end - 1].key;
+        const bool began = c0 == 0 || pairs[end - chunk - 1].key != key;  // in this chunk
+        if (pairs[end].key == key && key < (uint32_t)a.n_states && began) {
+          // the first place in [end, n) with a larger key, by halving
+          uint32_t lo = end, hi = n;
+          while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (pairs[mid].key == key) lo = mid + 1; else hi = mid;
+          }
+          last = (lo - 1) / chunk;
+        }
+      }
+      found[threadIdx.x] = last;
     }
-    const uint32_t last = (lo - 1) / chunk;  // chunks c0 .. last hold parts of it
-    const int64_t c = col0 + lane * 4;
-    const int cols = a.dim - c < 4 ? (int)(a.dim - c) : 4;  // may be <= 0
-    double sum[4] = {};
-    for (uint32_t k = c0 + group; k <= last; k += 16) {
-      const float* from = parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * (size_t)a.dim + c;
+    __syncthreads();
+    for (uint32_t f = 0; f < kJoinChunks; f++) {
+      const uint32_t c0 = c_first + f, last = found[f];
+      if (!last) continue;
+      const int64_t c = col0 + lane * 4;
+      const int cols = a.dim - c < 4 ? (int)(a.dim - c) : 4;  // may be <= 0
+      double sum[4] = {};
+      auto part = [&](uint32_t k) { return parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * (size_t)a.dim + c; };
+      uint32_t k = c0 + group;
       if (cols == 4) {
-        const Pack<float, 4> x = load_pack<float, 4>(from);
+        for (; k + 7 * kJoinGroups <= last; k += 8 * kJoinGroups) {
+          Pack<float, 4> x[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) sum[j] += (double)x.v[j];
-      } else {
+          for (int e = 0; e < 8; e++) x[e] = load_pack<float, 4>(part(k + e * kJoinGroups));
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum[j] += (double)x[e].v[j];
+        }
+      }
+      for (; k <= last; k += kJoinGroups) {
+        const float* from = part(k);
 #pragma unroll
         for (int j = 0; j < 4; j++)
           if (j < cols) sum[j] += (double)from[j];
       }
-    }
 #pragma unroll
-    for (int j = 0; j < 4; j++) sums[group][lane * 4 + j] = sum[j];
-    __syncthreads();
-    if (threadIdx.x < 64 && col0 + threadIdx.x < a.dim) {
-      double all = 0.0;
-#pragma unroll
-      for (int g = 0; g < 16; g++) all += sums[g][threadIdx.x];
-      put<T>(a, key, col0 + threadIdx.x, all);
+      for (int j = 0; j < 4; j++) sums[group][lane * 4 + j] = sum[j];
+      __syncthreads();
+      if (threadIdx.x < 32 && col0 + threadIdx.x < a.dim) {
+        double all = 0.0;
+#pragma unroll 8
+        for (int g = 0; g < kJoinGroups; g++) all += sums[g][threadIdx.x];
+        put<T>(a, pairs[(c0 + 1) * chunk - 1].key, col0 + threadIdx.x, all);
+      }
+      __syncthreads();
     }
     __syncthreads();
+  }
+}
+
+// Few tokens and states: a workgroup a state and 64 columns.  Its four waves look at 64 ids a turn; a wave's four groups
+// of 16 lanes take the hits among their 16 ids, four columns a lane.
+template <class T, class R>
+__global__ void __launch_bounds__(kBlock) direct_kernel(EmbedArgs a, int64_t col_tiles) {
+  __shared__ float sums[16][64];
+  const int64_t v = blockIdx.x / col_tiles, col0 = (blockIdx.x % col_tiles) * 64;
+  const int lane = threadIdx.x & 63, group = lane >> 4;
+  const int64_t c = col0 + (lane & 15) * 4;
+  float sum[4] = {};
+  bool any = false;
+  for (uint64_t at = threadIdx.x - lane; at < a.tokens; at += kBlock) {
+    const uint64_t i = at + lane;
+    const unsigned long long here = __ballot(i < a.tokens && id_at(a, i) == v);
+    any |= here != 0;
+    uint32_t hits = (uint32_t)(here >> (group * 16)) & 0xFFFFu;
+    while (__any(hits != 0)) {
+      float x[4][4];
+      bool in[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        in[k] = hits != 0;
+        const uint64_t t = at + group * 16 + (in[k] ? __ffs(hits) - 1 : 0);
+        hits &= hits - 1;
+        const R* from = static_cast<const R*>(a.rows) + (int64_t)t * a.rows_stride + c;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[k][j] = in[k] && c + j < a.dim ? to_f32(from[j]) : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (in[k]) sum[j] += x[k][j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) sums[threadIdx.x >> 4][(lane & 15) * 4 + j] = sum[j];
+  any = __syncthreads_or(any);
+  if (!any && a.accumulate) return;  // nothing to add: the state's row is left as it is
+  if (threadIdx.x < 64 && col0 + threadIdx.x < a.dim) {
+    double all = 0.0;
+#pragma unroll
+    for (int g = 0; g < 16; g++) all += (double)sums[g][threadIdx.x];
+    put<T>(a, (uint32_t)v, col0 + threadIdx.x, all);
   }
 }
 
@@ -550,7 +609,8 @@ hipError_t launch_embed_lookup(const EmbedArgs& a, int table, int rows, int, hip
   const dim3 grid(capped((a.tokens + each - 1) / each));
   return by_type(table, [&](auto t) {
     return by_type(rows, [&](auto r) {
-      hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(r)>), grid, dim3(kBlock), 0, stream, a, shift);
+      if (a.dim >= kPiece) hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(r), kPiece>), grid, dim3(kBlock), 0, stream, a, shift);
+      else hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(r), 1>), grid, dim3(kBlock), 0, stream, a, shift);
       return hipGetLastError();
     });
   });
@@ -561,55 +621,61 @@ size_t embed_grad_workspace(const EmbedArgs& a, int num_cus) { return grad_plan(
 hipError_t launch_embed_grad(const EmbedArgs& a, int table, int rows, void* workspace, int num_cus, hipStream_t stream) {
   const GradPlan p = grad_plan(a, num_cus);
   char* ws = static_cast<char*>(workspace);
-  // workgroups that clear the table: 16 KiB each, at most 16 a compute unit
+  if (p.direct) {
+    const int64_t col_tiles = (a.dim + 63) / 64;
+    return by_type(table, [&](auto t) {
+      return by_type(rows, [&](auto r) {
+        hipLaunchKernelGGL((direct_kernel<decltype(t), decltype(r)>), dim3((unsigned)(a.n_states * col_tiles)), dim3(kBlock), 0, stream, a, col_tiles);
+        return hipGetLastError();
+      });
+    });
+  }
+  // workgroups that clear the table: 64 KiB each, at most 4 a compute unit
   const uint64_t clear_bytes = a.accumulate ? 0 : (uint64_t)a.n_states * (uint64_t)a.dim * (table == GX_F32 ? 4 : 2);
-  uint64_t clear = (clear_bytes + 16383) / 16384;
-  if (clear > (uint64_t)num_cus * 16) clear = (uint64_t)num_cus * 16;
+  uint64_t clear = (clear_bytes + 65535) / 65536;
+  if (clear > (uint64_t)num_cus * 4) clear = (uint64_t)num_cus * 4;
   if (a.tokens == 0) {
     if (!clear) return hipSuccess;
     return by_type(table, [&](auto t) {
-      hipLaunchKernelGGL(clear_kernel<decltype(t)>, dim3((unsigned)clear), dim3(kBlock), 0, stream, a);
+      hipLaunchKernelGGL(clear_kernel<decltype(t)>, dim3((unsigned)clear), dim3(kSortThreads), 0, stream, a);
       return hipGetLastError();
     });
   }
-  uint32_t* keys = reinterpret_cast<uint32_t*>(ws + p.keys_a);
-  uint32_t* order = reinterpret_cast<uint32_t*>(ws + p.order_a);
+  Pair* pairs = reinterpret_cast<Pair*>(ws + p.pairs_a);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   return by_type(table, [&](auto t) -> hipError_t {
     using T = decltype(t);
     if (p.one) {
-      hipLaunchKernelGGL(sort_one_kernel<T>, dim3((unsigned)(1 + (clear + 3) / 4)), dim3(kSortThreads), 0, stream, a, p.bits, keys, order);
+      hipLaunchKernelGGL(sort_one_kernel<T>, dim3((unsigned)(1 + clear)), dim3(kSortThreads), 0, stream, a, p.bits, pairs);
     } else {
       uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
       uint32_t* totals = reinterpret_cast<uint32_t*>(ws + p.totals);
-      uint32_t* other_keys = reinterpret_cast<uint32_t*>(ws + p.keys_b);
-      uint32_t* other_order = reinterpret_cast<uint32_t*>(ws + p.order_b);
-      // the last pass ends in (keys, order)
-      const uint32_t *from_keys = nullptr, *from_order = nullptr;
+      const Pair* from = nullptr;
       for (int pass = 0; pass < p.passes; pass++) {
-        const bool to_a = (p.passes - 1 - pass) % 2 == 0;
-        uint32_t* to_keys = to_a ? keys : other_keys;
-        uint32_t* to_order = to_a ? order : other_order;
+        // the last pass ends in `pairs`
+        Pair* to = (p.passes - 1 - pass) % 2 == 0 ? pairs : reinterpret_cast<Pair*>(ws + p.pairs_b);
         const dim3 tiles(p.tiles), first((unsigned)(p.tiles + (pass == 0 ? clear : 0)));
-        hipLaunchKernelGGL(count_kernel<T>, first, dim3(kBlock), 0, stream, a, from_keys, p.tiles, pass * p.digit, p.digit, counts);
+        hipLaunchKernelGGL(count_kernel<T>, first, dim3(kSortThreads), 0, stream, a, from, p.tiles, pass * p.digit, p.digit, counts);
         hipLaunchKernelGGL(scan_tiles_kernel, dim3(1u << p.digit), dim3(kBlock), 0, stream, counts, p.tiles, totals);
-        hipLaunchKernelGGL(scatter_kernel, tiles, dim3(kBlock), 0, stream, a, from_keys, from_order, p.tiles, pass * p.digit, p.digit,
-                           counts, totals, to_keys, to_order);
-        from_keys = to_keys;
-        from_order = to_order;
+        hipLaunchKernelGGL(scatter_kernel, tiles, dim3(kSortThreads), 0, stream, a, from, p.tiles, pass * p.digit, p.digit, counts, totals, to);
+        from = to;
       }
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const uint64_t groups = (uint64_t)p.chunks * (uint64_t)p.col_tiles, per_block = kBlock >> p.lanes_shift;
+    const dim3 grid(capped((groups + per_block - 1) / per_block));
     e = by_type(rows, [&](auto r) {
-      hipLaunchKernelGGL((sum_kernel<T, decltype(r)>), dim3(capped((groups + per_block - 1) / per_block)), dim3(kBlock), 0, stream, a,
-                         p.lanes_shift, p.col_tiles, p.chunk, p.chunks, keys, order, parts);
+      using R = decltype(r);
+      if (a.dim >= kPiece)
+        hipLaunchKernelGGL((sum_kernel<T, R, kPiece>), grid, dim3(kBlock), 0, stream, a, p.lanes_shift, p.col_tiles, p.chunk, p.chunks, pairs, parts);
+      else
+        hipLaunchKernelGGL((sum_kernel<T, R, 1>), grid, dim3(kBlock), 0, stream, a, p.lanes_shift, p.col_tiles, p.chunk, p.chunks, pairs, parts);
       return hipGetLastError();
     });
     if (e != hipSuccess || p.chunks < 2) return e;
-    hipLaunchKernelGGL(join_kernel<T>, dim3(capped((uint64_t)(p.chunks - 1) * ((uint64_t)(a.dim + 63) / 64))), dim3(kBlock), 0, stream, a, p.chunk, p.chunks,
-                       keys, parts);
+    const uint64_t joins = (uint64_t)((p.chunks - 1 + kJoinChunks - 1) / kJoinChunks) * ((uint64_t)(a.dim + 31) / 32);
+    hipLaunchKernelGGL(join_kernel<T>, dim3(capped(joins)), dim3(kJoinThreads), 0, stream, a, p.chunk, p.chunks, pairs, parts);
     return hipGetLastError();
   });
 }
