@@ -19,6 +19,16 @@ template <class T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const 
 }
 template <class T, int N> __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) { __builtin_memcpy(p, &x, sizeof x); }
 
+// past the caches: nothing reads it soon
+template <class T, int N> __device__ __forceinline__ void stream_pack(T* p, const Pack<T, N>& x) {
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+  static_assert(sizeof x % 16 == 0, "whole 16-byte words");
+  Words w[sizeof x / 16];
+  __builtin_memcpy(w, &x, sizeof x);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof x / 16); i++) __builtin_nontemporal_store(w[i], reinterpret_cast<Words*>(p) + i);
+}
+
 // Rows are taken in pieces of kPiece elements, a lane each.  The last piece of a row that is no multiple of kPiece long
 // begins early, so that it is a whole one too; what it shares with the piece before it holds the same values twice in
 // the lookup and is written by the piece before it alone in the gradient.  Rows shorter than a piece go element by element.
@@ -27,9 +37,13 @@ constexpr int kPiece = 8;
 // ------------------------------------------------------------------ lookup ---
 // Bound by the rows it writes.  As many lanes a row as the row has pieces, so a wave takes several rows of a narrow
 // table; kRowsAhead rows a lane, so that many gathers are in flight behind the ids.
-constexpr int kRowsAhead = 4;
+constexpr int kRowsAhead = 2;
+// Outputs larger than the card's second-level caches (8 x 4 MiB) are written past them: 4 Mi rows of 128 bf16 (1 GiB)
+// 171 us so, 251 through the caches; 8 191 rows of 4 095 (67 MB) 24.2 and 25.1.  Four rows ahead: 174 and 25.0.  Smaller
+// outputs stay where their reader finds them.
+constexpr uint64_t kStreamBytes = 32u << 20;
 
-template <class T, class R, int N>
+template <class T, class R, int N, bool STREAM>
 __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_shift) {
   const int lanes = 1 << lanes_shift, rows = kBlock >> lanes_shift;
   const int lane = threadIdx.x & (lanes - 1), row = threadIdx.x >> lanes_shift;
@@ -55,7 +69,9 @@ __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_s
         Pack<R, N> y;
 #pragma unroll
         for (int j = 0; j < N; j++) y.v[j] = from_f32<R>(id[k] < 0 ? 0.0f : to_f32(x[k].v[j]) * a.scale);
-        store_pack(out + (int64_t)i * a.rows_stride + c, y);
+        R* to = out + (int64_t)i * a.rows_stride + c;
+        if constexpr (STREAM) stream_pack(to, y);
+        else store_pack(to, y);
       }
     }
   }
@@ -475,73 +491,100 @@ __global__ void __launch_bounds__(kBlock) sum_kernel(EmbedArgs a, int lanes_shif
   }
 }
 
-// The runs that leave the chunk they begin in.  A workgroup looks at kJoinChunks chunks' ends, then takes the runs it
-// found one after the other, 32 columns: 64 groups of 8 lanes add every 64th part, then the groups' sums are added in order.
-constexpr int kJoinThreads = 512, kJoinChunks = 16, kJoinGroups = kJoinThreads / 8;
+// The runs that leave the chunk they begin in: a wave looks at one chunk's end and, if such a run begins there, adds up its
+// parts, 256 columns, four a lane.  Runs of more than kJoinAlone parts are added by the whole workgroup.
+constexpr int kJoinWaves = 8, kJoinAlone = 32;
 
 template <class T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(EmbedArgs a, uint32_t chunk, uint32_t chunks, const Pair* pairs, const float* parts) {
-  const uint32_t n = (uint32_t)a.tokens, blocks = (chunks - 1 + kJoinChunks - 1) / kJoinChunks;  // the last chunk has nothing to join
-  const uint64_t col_tiles = (uint64_t)(a.dim + 31) / 32;
-  __shared__ double sums[kJoinGroups][32];
-  __shared__ uint32_t found[kJoinChunks];  // the run's last chunk, 0: none begins here
-  const int group = threadIdx.x >> 3, lane = threadIdx.x & 7;
-  for (uint64_t b = blockIdx.x; b < (uint64_t)blocks * col_tiles; b += gridDim.x) {
-    const uint32_t c_first = (uint32_t)(b / col_tiles) * kJoinChunks;
-    const int64_t col0 = (int64_t)(b % col_tiles) * 32;
-    if (threadIdx.x < kJoinChunks) {
-      uint32_t last = 0;
-      const uint32_t c0 = c_first + threadIdx.x;
-      if (c0 < chunks - 1) {
-        const uint32_t end = (c0 + 1) * chunk;
-        const uint32_t key = pairs[end - 1].key;
-        const bool began = c0 == 0 || pairs[end - chunk - 1].key != key;  // in this chunk
-        if (pairs[end].key == key && key < (uint32_t)a.n_states && began) {
-          // the first place in [end, n) with a larger key, by halving
-          uint32_t lo = end, hi = n;
-          while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (pairs[mid].key == key) lo = mid + 1; else hi = mid;
-          }
-          last = (lo - 1) / chunk;
-        }
-      }
-      found[threadIdx.x] = last;
-    }
-    __syncthreads();
-    for (uint32_t f = 0; f < kJoinChunks; f++) {
-      const uint32_t c0 = c_first + f, last = found[f];
-      if (!last) continue;
-      const int64_t c = col0 + lane * 4;
-      const int cols = a.dim - c < 4 ? (int)(a.dim - c) : 4;  // may be <= 0
-      double sum[4] = {};
-      auto part = [&](uint32_t k) { return parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * (size_t)a.dim + c; };
-      uint32_t k = c0 + group;
-      if (cols == 4) {
-        for (; k + 7 * kJoinGroups <= last; k += 8 * kJoinGroups) {
-          Pack<float, 4> x[8];
+__global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(EmbedArgs a, int lanes_shift, uint32_t chunk, uint32_t chunks, const Pair* pairs,
+                                                               const float* parts) {
+  __shared__ double sums[kJoinWaves][256];
+  __shared__ uint32_t long_last[kJoinWaves];  // the run's last chunk, 0: none for the workgroup
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int group = lane >> lanes_shift, n_groups = 64 >> lanes_shift;
+  const uint64_t col_tiles = (uint64_t)(a.dim + 255) / 256, units = (uint64_t)(chunks - 1) * col_tiles;  // the last chunk has nothing to join
+  // parts first, first + step, .. last of the run that begins in c0, in four columns from c on
+  auto add_parts = [&](uint32_t c0, uint32_t first, uint32_t last, uint32_t step, int64_t c, double* sum) {
+    const int cols = a.dim - c < 4 ? (int)(a.dim - c) : 4;  // may be <= 0
+    auto part = [&](uint32_t k) { return parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * (size_t)a.dim + c; };
+    uint32_t k = first;
+    if (cols == 4) {
+      for (; k <= last; k += 8 * step) {
+        Pack<float, 4> x[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) x[e] = load_pack<float, 4>(part(k + e * kJoinGroups));
+        for (int e = 0; e < 8; e++) x[e] = load_pack<float, 4>(part(k + e * step <= last ? k + e * step : last));
 #pragma unroll
-          for (int e = 0; e < 8; e++)
+        for (int e = 0; e < 8; e++)
+          if (k + e * step <= last)
 #pragma unroll
             for (int j = 0; j < 4; j++) sum[j] += (double)x[e].v[j];
-        }
       }
-      for (; k <= last; k += kJoinGroups) {
-        const float* from = part(k);
+    } else {
+      for (; k <= last; k += step)
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          if (j < cols) sum[j] += (double)from[j];
-      }
+          if (j < cols) sum[j] += (double)part(k)[j];
+    }
+    for (int d = 1 << lanes_shift; d < 64; d <<= 1)
 #pragma unroll
-      for (int j = 0; j < 4; j++) sums[group][lane * 4 + j] = sum[j];
+      for (int j = 0; j < 4; j++) sum[j] += shfl_xor_f64(sum[j], d);
+  };
+  for (uint64_t u0 = (uint64_t)blockIdx.x * kJoinWaves; u0 < units; u0 += (uint64_t)gridDim.x * kJoinWaves) {
+    const uint64_t u = u0 + wave;
+    const uint32_t c0 = (uint32_t)(u / col_tiles);
+    const int64_t col0 = (int64_t)(u % col_tiles) * 256;
+    uint32_t last = 0, key = 0;
+    if (u < units) {
+      // the last token of the chunk, the one after it, the last of the chunk before
+      const uint32_t end = (c0 + 1) * chunk;
+      const uint32_t at = lane == 0 ? end - 1 : (lane == 1 ? end : (c0 ? end - chunk - 1 : 0));
+      const uint32_t k = pairs[at].key;
+      key = __shfl(k, 0, 64);
+      const bool begins = (c0 == 0 || __shfl(k, 2, 64) != key) && __shfl(k, 1, 64) == key && key < (uint32_t)a.n_states;
+      if (begins) {
+        // the last chunk that begins with the key: 64 chunks at a time, then 64 steps through what is left, finer and finer
+        auto begins_with_key = [&](uint64_t c) { return c < chunks && pairs[c * chunk].key == key; };
+        last = c0 + 1;
+        int ones = __popcll(__ballot(begins_with_key((uint64_t)last + 1 + lane)));
+        last += ones;
+        if (ones == 64) {
+          uint64_t stride = chunks;
+          do {
+            stride = (stride + 63) / 64;
+            ones = __popcll(__ballot(begins_with_key(last + (lane + 1) * stride)));
+            last += (uint32_t)(ones * stride);
+          } while (stride > 1);
+        }
+      }
+    }
+    const bool alone = last - c0 < (uint32_t)kJoinAlone;
+    if (lane == 0) long_last[wave] = last && !alone ? last : 0;
+    if (last && alone) {
+      const int64_t c = col0 + (int64_t)(lane & ((1 << lanes_shift) - 1)) * 4;
+      double sum[4] = {};
+      add_parts(c0, c0 + group, last, n_groups, c, sum);
+      if (group == 0)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (c + j < a.dim) put<T>(a, key, c + j, sum[j]);
+    }
+    __syncthreads();
+    for (int w = 0; w < kJoinWaves; w++) {
+      const uint32_t long_end = long_last[w];
+      if (!long_end) continue;
+      const uint32_t l0 = (uint32_t)((u0 + w) / col_tiles);
+      const int64_t base = (int64_t)((u0 + w) % col_tiles) * 256, c = base + (int64_t)(lane & ((1 << lanes_shift) - 1)) * 4;
+      double sum[4] = {};
+      add_parts(l0, l0 + wave * n_groups + group, long_end, kJoinWaves * n_groups, c, sum);
+      if (group == 0)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sums[wave][lane * 4 + j] = sum[j];
       __syncthreads();
-      if (threadIdx.x < 32 && col0 + threadIdx.x < a.dim) {
+      if (threadIdx.x < (4u << lanes_shift) && base + threadIdx.x < a.dim) {
         double all = 0.0;
-#pragma unroll 8
-        for (int g = 0; g < kJoinGroups; g++) all += sums[g][threadIdx.x];
-        put<T>(a, pairs[(c0 + 1) * chunk - 1].key, col0 + threadIdx.x, all);
+#pragma unroll
+        for (int q = 0; q < kJoinWaves; q++) all += sums[q][threadIdx.x];
+        put<T>(a, pairs[(l0 + 1) * chunk - 1].key, base + threadIdx.x, all);
       }
       __syncthreads();
     }
@@ -609,8 +652,12 @@ hipError_t launch_embed_lookup(const EmbedArgs& a, int table, int rows, int, hip
   const dim3 grid(capped((a.tokens + each - 1) / each));
   return by_type(table, [&](auto t) {
     return by_type(rows, [&](auto r) {
-      if (a.dim >= kPiece) hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(r), kPiece>), grid, dim3(kBlock), 0, stream, a, shift);
-      else hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(r), 1>), grid, dim3(kBlock), 0, stream, a, shift);
+      using T = decltype(t);
+      using R = decltype(r);
+      const bool stream_out = a.tokens * (uint64_t)a.dim * sizeof(R) > kStreamBytes;
+      if (a.dim < kPiece) hipLaunchKernelGGL((lookup_kernel<T, R, 1, false>), grid, dim3(kBlock), 0, stream, a, shift);
+      else if (stream_out) hipLaunchKernelGGL((lookup_kernel<T, R, kPiece, true>), grid, dim3(kBlock), 0, stream, a, shift);
+      else hipLaunchKernelGGL((lookup_kernel<T, R, kPiece, false>), grid, dim3(kBlock), 0, stream, a, shift);
       return hipGetLastError();
     });
   });
@@ -674,8 +721,11 @@ hipError_t launch_embed_grad(const EmbedArgs& a, int table, int rows, void* work
       return hipGetLastError();
     });
     if (e != hipSuccess || p.chunks < 2) return e;
-    const uint64_t joins = (uint64_t)((p.chunks - 1 + kJoinChunks - 1) / kJoinChunks) * ((uint64_t)(a.dim + 31) / 32);
-    hipLaunchKernelGGL(join_kernel<T>, dim3(capped(joins)), dim3(kJoinThreads), 0, stream, a, p.chunk, p.chunks, pairs, parts);
+    int join_shift = 0;  // lanes a row at four columns each
+    while (join_shift < 6 && ((int64_t)4 << join_shift) < a.dim) join_shift++;
+    const uint64_t units = (uint64_t)(p.chunks - 1) * ((uint64_t)(a.dim + 255) / 256);
+    hipLaunchKernelGGL(join_kernel<T>, dim3(capped((units + kJoinWaves - 1) / kJoinWaves)), dim3(64 * kJoinWaves), 0, stream, a, join_shift,
+                       p.chunk, p.chunks, pairs, parts);
     return hipGetLastError();
   });
 }

@@ -243,6 +243,13 @@ def test_lookup(dtype, out):
     assert torch.all(got[:3] == 0) and torch.equal(got[3], w[0])
 
 
+def test_lookup_of_outputs_past_the_caches():
+    for dtype, out, tokens, dim in [(BF16, BF16, 70_001, 257), (F32, F32, 33_333, 260), (BF16, F32, 1_100_003, 9)]:
+        w, ids = make_embed(tokens, 100, dim, dtype, dim)
+        got = policy.embed_lookup(w, ids, scale=3.0, dtype=out)
+        assert got.numel() * got.element_size() > 32 << 20 and torch.equal(got, want_lookup(w, ids, 3.0, out))
+
+
 @pytest.mark.parametrize("dim", [1, 3, 8, 64, 100, 1001])
 def test_lookup_strides(dim):
     for dtype in (F32, BF16):
