@@ -1410,7 +1410,9 @@ int sample_args(const char* who, const gx_sample* s, bool draws, SampleArgs* a) 
   a->logits = s->logits; a->rows = s->rows; a->row_stride = s->row_stride; a->col_stride = s->col_stride;
   a->n = s->n_actions;
   a->u = s->u; a->temperature = s->temperature; a->top_k = s->top_k; a->top_p = s->top_p; a->min_p = s->min_p;
-  a->temperature_all = s->temperature_all; a->top_k_all = s->top_k_all; a->top_p_all = s->top_p_all; a->min_p_all = s->min_p_all;
+  a->greedy_all = !s->temperature && s->temperature_all == 0.0f;
+  a->inv_t_all = s->temperature || a->greedy_all ? 1.0 : 1.0 / (double)s->temperature_all;
+  a->top_k_all = s->top_k_all; a->top_p_all = s->top_p_all; a->min_p_all = s->min_p_all;
   a->actions = s->actions; a->logprob = s->logprob;
   return GX_OK;
 }

@@ -13,7 +13,9 @@ struct SampleArgs {
   int64_t row_stride, col_stride;
   int32_t n;
   int32_t top_k_all;
-  float temperature_all, top_p_all, min_p_all;
+  float top_p_all, min_p_all;
+  int32_t greedy_all;  // the common temperature is 0
+  double inv_t_all;    // 1 / the common temperature
   const float* u;  // nullptr: from the generator, see u_of
   const float* temperature;
   const int32_t* top_k;
