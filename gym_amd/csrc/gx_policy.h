@@ -53,19 +53,53 @@ template <> __device__ __forceinline__ f16 from_f32<f16>(float v) {
   return (f16)v;
 }
 
-// butterfly folds: every lane ends with the same bits, whatever the values
+// ---- lanes of a wavefront ----
+// the value of the lane whose number differs in the bits of M
+template <int M> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+  static_assert(M == 1 || M == 2 || M == 4 || M == 8 || M == 16 || M == 32, "one bit");
+  if constexpr (M == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);        // quad_perm 1 0 3 2
+  else if constexpr (M == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);   // quad_perm 2 3 0 1
+  else if constexpr (M == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, true);  // row_ror 8, of 16
+  else if constexpr (M == 32) return (uint32_t)__shfl_xor((int)v, 32, 64);
+  else return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, M << 10 | 0x1F);
+}
+// running sums over 16 or 64 lanes, the lane's own included.  Within a row of 16 by shifts that bring zeros in; then the
+// last lane of a row into the next (rows 1 and 3), and lane 31 into the upper half.
+template <int CTRL, int ROWS> __device__ __forceinline__ double moved_f64(double v) {
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, true);
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, true);
+  return __hiloint2double(hi, lo);
+}
+template <int G> __device__ __forceinline__ double running_sum(double v) {
+  v += moved_f64<0x111, 0xF>(v);
+  v += moved_f64<0x112, 0xF>(v);
+  v += moved_f64<0x114, 0xF>(v);
+  v += moved_f64<0x118, 0xF>(v);
+  if constexpr (G == 64) {
+    v += moved_f64<0x142, 0xA>(v);  // row_bcast 15
+    v += moved_f64<0x143, 0xC>(v);  // row_bcast 31
+  }
+  return v;
+}
+template <int G> __device__ __forceinline__ int running_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  if constexpr (G == 64) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);
+  }
+  return v;
+}
 __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
   return __hiloint2double(__shfl_xor(__double2hiint(v), mask, 64), __shfl_xor(__double2loint(v), mask, 64));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += shfl_xor_f64(v, d);
-  return v;
+__device__ __forceinline__ double shfl_f64(double v, int lane, int width = 64) {
+  return __hiloint2double(__shfl(__double2hiint(v), lane, width), __shfl(__double2loint(v), lane, width));
 }
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-  return v;
-}
+// of the wave, in every lane: the same order of additions, so the same bits, in each
+__device__ __forceinline__ double wave_sum(double v) { return shfl_f64(running_sum<64>(v), 63); }
+__device__ __forceinline__ int wave_sum(int v) { return __shfl(running_sum<64>(v), 63, 64); }
 
 }  // namespace gx

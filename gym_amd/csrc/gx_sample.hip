@@ -13,6 +13,12 @@
 #include "gx_launch.h"
 #include "gx_policy.h"
 
+#ifndef GX_WB
+#define GX_WB 1024
+#endif
+#ifndef GX_AHEAD
+#define GX_AHEAD 4
+#endif
 namespace gx {
 
 namespace {
@@ -41,6 +47,7 @@ template <class T, int N> __device__ __forceinline__ void load_logits(const T* p
 // A row's parameters, read as the interface says.
 struct RowParams {
   double inv_t;  // 1 / T
+  double per_t;  // log2(e) / T
   double p, q;   // p = 1: no cut
   int32_t k;     // 1 .. n
   double u;
@@ -56,6 +63,7 @@ template <bool CUT> __device__ __forceinline__ RowParams row_params(const Sample
     greedy = !(t > 0.0f);  // T = 0, and what reads as it
     s.inv_t = greedy ? 1.0 : 1.0 / (double)t;
   }
+  s.per_t = s.inv_t * 1.4426950408889634;
   s.k = a.n;
   s.p = 1.0;
   s.q = 0.0;
@@ -77,22 +85,20 @@ template <bool CUT> __device__ __forceinline__ RowParams row_params(const Sample
   return s;
 }
 
-// exp(z), z <= 0, to 1e-14 relative: z = k ln 2 + f, |f| <= ln 2 / 2, the series to f^11 / 11!
-__device__ __forceinline__ double exp_neg(double z) {
-  z = fmax(z, -746.0);  // exp is 0 there
-  const double k = rint(z * 1.4426950408889634);
-  double f = __builtin_fma(k, -0x1.62e42fefa39efp-1, z);  // k < 2^11: the product's error stays below 2^-43, of z's 2^-44
-  double e = 1.0 / 39916800.0;
-  e = __builtin_fma(e, f, 1.0 / 3628800.0);
-  e = __builtin_fma(e, f, 1.0 / 362880.0);
-  e = __builtin_fma(e, f, 1.0 / 40320.0);
-  e = __builtin_fma(e, f, 1.0 / 5040.0);
-  e = __builtin_fma(e, f, 1.0 / 720.0);
-  e = __builtin_fma(e, f, 1.0 / 120.0);
-  e = __builtin_fma(e, f, 1.0 / 24.0);
-  e = __builtin_fma(e, f, 1.0 / 6.0);
-  e = __builtin_fma(e, f, 0.5);
-  e = __builtin_fma(e, f, 1.0);
+// 2^t, t <= 0: t = k + f, |f| <= 1/2, and a polynomial for 2^f with a relative error below 1.5e-13 (an equal-ripple fit
+// of degree 9, exact at f = 0)
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = fmax(t, -1100.0);  // 2^t is 0 there, and for a NaN
+  const double k = rint(t), f = t - k;
+  double e = 0x1.89efabdef686ep-24;
+  e = __builtin_fma(e, f, 0x1.63c688cf3cab8p-20);
+  e = __builtin_fma(e, f, 0x1.fffb62b51cef6p-17);
+  e = __builtin_fma(e, f, 0x1.4308b503274e4p-13);
+  e = __builtin_fma(e, f, 0x1.5d87ed72fbd66p-10);
+  e = __builtin_fma(e, f, 0x1.3b2ab71455231p-7);
+  e = __builtin_fma(e, f, 0x1.c6b08d793b970p-5);
+  e = __builtin_fma(e, f, 0x1.ebfbdff8256ebp-3);
+  e = __builtin_fma(e, f, 0x1.62e42fefa11f3p-1);
   e = __builtin_fma(e, f, 1.0);
   return __builtin_ldexp(e, (int)k);
 }
@@ -122,15 +128,16 @@ __device__ __forceinline__ double log_from_one(double c) {
   return __builtin_fma((double)k, 0.69314718055994531, 2.0 * s * e);
 }
 
-// the weight of a logit: 1 at the largest, 0 at -inf and beside +inf
-__device__ __forceinline__ double weight(float x, float m, double inv_t) {
-  const double w = exp_neg(((double)x - (double)m) * inv_t);
-  return x == m ? 1.0 : (x == -kInf || m == kInf ? 0.0 : w);
-}
+// The weight of a logit beside the largest, which is finite (see without_inf): 1 for that, 0 for -inf.  `per_t` is
+// log2(e) / T.  (-inf / inf is a NaN on the way and 0 in the end.)
+__device__ __forceinline__ double weight(float x, float m, double per_t) { return exp2_neg(((double)x - (double)m) * per_t); }
+
+// Beside +inf every finite logit weighs nothing, and those that are +inf weigh the same: 0 and -inf say that in finite terms.
+__device__ __forceinline__ float without_inf(float x) { return x == kInf ? 0.0f : -kInf; }
 
 __device__ __forceinline__ void write_result(const SampleArgs& a, uint64_t r, int action, float x, float m, double inv_t, double total) {
   a.actions[r] = action;
-  if (a.logprob) a.logprob[r] = action < 0 ? -kInf : (float)((x == m ? 0.0 : ((double)x - (double)m) * inv_t) - log_from_one(total));
+  if (a.logprob) a.logprob[r] = action < 0 ? -kInf : (float)(((double)x - (double)m) * inv_t - log_from_one(total));
 }
 
 // ------------------------------------------------------- up to 8 actions ---
@@ -149,35 +156,43 @@ __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < N; i++) m = fmaxf(m, x[i]);
+    if (__any(m == kInf) && m == kInf) {
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = without_inf(x[i]);
+      m = 0.0f;
+    }
     double w[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) w[i] = weight(x[i], m, s.inv_t);
+    for (int i = 0; i < N; i++) w[i] = weight(x[i], m, s.per_t);
     if (CUT) {
-      int rank[N];
+      if (__any(s.k < N)) {
+        int rank[N] = {};
 #pragma unroll
-      for (int i = 0; i < N; i++) rank[i] = 0;
+        for (int i = 0; i < N; i++)
+#pragma unroll
+          for (int j = i + 1; j < N; j++) {
+            const bool later = x[j] > x[i];  // equal: the lower index first
+            rank[i] += later ? 1 : 0;
+            rank[j] += later ? 0 : 1;
+          }
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = rank[i] < s.k ? w[i] : 0.0;
+      }
+      double s1 = 0.0, ahead[N] = {};
+#pragma unroll
+      for (int i = 0; i < N; i++) s1 += w[i];
+      const double target = s.p < 1.0 ? s.p * s1 : __builtin_inf();
 #pragma unroll
       for (int i = 0; i < N; i++)
 #pragma unroll
         for (int j = i + 1; j < N; j++) {
-          const bool later = x[j] > x[i];  // equal: the lower index first
-          rank[i] += later ? 1 : 0;
-          rank[j] += later ? 0 : 1;
+          const bool later = x[j] > x[i];
+          ahead[i] += later ? w[j] : 0.0;
+          ahead[j] += later ? 0.0 : w[i];
         }
-      double s1 = 0.0;
+      // nothing lies ahead of the first alone
 #pragma unroll
-      for (int i = 0; i < N; i++) s1 += rank[i] < s.k ? w[i] : 0.0;
-      const double target = s.p * s1;
-      bool kept[N];
-#pragma unroll
-      for (int i = 0; i < N; i++) {
-        double ahead = 0.0;
-#pragma unroll
-        for (int j = 0; j < N; j++) ahead += rank[j] < rank[i] ? w[j] : 0.0;
-        kept[i] = rank[i] == 0 || (rank[i] < s.k && (s.p >= 1.0 || ahead < target) && w[i] >= s.q);
-      }
-#pragma unroll
-      for (int i = 0; i < N; i++) w[i] = kept[i] ? w[i] : 0.0;
+      for (int i = 0; i < N; i++) w[i] = (ahead[i] < target || ahead[i] == 0.0) && w[i] >= s.q ? w[i] : 0.0;
     }
     double total = 0.0;
 #pragma unroll
@@ -206,53 +221,66 @@ __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
 // G lanes a row (16: four rows a wave), E consecutive actions a lane.  Bound by instructions.  With top-k or top-p the
 // row's values are sorted in registers (a bitonic network: the values alone, not their indices, for t and j are all that
 // is wanted), weighed in that order and summed along it; the draw then goes over the row as it lies.
+template <int M> struct Bit { static constexpr int value = M; };
 template <int G> __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  auto other = [](float f, auto m) { return __uint_as_float(xor_lane<decltype(m)::value>(__float_as_uint(f))); };
+  v = fmaxf(v, other(v, Bit<1>()));
+  v = fmaxf(v, other(v, Bit<2>()));
+  v = fmaxf(v, other(v, Bit<4>()));
+  v = fmaxf(v, other(v, Bit<8>()));
+  if (G == 64) {
+    v = fmaxf(v, other(v, Bit<16>()));
+    v = fmaxf(v, other(v, Bit<32>()));
+  }
   return v;
 }
-// running sums over the lanes of a group, without the lane's own
+// sums over the lanes of a group before this one
 template <int G> __device__ __forceinline__ double group_before(double v, double* all) {
-  const int lane = threadIdx.x & (G - 1);
-  double run = v;
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) {
-    const double o = __hiloint2double(__shfl_up(__double2hiint(run), d, G), __shfl_up(__double2loint(run), d, G));
-    if (lane >= d) run += o;
-  }
-  *all = __hiloint2double(__shfl(__double2hiint(run), G - 1, G), __shfl(__double2loint(run), G - 1, G));
-  const double before = __hiloint2double(__shfl_up(__double2hiint(run), 1, G), __shfl_up(__double2loint(run), 1, G));
-  return lane ? before : 0.0;
+  const double run = running_sum<G>(v);
+  *all = shfl_f64(run, G - 1, G);
+  const double before = moved_f64<0x138, 0xF>(run);  // from the lane before, of all 64
+  return threadIdx.x & (G - 1) ? before : 0.0;
 }
 template <int G> __device__ __forceinline__ unsigned long long group_ballot(bool b) {
   const unsigned long long m = __ballot(b);
   return G == 64 ? m : (m >> (threadIdx.x & 63 & ~(G - 1))) & ((1ull << (G & 63)) - 1);
 }
 
-// descending over index lane * E + e
-template <int G, int E> __device__ __forceinline__ void group_sort(float* v) {
+__device__ __forceinline__ uint32_t med3(uint32_t a, uint32_t b, uint32_t c) {
+  return max(min(a, b), min(max(a, b), c));
+}
+// Descending over index lane * E + e, of ordered keys.  A step gives a lane the larger or the smaller of two: the median of
+// them and a bound, which is one instruction.
+template <int D, int E> __device__ __forceinline__ void sort_across(uint32_t* v, uint32_t bound) {
+#pragma unroll
+  for (int e = 0; e < E; e++) v[e] = med3(v[e], xor_lane<D>(v[e]), bound);
+}
+template <int G, int E> __device__ __forceinline__ void group_sort(uint32_t* v) {
   const int lane = threadIdx.x & (G - 1);
 #pragma unroll
   for (int size = 2; size <= G * E; size <<= 1) {
 #pragma unroll
     for (int d = size >> 1; d >= 1; d >>= 1) {
+      // a block of `size` is sorted downwards if its number is even, the last one of all downwards
       if (d >= E) {
-        const bool low = !(lane & (d / E));                               // of the pair
-        const bool down = size == G * E || !(lane & (size / E));          // this block's direction
-        const bool larger = low == down;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const float o = __shfl_xor(v[e], d / E, 64);
-          v[e] = larger ? fmaxf(v[e], o) : fminf(v[e], o);
+        const bool low = !(lane & (d / E)), down = size == G * E || !(lane & (size / E));
+        const uint32_t bound = low == down ? 0xFFFFFFFFu : 0u;
+        switch (d / E) {
+          case 1: sort_across<1, E>(v, bound); break;
+          case 2: sort_across<2, E>(v, bound); break;
+          case 4: sort_across<4, E>(v, bound); break;
+          case 8: sort_across<8, E>(v, bound); break;
+          case 16: sort_across<16, E>(v, bound); break;
+          default: sort_across<32, E>(v, bound); break;
         }
       } else {
 #pragma unroll
         for (int e = 0; e < E; e++)
           if (!(e & d)) {
-            const bool down = size == G * E ? true : (size >= E ? !(lane & (size / E)) : !(e & size));
-            const float hi = fmaxf(v[e], v[e + d]), lo = fminf(v[e], v[e + d]);
-            v[e] = down ? hi : lo;
-            v[e + d] = down ? lo : hi;
+            const bool down = size == G * E || (size >= E ? !(lane & (size / E)) : !(e & size));
+            const uint32_t bound = down ? 0xFFFFFFFFu : 0u, x = v[e], y = v[e + d];
+            v[e] = med3(x, y, bound);
+            v[e + d] = med3(x, y, ~bound);
           }
       }
     }
@@ -279,52 +307,54 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 #pragma unroll
     for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
     m = group_max<G>(m);
+    if (__any(m == kInf) && m == kInf) {
+#pragma unroll
+      for (int e = 0; e < E; e++) x[e] = without_inf(x[e]);
+      m = 0.0f;
+    }
     double w[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) w[e] = weight(x[e], m, s.inv_t);
+    for (int e = 0; e < E; e++) w[e] = weight(x[e], m, s.per_t);
     if (CUT) {
       if (__any(s.k < a.n || s.p < 1.0)) {
-        float v[E];
+        uint32_t key[E], v[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = x[e];
+        for (int e = 0; e < E; e++) key[e] = v[e] = key_of(x[e]);
         group_sort<G, E>(v);
         double sw[E], sum = 0.0;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          sw[e] = first + e < s.k ? weight(v[e], m, s.inv_t) : 0.0;
+          sw[e] = first + e < s.k ? weight(value_of(v[e]), m, s.per_t) : 0.0;
           sum += sw[e];
         }
         double s1, ahead = group_before<G>(sum, &s1);
-        const double target = s.p * s1;
-        int count = 0;  // kept: a beginning of the order
-        float t = kInf;
+        const double target = s.p < 1.0 ? s.p * s1 : __builtin_inf();
+        // kept: a beginning of the order.  The last one kept is t.
+        uint32_t mine = 0;
+        int kept = 0;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          const bool in = first + e == 0 || (first + e < s.k && (s.p >= 1.0 || ahead < target) && v[e] > -kInf);
+          const bool in = first + e == 0 || (first + e < s.k && ahead < target && sw[e] > 0.0);
           ahead += sw[e];
-          count += __popcll(group_ballot<G>(in));
-          if (in) t = v[e];  // descending: the lane's last one kept is its smallest
+          mine = in ? v[e] : mine;
+          kept += in ? 1 : 0;
         }
-#pragma unroll
-        for (int d = 1; d < G; d <<= 1) t = fminf(t, __shfl_xor(t, d, 64));
+        const unsigned long long some = group_ballot<G>(kept > 0);
+        const int last_lane = 63 - __clzll(some);
+        const uint32_t t = (uint32_t)__shfl((int)mine, last_lane, G);
+        const int count = last_lane * E + __shfl(kept, last_lane, G);  // the lanes before it keep all of theirs
         int above = 0, equal = 0;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          above += __popcll(group_ballot<G>(x[e] > t));
-          equal += x[e] == t ? 1 : 0;
+          above += __popcll(group_ballot<G>(key[e] > t));
+          equal += key[e] == t ? 1 : 0;
         }
-        int before = 0;  // ties at lower indices
-#pragma unroll
-        for (int d = 1, run = equal; d < G; d <<= 1) {
-          const int o = __shfl_up(run, d, G);
-          if (lane >= d) run += o;
-          before = run - equal;
-        }
+        int before = running_sum<G>(equal) - equal;  // ties at lower indices
         const int ties = count - above;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          const bool tie = x[e] == t;
-          if (x[e] < t || (tie && before >= ties)) w[e] = 0.0;
+          const bool tie = key[e] == t;
+          w[e] = key[e] > t || (tie && before < ties) ? w[e] : 0.0;
           before += tie ? 1 : 0;
         }
       }
@@ -365,19 +395,31 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 // stretches of a multiple of 512 actions, a wave each, eight consecutive actions a lane.
 //   without a cut   one pass: each segment's largest logit and the sum of its weights relative to that
 //   with one        a pass for the largest logit (and, for top-p alone, the sum); a lower bound on what can be kept, so
-//                   that the passes after it touch few elements: the k-th largest of the lanes' largest logits, or the
-//                   weight below which all actions together weigh less than (1 - p) of the sum; a pass that puts what is
-//                   above into BINS bins by m - x, with counts and integer masses (whose order of adding changes nothing);
-//                   the bin the border falls into again by finer bins, until it holds one value; and a pass over
-//                   what is kept
-// then the segment u falls into, and in it the action.
+//                   that the passes after it touch few elements: the k-th largest of the lanes' largest logits, the
+//                   weight below which all actions together weigh less than (1 - p) of the sum, or min-p's own;
+//                   a pass that puts what is above into BINS bins by m - x, with counts and integer masses (whose order
+//                   of adding changes nothing), and lists it while that is short.  A short list is finished by comparing
+//                   every pair on it.  Otherwise the bin the border falls into goes into finer bins, until it holds one
+//                   value; and a pass over what is kept
+// then the segment u falls into, and in it the action.  Every pass's body stands once in the code, and what runs for few
+// elements is a loop: unrolled, the kernel outgrew the instruction cache and took three times as long.
 constexpr int kWideSmall = 4096;
-constexpr int kLaneRun = 8, kSegment = 64 * kLaneRun;
+constexpr int kLaneRun = 8, kSegment = 64 * kLaneRun, kAhead = GX_AHEAD;
 
 // low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
 template <class T> constexpr int kFixedBits = 0;
 template <> constexpr int kFixedBits<f16> = 13;
 template <> constexpr int kFixedBits<bf16> = 16;
+
+// logit j of a run of words
+template <class T> __device__ __forceinline__ float word_value(const uint32_t* w, int j);
+template <> __device__ __forceinline__ float word_value<float>(const uint32_t* w, int j) { return __uint_as_float(w[j]); }
+template <> __device__ __forceinline__ float word_value<bf16>(const uint32_t* w, int j) {
+  return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
+}
+template <> __device__ __forceinline__ float word_value<f16>(const uint32_t* w, int j) {
+  return (float)__builtin_bit_cast(f16, (uint16_t)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]));
+}
 
 template <int BLOCK, int BINS, int SEGMENTS> struct WideShared {
   double seg_sum[SEGMENTS];
@@ -389,14 +431,40 @@ template <int BLOCK, int BINS, int SEGMENTS> struct WideShared {
   unsigned long long wave_u64[BLOCK / 64];
   float wave_f32[2][BLOCK / 64];
   uint32_t wave_u32[BLOCK / 64];
+  // what may be kept, if that is little, as met
+  float list_x[BLOCK];
+  int list_i[BLOCK];
+  uint32_t listed;
+  int wave_kept[BLOCK / 64];
   // the border's bin
   int bin;
   uint32_t bin_count, above_count;
   unsigned long long bin_mass, above_mass;
 };
 
-// of one wave's lanes, all lanes the result
-__device__ __forceinline__ float wave_max(float v) { return group_max<64>(v); }
+// One value a thread, the first `size` of them (a power of two) sorted downwards; `swap` holds a value a thread.
+template <int BLOCK> __device__ __forceinline__ unsigned long long block_sort(unsigned long long v, int size, unsigned long long* swap) {
+  const int me = threadIdx.x;
+#pragma unroll 1
+  for (int block = 2; block <= size; block <<= 1) {
+#pragma unroll 1
+    for (int d = block >> 1; d >= 1; d >>= 1) {
+      unsigned long long o;
+      if (d >= 64) {
+        __syncthreads();
+        swap[me] = v;
+        __syncthreads();
+        o = swap[me ^ d];
+      } else {
+        o = __shfl_xor(v, d, 64);
+      }
+      const bool larger = !(me & d) == !(me & block);
+      v = (v > o) == larger ? v : o;
+    }
+  }
+  __syncthreads();
+  return v;
+}
 
 template <class T, int BLOCK, int BINS, int SEGMENTS, bool CUT, bool PACKED>
 __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
@@ -406,33 +474,82 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
   // turns of 512 actions a segment takes, so that SEGMENTS are enough
   const int turns = (a.n + kSegment * SEGMENTS - 1) / (kSegment * SEGMENTS), seg_len = kSegment * turns;
   const int segments = (a.n + seg_len - 1) / seg_len;
+  const int units = ((segments - wave + kWaves - 1) / kWaves) * turns;  // turns of this wave
 
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
     const RowParams s = row_params<CUT>(a, r);
-    // the eight logits of this lane in a turn of a segment
-    auto load = [&](int i, float* x) {
-      if (PACKED && i + kLaneRun <= a.n) load_logits<T, kLaneRun>(row + i, x);
-      else
+    bool inf_row = false;  // +inf among the logits: values says that in finite terms
+    // Eight logits from c on, as words.  c is i, or the last eight of the row where i is closer to its end: those before i
+    // are the lane's before and are taken out of the values.
+    struct Run { uint32_t w[kLaneRun * sizeof(T) / 4]; };
+    auto start = [&](int i) { return min(i, a.n - kLaneRun); };
+    auto load = [&](int i) {
+      Run e;
+      const T* at = row + (PACKED ? (int64_t)start(i) : (int64_t)start(i) * a.col_stride);
+      if (PACKED) __builtin_memcpy(&e, at, sizeof e);
+      else {
+        T v[kLaneRun];
 #pragma unroll
-        for (int j = 0; j < kLaneRun; j++) x[j] = i + j < a.n ? clean(to_f32(row[(int64_t)(i + j) * a.col_stride])) : -kInf;
+        for (int j = 0; j < kLaneRun; j++) v[j] = at[j * a.col_stride];
+        __builtin_memcpy(&e, v, sizeof e);
+      }
+      return e;
     };
-    auto each = [&](auto f) {  // f(segment, first action of this lane, its logits) over the wave's share of the row
-      for (int g = wave; g < segments; g += kWaves)
-        for (int t = 0; t < turns; t++) {
-          const int i = g * seg_len + t * kSegment + lane * kLaneRun;
-          float x[kLaneRun];
-          load(i, x);
-          f(g, x);
-        }
+    auto values = [&](const Run& e, int i, float* x) {
+#pragma unroll
+      for (int j = 0; j < kLaneRun; j++) x[j] = clean(word_value<T>(e.w, j));
+      if (inf_row)
+#pragma unroll
+        for (int j = 0; j < kLaneRun; j++) x[j] = without_inf(x[j]);
+      const int before = i - start(i);
+      if (__any(before > 0))
+#pragma unroll
+        for (int j = 0; j < kLaneRun; j++) x[j] = j < before ? -kInf : x[j];
+    };
+    // f(segment, whether this was its last turn, index of the lane's first logit, its logits) over the wave's share of the
+    // row, the next kAhead loads under way
+    auto each = [&](auto f) {
+      int g = wave, t = 0;            // of the turn at hand
+      int load_g = wave, load_t = 0;  // of the next one to load
+      auto next = [&]() {
+        const int i = load_g * seg_len + load_t * kSegment + lane * kLaneRun;
+        const bool end = load_t == turns - 1;
+        load_t = end ? 0 : load_t + 1;
+        load_g += end ? kWaves : 0;
+        return load(i);
+      };
+      Run e[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) e[k] = next();
+#pragma unroll 1
+      for (int q = 0; q < units; q++) {
+        const int i = g * seg_len + t * kSegment + lane * kLaneRun;
+        float x[kLaneRun];
+        values(e[0], i, x);
+#pragma unroll
+        for (int k = 0; k + 1 < kAhead; k++) e[k] = e[k + 1];
+        e[kAhead - 1] = next();
+        const bool end = t == turns - 1;
+        f(g, end, start(i), x);
+        t = end ? 0 : t + 1;
+        g += end ? kWaves : 0;
+      }
+    };
+    auto largest = [&](const float* x) {
+      float v = x[0];
+#pragma unroll
+      for (int j = 1; j < kLaneRun; j++) v = fmaxf(v, x[j]);
+      return v;
     };
     auto block_max = [&](float v, int slot) {
-      v = wave_max(v);
+      v = group_max<64>(v);
       if (lane == 0) sh.wave_f32[slot][wave] = v;
       __syncthreads();
       v = sh.wave_f32[slot][0];
 #pragma unroll
       for (int w = 1; w < kWaves; w++) v = fmaxf(v, sh.wave_f32[slot][w]);
+      __syncthreads();
       return v;
     };
     auto block_sum = [&](double v) {
@@ -451,66 +568,76 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
     uint32_t lo = 0, hi = 0;
     int ties = 0;
     bool ordered = false;  // some of those in [lo, hi] are left out
+    bool done = false;
     if (!CUT) {
       // largest logit and sum of a segment: a lane's own first, then the wave's
-      for (int g = wave; g < segments; g += kWaves) {
-        float top = -kInf;
-        double sum = 0.0;
-        for (int t = 0; t < turns; t++) {
-          float x[kLaneRun];
-          load(g * seg_len + t * kSegment + lane * kLaneRun, x);
-          float here = x[0];
+#pragma unroll 1
+      for (;; inf_row = true) {
+      float top = -kInf;
+      double sum = 0.0;
+      each([&](int g, bool end, int, const float* x) {
+        const float here = largest(x);
+        if (here > top) {
+          sum *= weight(top, here, s.per_t);
+          top = here;
+        }
+        if (top > -kInf)
 #pragma unroll
-          for (int j = 1; j < kLaneRun; j++) here = fmaxf(here, x[j]);
-          if (here > top) {
-            sum *= weight(top, here, s.inv_t);
-            top = here;
+          for (int j = 0; j < kLaneRun; j++) sum += weight(x[j], top, s.per_t);
+        if (end) {
+          const float seg_top = group_max<64>(top);
+          sum = wave_sum(top > -kInf ? sum * weight(top, seg_top, s.per_t) : 0.0);
+          if (lane == 0) {
+            sh.seg_max[g] = seg_top;
+            sh.seg_sum[g] = sum;
           }
-#pragma unroll
-          for (int j = 0; j < kLaneRun; j++) sum += weight(x[j], top, s.inv_t) * (x[j] > -kInf ? 1.0 : 0.0);
+          top = -kInf;
+          sum = 0.0;
         }
-        const float seg_top = wave_max(top);
-        sum = wave_sum(top > -kInf ? sum * weight(top, seg_top, s.inv_t) : 0.0);
-        if (lane == 0) {
-          sh.seg_max[g] = seg_top;
-          sh.seg_sum[g] = sum;
-        }
-      }
+      });
       __syncthreads();
+      m = -kInf;
       for (int g = threadIdx.x; g < segments; g += BLOCK) m = fmaxf(m, sh.seg_max[g]);
       m = block_max(m, 0);
+      if (m < kInf) break;
+      }
       for (int g = threadIdx.x; g < segments; g += BLOCK)
-        if (sh.seg_max[g] > -kInf) sh.seg_sum[g] *= weight(sh.seg_max[g], m, s.inv_t);
+        if (sh.seg_max[g] > -kInf) sh.seg_sum[g] *= weight(sh.seg_max[g], m, s.per_t);
       __syncthreads();
     } else {
       // ---- the largest logit; the smallest finite one; the sum, relative to the lane's own largest
       const bool by_k = s.k < a.n, by_p = s.p < 1.0, sums = by_p && !by_k;
-      float top = -kInf, bottom = kInf;
-      double sum = 0.0;
-      each([&](int, const float* x) {
-        float here = x[0];
-#pragma unroll
-        for (int j = 1; j < kLaneRun; j++) here = fmaxf(here, x[j]);
+      float top, bottom;
+      double sum;
+#pragma unroll 1
+      for (;; inf_row = true) {
+      top = -kInf;
+      bottom = kInf;
+      sum = 0.0;
+      each([&](int, bool, int, const float* x) {
+        const float here = largest(x);
 #pragma unroll
         for (int j = 0; j < kLaneRun; j++) bottom = fminf(bottom, x[j] > -kInf ? x[j] : kInf);
         if (here > top) {
-          if (sums) sum *= weight(top, here, s.inv_t);
+          if (sums) sum *= weight(top, here, s.per_t);
           top = here;
         }
         if (sums && top > -kInf)
 #pragma unroll
-          for (int j = 0; j < kLaneRun; j++) sum += weight(x[j], top, s.inv_t);
+          for (int j = 0; j < kLaneRun; j++) sum += weight(x[j], top, s.per_t);
       });
       m = block_max(top, 0);
+      if (m < kInf) break;
+      }
       bottom = -block_max(-bottom, 1);
-      double s1 = sums ? block_sum(top > -kInf ? sum * weight(top, m, s.inv_t) : 0.0) : 0.0;
+      double s1 = sums ? block_sum(top > -kInf ? sum * weight(top, m, s.per_t) : 0.0) : 0.0;
       if (m > -kInf) {
         // ---- a bound below everything that can be kept.  Weights below exp(-745) are 0.
         double bound = (double)m - 745.0 / s.inv_t;
         if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * s1 / (double)a.n, 1e-320)) / s.inv_t);
+        if (!by_k && s.q > 0.0) bound = fmax(bound, (double)m + log(s.q) / s.inv_t);
         float from = fminf(m, fmaxf(bottom, (float)(bound - fabs(bound) * 1e-6)));
-        if (m == kInf) from = kInf;
-        if (by_k && s.k <= BLOCK && m < kInf) {
+        if (by_k && s.k <= BLOCK) {
           // a value that k lanes' largest reach: halving between the smallest and the largest
           float low = from, high = m;
           for (int step = 0; step < 14; step++) {
@@ -521,11 +648,15 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           if (__syncthreads_count(top >= low) >= s.k) from = low;
         }
         // ---- bins
-        // masses as integers: the sum (at most k where it is not known) below 2^62
+        // masses as integers: the sum (at most k, or n, where it is not known) below 2^62
         const int scale_bits = 61 - __builtin_amdgcn_frexp_exp(sums ? s1 : (double)s.k);
-        const float per = m > from && m < kInf ? (float)(BINS - 1) / (m - from) : 0.0f;
-        auto bin_of = [&](float x) { return x == m ? 0 : (int)fminf((m - x) * per, (float)(BINS - 1)); };
+        const float per = m > from ? (float)(BINS - 1) / (m - from) : 0.0f;
+        auto bin_of = [&](float x) { return (int)fminf((m - x) * per, (float)(BINS - 1)); };
         const uint32_t key_from = key_of(from), key_m = key_of(m);
+        auto put_in = [&](int b, float x) {
+          atomicAdd(&sh.count[b], 1u);
+          atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(weight(x, m, s.per_t), scale_bits));
+        };
         // the border by counts or by masses: the first bin where what lies up to its end reaches the target
         auto find_bin = [&](bool mass, uint32_t want_count, unsigned long long want_mass) {
           constexpr int kEach = BINS / BLOCK;
@@ -568,155 +699,229 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           __syncthreads();
           return sh.bin;
         };
-        auto clear_bins = [&]() {
-          for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = 0; sh.mass[b] = 0; }
-          __syncthreads();
-        };
-        auto put_in = [&](int b, float x) {
-          atomicAdd(&sh.count[b], 1u);
-          atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(weight(x, m, s.inv_t), scale_bits));
-        };
-        auto coarse = [&]() {
-          clear_bins();
-          each([&](int, const float* x) {
+        auto all_mass = [&]() {
+          unsigned long long all = 0;
+          for (int b = threadIdx.x; b < BINS; b += BLOCK) all += sh.mass[b];
 #pragma unroll
-            for (int j = 0; j < kLaneRun; j++)
-              if (x[j] >= from) put_in(bin_of(x[j]), x[j]);
-          });
+          for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
+          if (lane == 0) sh.wave_u64[wave] = all;
           __syncthreads();
+          all = 0;
+          for (int v = 0; v < kWaves; v++) all += sh.wave_u64[v];
+          __syncthreads();
+          return all;
         };
-        // the border: [lo, hi] that hold one value (or one action), what is above them, and how many of them are kept
-        auto border = [&](bool mass, uint32_t want_count, unsigned long long want_mass) {
-          if (find_bin(mass, want_count, want_mass) < 0) return false;
-          {
-            // the keys of the bin: bin_of falls as the key rises
-            const int b = sh.bin;
-            uint32_t l = key_from, h = key_m;
-            while (l < h) {  // the smallest key whose bin is at most b
-              const uint32_t mid = l + (h - l) / 2;
-              if (bin_of(value_of(mid)) <= b) h = mid; else l = mid + 1;
-            }
-            lo = l;
-            h = key_m;
-            while (l < h) {  // the largest whose bin is at least b
-              const uint32_t mid = l + (h - l + 1) / 2;
-              if (bin_of(value_of(mid)) >= b) l = mid; else h = mid - 1;
-            }
-            hi = l;
-          }
-          while (sh.bin_count > 1 && (hi - lo) >> kFixedBits<T>) {
-            const uint32_t above_count = sh.above_count;
-            const unsigned long long above_mass = sh.above_mass;
-            const int width = 32 - __clz(hi - lo), shift = width > __builtin_ctz(BINS) ? width - __builtin_ctz(BINS) : 0;
+        bool cut = false;                          // the border is known
+        bool by_mass = !by_k;                      // top-k first, then top-p of what that left
+        uint32_t want_count = (uint32_t)s.k;
+        unsigned long long want_mass = sums ? (unsigned long long)ceil(s.p * __builtin_ldexp(s1, scale_bits)) : 0;
+        uint32_t k_lo = 0, k_hi = 0;               // top-k's border
+        int k_ties = 0;
+        bool k_cut = false, k_ordered = false;
+        // Each round: all elements from `from` on into coarse bins (level 0), then the border's bin into finer ones
+#pragma unroll 1
+        for (bool first = true;; first = false) {
+          uint32_t below_lo = key_from, below_hi = 0xFFFFFFFFu;  // the keys that are binned
+          int shift = 0;
+          uint32_t above_count = 0;
+          unsigned long long above_mass = 0;
+          bool found = true;
+#pragma unroll 1
+          for (int level = 0;; level++) {
+            if (first && threadIdx.x == 0 && level == 0) sh.listed = 0;
+            for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = 0; sh.mass[b] = 0; }
             __syncthreads();
-            clear_bins();
-            each([&](int, const float* x) {
+            each([&](int, bool, int i, const float* x) {
+              uint32_t in = 0;  // which of the eight
 #pragma unroll
               for (int j = 0; j < kLaneRun; j++) {
                 const uint32_t key = key_of(x[j]);
-                if (key >= lo && key <= hi) put_in((int)((hi - key) >> shift), x[j]);
+                in |= key >= below_lo && key <= below_hi ? 1u << j : 0u;
+              }
+#pragma unroll 1
+              while (in) {
+                const int j = __ffs(in) - 1;
+                in &= in - 1;
+                float v = x[0];
+#pragma unroll
+                for (int k = 1; k < kLaneRun; k++) v = j == k ? x[k] : v;
+                put_in(level ? (int)((below_hi - key_of(v)) >> shift) : bin_of(v), v);
+                if (first && level == 0 && sh.listed <= (uint32_t)BLOCK) {
+                  const uint32_t at = atomicAdd(&sh.listed, 1u);
+                  if (at < (uint32_t)BLOCK) {
+                    sh.list_x[at] = v;
+                    sh.list_i[at] = i + j;
+                  }
+                }
               }
             });
             __syncthreads();
-            find_bin(mass, want_count - above_count, want_mass - above_mass);
-            hi -= (uint32_t)sh.bin << shift;
-            const uint32_t low = hi - ((1u << shift) - 1);
-            lo = low > lo && low <= hi ? low : lo;
-            if (threadIdx.x == 0) {
-              sh.above_count += above_count;
-              sh.above_mass += above_mass;
+            if (first && level == 0 && (sh.listed <= (uint32_t)BLOCK || (!by_k && !by_p))) {
+              done = sh.listed <= (uint32_t)BLOCK;
+              found = false;
+              break;
             }
+            if (level == 0) {
+              found = find_bin(by_mass, want_count, want_mass > 0 ? want_mass : 1) >= 0;
+              if (!found) break;
+              // the keys of the bin: bin_of falls as the key rises
+              const int b = sh.bin;
+              uint32_t l = key_from, h = key_m;
+              while (l < h) {  // the smallest key whose bin is at most b
+                const uint32_t mid = l + (h - l) / 2;
+                if (bin_of(value_of(mid)) <= b) h = mid; else l = mid + 1;
+              }
+              below_lo = l;
+              h = key_m;
+              while (l < h) {  // the largest whose bin is at least b
+                const uint32_t mid = l + (h - l + 1) / 2;
+                if (bin_of(value_of(mid)) >= b) l = mid; else h = mid - 1;
+              }
+              below_hi = l;
+            } else {
+              (void)find_bin(by_mass, want_count - above_count, (want_mass > 0 ? want_mass : 1) - above_mass);
+              below_hi -= (uint32_t)sh.bin << shift;
+              const uint32_t low = below_hi - ((1u << shift) - 1);
+              below_lo = low > below_lo && low <= below_hi ? low : below_lo;
+            }
+            above_count += sh.above_count;
+            above_mass += sh.above_mass;
+            if (sh.bin_count == 1 || !((below_hi - below_lo) >> kFixedBits<T>)) break;  // one action, or one value
+            const int width = 32 - __clz(below_hi - below_lo);
+            shift = width > __builtin_ctz(BINS) ? width - __builtin_ctz(BINS) : 0;
             __syncthreads();
           }
-          // one value: that of the key with the type's fixed bits, in [lo, hi]
-          if (mass) {
-            const double one = (double)sh.bin_mass / (double)sh.bin_count;
-            const double need = ceil((double)(want_mass - sh.above_mass) / one);
-            ties = need < (double)sh.bin_count ? (int)need : (int)sh.bin_count;
-            if (ties < 1) ties = 1;
-          } else {
-            ties = (int)(want_count - sh.above_count);
-          }
-          ordered = (uint32_t)ties < sh.bin_count;
-          return true;
-        };
-        bool cut = false;
-        if (by_k || by_p) {
-          coarse();
-          if (by_k) {
-            cut = border(false, (uint32_t)s.k, 0);
-            if (by_p) {
-              unsigned long long all = 0;  // of the first k
-              if (cut) {
-                all = sh.above_mass + (unsigned long long)((double)sh.bin_mass / (double)sh.bin_count * (double)ties);
-              } else {
-                // fewer than k: everything above `from`
-                for (int b = threadIdx.x; b < BINS; b += BLOCK) all += sh.mass[b];
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
-                if (lane == 0) sh.wave_u64[wave] = all;
-                __syncthreads();
-                all = 0;
-                for (int v = 0; v < kWaves; v++) all += sh.wave_u64[v];
-                __syncthreads();
-              }
-              const unsigned long long want = (unsigned long long)ceil(s.p * (double)all);
-              const uint32_t k_lo = lo, k_hi = hi;
-              const int k_ties = ties;
-              const bool k_cut = cut, k_ordered = ordered;
-              if (cut) coarse();  // finer bins have taken their place
-              const bool found = border(true, 0, want > 0 ? want : 1);
-              // the border by mass counts only where it is the stricter one
-              if (k_cut && (!found || hi < k_hi || (hi == k_hi && ties > k_ties))) {
-                lo = k_lo; hi = k_hi; ties = k_ties; ordered = k_ordered;
-                cut = true;
-              } else {
-                cut = found;
-              }
+          if (!found && (done || (!by_k && !by_p))) break;
+          const uint32_t bin_count = sh.bin_count;
+          const double one = found ? (double)sh.bin_mass / (double)bin_count : 0.0;
+          if (!by_mass) {
+            k_cut = found;
+            k_lo = below_lo;
+            k_hi = below_hi;
+            k_ties = (int)(want_count - above_count);
+            k_ordered = (uint32_t)k_ties < bin_count;
+            if (!by_p) {
+              cut = found;
+              lo = k_lo; hi = k_hi; ties = k_ties; ordered = k_ordered;
+              break;
             }
-          } else {
-            const unsigned long long want = (unsigned long long)ceil(s.p * __builtin_ldexp(s1, scale_bits));
-            cut = border(true, 0, want > 0 ? want : 1);
+            // top-p's share of the first k, or of all there are
+            const unsigned long long all = found ? above_mass + (unsigned long long)(one * (double)k_ties) : all_mass();
+            want_mass = (unsigned long long)ceil(s.p * (double)all);
+            by_mass = true;
+            __syncthreads();
+            continue;
           }
-        }
-        if (!cut) {  // everything above the bound
-          lo = key_from;
-          hi = key_from - 1;
-          ties = 0;
-          ordered = false;
+          const double need = ceil((double)((want_mass > 0 ? want_mass : 1) - above_mass) / one);
+          cut = found;
+          lo = below_lo;
+          hi = below_hi;
+          ties = need < (double)bin_count ? (need > 1.0 ? (int)need : 1) : (int)bin_count;
+          ordered = (uint32_t)ties < bin_count;
+          // the border by mass counts only where it is the stricter one
+          if (k_cut && (!found || hi < k_hi || (hi == k_hi && ties > k_ties))) {
+            cut = true;
+            lo = k_lo; hi = k_hi; ties = k_ties; ordered = k_ordered;
+          }
+          break;
         }
         __syncthreads();
-        // ---- what is kept, by segments
-        for (int g = wave; g < segments; g += kWaves) {
-          double sum = 0.0;
-          int here = 0;
-          for (int t = 0; t < turns; t++) {
-            float x[kLaneRun];
-            load(g * seg_len + t * kSegment + lane * kLaneRun, x);
+        if (done) {
+          // ---- little is left: an action a thread, sorted by value where an order is asked for, then by index
+          const int n = (int)sh.listed, me = threadIdx.x;
+          int left = n;  // of them, still in
+          auto size_for = [](int count) { return count <= 64 ? 64 : 1 << (32 - __clz(count - 1)); };
+          // running sums over the threads, the own included
+          auto block_running = [&](double v, double* all) {
+            double run = running_sum<64>(v);
+            if (lane == 63) sh.wave_f64[wave] = run;
+            __syncthreads();
+            double total = 0.0;
+#pragma unroll
+            for (int q = 0; q < kWaves; q++) {
+              if (q == wave) run += total;
+              total += sh.wave_f64[q];
+            }
+            __syncthreads();
+            *all = total;
+            return run;
+          };
+          float x = me < n ? sh.list_x[me] : -kInf;
+          int i = me < n ? sh.list_i[me] : 0;
+          double w = 0.0;
+          // first round: by value, and the cuts; second: by index
+#pragma unroll 1
+          for (int round = by_k || by_p ? 0 : 1; round < 2; round++) {
+            const bool in = me < left;
+            const unsigned long long mine = round == 0 ? (unsigned long long)key_of(x) << 32 | (uint32_t)~i : (unsigned long long)(uint32_t)~i << 32 | key_of(x);
+            const unsigned long long key = block_sort<BLOCK>(in ? mine : 0, size_for(left), sh.mass);
+            x = value_of(round == 0 ? (uint32_t)(key >> 32) : (uint32_t)key);
+            i = (int)~(round == 0 ? (uint32_t)key : (uint32_t)(key >> 32));
+            w = in ? weight(x, m, s.per_t) : 0.0;
+            if (round == 0) {
+              if (me >= s.k) w = 0.0;
+              double all;
+              const double ahead = block_running(w, &all) - w;
+              const bool keep = in && me < s.k && (me == 0 || !by_p || ahead < s.p * (by_k ? all : s1));
+              left = __syncthreads_count(keep);  // a beginning of the order
+            }
+          }
+          if (w < s.q) w = 0.0;
+          double total;
+          const double c = block_running(w, &total);
+          // the first past the border; rounding may have put that at the total: then the last one kept
+          const unsigned long long past = __ballot(w > 0.0 && c > s.u * total), kept = __ballot(w > 0.0);
+          if (lane == 0) {
+            sh.wave_u32[wave] = past ? wave * 64 + __ffsll(past) - 1 : BLOCK;
+            sh.wave_kept[wave] = kept ? wave * 64 + 63 - __clzll(kept) : -1;
+          }
+          __syncthreads();
+          int chosen = BLOCK, last = 0;
+#pragma unroll
+          for (int q = 0; q < kWaves; q++) {
+            chosen = min(chosen, (int)sh.wave_u32[q]);
+            last = max(last, sh.wave_kept[q]);
+          }
+          if (me == (chosen < BLOCK ? chosen : last)) write_result(a, r, i, x, m, s.inv_t, total);
+        } else {
+          if (!cut) {  // everything above the bound
+            lo = key_from;
+            hi = key_from - 1;
+            ties = 0;
+            ordered = false;
+          }
+          // ---- what is kept, by segments
+          double sum_here = 0.0;
+          int ties_here = 0;
+          each([&](int g, bool end, int, const float* x) {
 #pragma unroll
             for (int j = 0; j < kLaneRun; j++) {
               const uint32_t key = key_of(x[j]);
               const bool tie = key >= lo && key <= hi;
-              here += tie ? 1 : 0;
+              ties_here += tie ? 1 : 0;
               if (key > hi || (tie && !ordered)) {
-                const double w = weight(x[j], m, s.inv_t);
-                sum += w >= s.q ? w : 0.0;
+                const double w = weight(x[j], m, s.per_t);
+                sum_here += w >= s.q ? w : 0.0;
               }
             }
-          }
-          sum = wave_sum(sum);
-          if (ordered) here = wave_sum(here);
-          if (lane == 0) {
-            sh.seg_sum[g] = sum;
-            sh.seg_ties[g] = here;
-          }
+            if (end) {
+              sum_here = wave_sum(sum_here);
+              if (ordered) ties_here = wave_sum(ties_here);
+              if (lane == 0) {
+                sh.seg_sum[g] = sum_here;
+                sh.seg_ties[g] = ties_here;
+              }
+              sum_here = 0.0;
+              ties_here = 0;
+            }
+          });
         }
         __syncthreads();
       }
     }
 
     // ---- the segment, and in it the action: one wave's work
-    if (wave == 0) {
+    if (wave == 0 && !done) {
       int action = -1;
       float chosen = 0.0f;
       double total = 0.0;
@@ -728,8 +933,8 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         if (CUT && ordered) {
           // the value in [lo, hi]: by the type's fixed bits, or (one binary32 value) lo = hi
           const uint32_t mask = (1u << kFixedBits<T>) - 1;
-          const float t = value_of(hi & 0x80000000u ? hi & ~mask : (hi + 1 - (mask + 1)) | mask);
-          tie_weight = weight(t, m, s.inv_t);
+          const float t = value_of(hi & 0x80000000u ? hi & ~mask : (hi - mask) | mask);
+          tie_weight = weight(t, m, s.per_t);
           if (tie_weight < s.q) tie_weight = 0.0;
           int mine = 0;
           for (int g = g0; g < g1; g++) mine += sh.seg_ties[g];
@@ -779,11 +984,12 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         double base = over ? __hiloint2double(__shfl(__double2hiint(past_before), from_lane, 64), __shfl(__double2loint(past_before), from_lane, 64))
                            : -__builtin_inf();
         bool found = false;
+#pragma unroll 1
         for (int t = 0; t < turns && !found; t++) {
-          const int i = seg * seg_len + t * kSegment + lane * kLaneRun;
+          const int at = seg * seg_len + t * kSegment + lane * kLaneRun, i = start(at);
           float x[kLaneRun];
           double w[kLaneRun], mine = 0.0;
-          load(i, x);
+          values(load(at), at, x);
           int equal = 0;
 #pragma unroll
           for (int j = 0; j < kLaneRun; j++) {
@@ -809,7 +1015,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
               in = key > hi || (tie && (!ordered || rank < ties));
               rank += tie ? 1 : 0;
             }
-            w[j] = in ? weight(x[j], m, s.inv_t) : 0.0;
+            w[j] = in ? weight(x[j], m, s.per_t) : 0.0;
             if (CUT && w[j] < s.q) w[j] = 0.0;
             mine += w[j];
           }
@@ -870,7 +1076,7 @@ template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArg
   GX_GROUP(16, 1) GX_GROUP(16, 2) GX_GROUP(16, 4) GX_GROUP(64, 2) GX_GROUP(64, 4)
 #undef GX_GROUP
   if (a.n <= kWideSmall) hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, CUT, PACKED>), grid(1), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((wide_kernel<T, 1024, 2048, 1024, CUT, PACKED>), grid(1), dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL((wide_kernel<T, GX_WB, 2048, 1024, CUT, PACKED>), grid(1), dim3(GX_WB), 0, stream, a);
   return hipGetLastError();
 }
 
