@@ -392,19 +392,23 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 
 // --------------------------------------------------- more than 256 actions ---
 // A workgroup a row, which it reads from memory once and again from the caches.  The row is cut into at most SEGMENTS
-// stretches of a multiple of 512 actions, a wave each, eight consecutive actions a lane.
-//   without a cut   one pass: each segment's largest logit and the sum of its weights relative to that
-//   with one        a pass for the largest logit (and, for top-p alone, the sum); a lower bound on what can be kept, so
-//                   that the passes after it touch few elements: the k-th largest of the lanes' largest logits, the
-//                   weight below which all actions together weigh less than (1 - p) of the sum, or min-p's own;
-//                   a pass that puts what is above into BINS bins by m - x, with counts and integer masses (whose order
-//                   of adding changes nothing), and lists it while that is short.  A short list is finished by comparing
-//                   every pair on it.  Otherwise the bin the border falls into goes into finer bins, until it holds one
-//                   value; and a pass over what is kept
-// then the segment u falls into, and in it the action.  Every pass's body stands once in the code, and what runs for few
-// elements is a loop: unrolled, the kernel outgrew the instruction cache and took three times as long.
+// stretches, a wave each, 32 bytes of consecutive logits a lane and turn.
+//
+// Without a cut, one pass: each segment's largest logit and the sum of its weights relative to that.  With one:
+//   1  the largest logit, and for top-p alone the sum of the weights, estimated in binary32
+//   2  a lower bound on what can be kept (the k-th largest of the lanes' largest logits; the weight below which all
+//      actions together weigh less than 1 - p of the sum; min-p's own); what is above goes into BINS bins by m - x, and is
+//      listed while the list is short
+//   3  for top-p alone: the exact sum, the exact sums of the segments above the bins where the estimates put the border,
+//      and the list of what lies in those
+//   4  a short list is sorted: it ends with the border.  Where it is too long, or the estimate was wrong, the border's bin
+//      goes into finer and finer bins with integer masses (whose order of adding changes nothing) until it holds one
+//      value, and a last pass adds up what is kept by segments
+// then the segment u falls into, and in it the action.  The passes are bound by instructions: 20 an exponential in
+// binary64, so step 3 is the only one that takes them of every action.  What runs for few elements is a loop: unrolled,
+// the kernel outgrew the instruction cache and took three times as long.
 constexpr int kWideSmall = 4096;
-constexpr int kLaneRun = 8, kSegment = 64 * kLaneRun, kAhead = GX_AHEAD;
+constexpr int kAhead = 2;
 
 // low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
 template <class T> constexpr int kFixedBits = 0;
@@ -429,13 +433,14 @@ template <int BLOCK, int BINS, int SEGMENTS> struct WideShared {
   uint32_t count[BINS];
   double wave_f64[BLOCK / 64];
   unsigned long long wave_u64[BLOCK / 64];
-  float wave_f32[2][BLOCK / 64];
+  float wave_f32[BLOCK / 64];
   uint32_t wave_u32[BLOCK / 64];
-  // what may be kept, if that is little, as met
+  int wave_kept[BLOCK / 64];
+  // what may be kept, or the border's surroundings, if that is little
   float list_x[BLOCK];
   int list_i[BLOCK];
   uint32_t listed;
-  int wave_kept[BLOCK / 64];
+  float bound;
   // the border's bin
   int bin;
   uint32_t bin_count, above_count;
@@ -468,52 +473,54 @@ template <int BLOCK> __device__ __forceinline__ unsigned long long block_sort(un
 
 template <class T, int BLOCK, int BINS, int SEGMENTS, bool CUT, bool PACKED>
 __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
-  constexpr int kWaves = BLOCK / 64;
+  constexpr int kWaves = BLOCK / 64, kRun = 32 / sizeof(T), kTurn = 64 * kRun;
   __shared__ WideShared<BLOCK, BINS, SEGMENTS> sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // turns of 512 actions a segment takes, so that SEGMENTS are enough
-  const int turns = (a.n + kSegment * SEGMENTS - 1) / (kSegment * SEGMENTS), seg_len = kSegment * turns;
+  // turns a segment takes, so that SEGMENTS are enough
+  const int turns = (a.n + kTurn * SEGMENTS - 1) / (kTurn * SEGMENTS), seg_len = kTurn * turns;
   const int segments = (a.n + seg_len - 1) / seg_len;
   const int units = ((segments - wave + kWaves - 1) / kWaves) * turns;  // turns of this wave
 
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
     const RowParams s = row_params<CUT>(a, r);
-    bool inf_row = false;  // +inf among the logits: values says that in finite terms
-    // Eight logits from c on, as words.  c is i, or the last eight of the row where i is closer to its end: those before i
-    // are the lane's before and are taken out of the values.
-    struct Run { uint32_t w[kLaneRun * sizeof(T) / 4]; };
-    auto start = [&](int i) { return min(i, a.n - kLaneRun); };
+    // 0: logits as they are.  A NaN is then no more than any bound and weighs nothing; where the largest comes out as +inf
+    // (some NaN can make it that) the row is read again with 1: NaN as -inf, and if that was not it 2: +inf in finite terms
+    int mode = 0;
+    // A run of logits from c on, as words.  c is i, or the last run of the row where i is closer to its end: those before
+    // i are the lane's before and are taken out of the values.
+    struct Run { uint32_t w[8]; };
+    auto start = [&](int i) { return min(i, a.n - kRun); };
     auto load = [&](int i) {
       Run e;
       const T* at = row + (PACKED ? (int64_t)start(i) : (int64_t)start(i) * a.col_stride);
       if (PACKED) __builtin_memcpy(&e, at, sizeof e);
       else {
-        T v[kLaneRun];
+        T v[kRun];
 #pragma unroll
-        for (int j = 0; j < kLaneRun; j++) v[j] = at[j * a.col_stride];
+        for (int j = 0; j < kRun; j++) v[j] = at[j * a.col_stride];
         __builtin_memcpy(&e, v, sizeof e);
       }
       return e;
     };
     auto values = [&](const Run& e, int i, float* x) {
 #pragma unroll
-      for (int j = 0; j < kLaneRun; j++) x[j] = clean(word_value<T>(e.w, j));
-      if (inf_row)
+      for (int j = 0; j < kRun; j++) x[j] = word_value<T>(e.w, j);
+      if (mode)
 #pragma unroll
-        for (int j = 0; j < kLaneRun; j++) x[j] = without_inf(x[j]);
+        for (int j = 0; j < kRun; j++) x[j] = mode == 2 ? without_inf(clean(x[j])) : clean(x[j]);
       const int before = i - start(i);
       if (__any(before > 0))
 #pragma unroll
-        for (int j = 0; j < kLaneRun; j++) x[j] = j < before ? -kInf : x[j];
+        for (int j = 0; j < kRun; j++) x[j] = j < before ? -kInf : x[j];
     };
     // f(segment, whether this was its last turn, index of the lane's first logit, its logits) over the wave's share of the
-    // row, the next kAhead loads under way
+    // row, the next loads under way
     auto each = [&](auto f) {
       int g = wave, t = 0;            // of the turn at hand
       int load_g = wave, load_t = 0;  // of the next one to load
       auto next = [&]() {
-        const int i = load_g * seg_len + load_t * kSegment + lane * kLaneRun;
+        const int i = load_g * seg_len + load_t * kTurn + lane * kRun;
         const bool end = load_t == turns - 1;
         load_t = end ? 0 : load_t + 1;
         load_g += end ? kWaves : 0;
@@ -523,140 +530,187 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll
       for (int k = 0; k < kAhead; k++) e[k] = next();
 #pragma unroll 1
-      for (int q = 0; q < units; q++) {
-        const int i = g * seg_len + t * kSegment + lane * kLaneRun;
-        float x[kLaneRun];
-        values(e[0], i, x);
+      for (int q = 0; q < units; q += kAhead)
 #pragma unroll
-        for (int k = 0; k + 1 < kAhead; k++) e[k] = e[k + 1];
-        e[kAhead - 1] = next();
-        const bool end = t == turns - 1;
-        f(g, end, start(i), x);
-        t = end ? 0 : t + 1;
-        g += end ? kWaves : 0;
-      }
+        for (int k = 0; k < kAhead; k++)
+          if (q + k < units) {
+            const int i = g * seg_len + t * kTurn + lane * kRun;
+            float x[kRun];
+            values(e[k], i, x);
+            e[k] = next();
+            const bool end = t == turns - 1;
+            f(g, end, start(i), x);
+            t = end ? 0 : t + 1;
+            g += end ? kWaves : 0;
+          }
     };
-    auto largest = [&](const float* x) {
-      float v = x[0];
-#pragma unroll
-      for (int j = 1; j < kLaneRun; j++) v = fmaxf(v, x[j]);
-      return v;
-    };
-    auto block_max = [&](float v, int slot) {
+    // the larger of two in one instruction: their median with +inf
+    auto larger_of = [](float x, float y) { return __builtin_amdgcn_fmed3f(x, y, kInf); };
+    auto block_max = [&](float v) {
       v = group_max<64>(v);
-      if (lane == 0) sh.wave_f32[slot][wave] = v;
+      if (lane == 0) sh.wave_f32[wave] = v;
       __syncthreads();
-      v = sh.wave_f32[slot][0];
+      v = sh.wave_f32[0];
 #pragma unroll
-      for (int w = 1; w < kWaves; w++) v = fmaxf(v, sh.wave_f32[slot][w]);
+      for (int w = 1; w < kWaves; w++) v = fmaxf(v, sh.wave_f32[w]);
       __syncthreads();
       return v;
+    };
+    // running sums over the threads, the own included, and the sum of all
+    auto block_running = [&](double v, double* all) {
+      double run = running_sum<64>(v);
+      if (lane == 63) sh.wave_f64[wave] = run;
+      __syncthreads();
+      double total = 0.0;
+#pragma unroll
+      for (int q = 0; q < kWaves; q++) {
+        if (q == wave) run += total;
+        total += sh.wave_f64[q];
+      }
+      __syncthreads();
+      *all = total;
+      return run;
     };
     auto block_sum = [&](double v) {
-      v = wave_sum(v);
-      if (lane == 0) sh.wave_f64[wave] = v;
-      __syncthreads();
-      v = 0.0;
-#pragma unroll
-      for (int w = 0; w < kWaves; w++) v += sh.wave_f64[w];
-      __syncthreads();
-      return v;
+      double all;
+      (void)block_running(v, &all);
+      return all;
     };
 
     float m = -kInf;
-    // what is kept: keys above `hi`, and the first `ties` of those in [lo, hi]
-    uint32_t lo = 0, hi = 0;
-    int ties = 0;
-    bool ordered = false;  // some of those in [lo, hi] are left out
-    bool done = false;
+    // What is kept: logits above `hi`, and of those in [lo, hi] all, or (ordered) the first `ties` by index, or (listed)
+    // those up to the index `tie_index`.
+    float lo = 0.0f, hi = 0.0f;
+    int ties = 0, tie_index = 0;
+    bool ordered = false, by_index = false;
+    bool done = false;  // the action is written
     if (!CUT) {
       // largest logit and sum of a segment: a lane's own first, then the wave's
 #pragma unroll 1
-      for (;; inf_row = true) {
-      float top = -kInf;
-      double sum = 0.0;
-      each([&](int g, bool end, int, const float* x) {
-        const float here = largest(x);
-        if (here > top) {
-          sum *= weight(top, here, s.per_t);
-          top = here;
-        }
-        if (top > -kInf)
+      for (;; mode++) {
+        float top = -kInf;
+        double sum = 0.0;
+        each([&](int g, bool end, int, const float* x) {
+          float here = x[0];
 #pragma unroll
-          for (int j = 0; j < kLaneRun; j++) sum += weight(x[j], top, s.per_t);
-        if (end) {
-          const float seg_top = group_max<64>(top);
-          sum = wave_sum(top > -kInf ? sum * weight(top, seg_top, s.per_t) : 0.0);
-          if (lane == 0) {
-            sh.seg_max[g] = seg_top;
-            sh.seg_sum[g] = sum;
+          for (int j = 1; j < kRun; j++) here = larger_of(here, x[j]);
+          if (here > top) {
+            sum *= weight(top, here, s.per_t);
+            top = here;
           }
-          top = -kInf;
-          sum = 0.0;
-        }
-      });
-      __syncthreads();
-      m = -kInf;
-      for (int g = threadIdx.x; g < segments; g += BLOCK) m = fmaxf(m, sh.seg_max[g]);
-      m = block_max(m, 0);
-      if (m < kInf) break;
+          if (__any(top > -kInf))
+#pragma unroll
+            for (int j = 0; j < kRun; j++) sum += weight(x[j], top, s.per_t);
+          if (end) {
+            const float seg_top = group_max<64>(top);
+            sum = wave_sum(top > -kInf ? sum * weight(top, seg_top, s.per_t) : 0.0);
+            if (lane == 0) {
+              sh.seg_max[g] = seg_top;
+              sh.seg_sum[g] = sum;
+            }
+            top = -kInf;
+            sum = 0.0;
+          }
+        });
+        __syncthreads();
+        m = -kInf;
+        for (int g = threadIdx.x; g < segments; g += BLOCK) m = fmaxf(m, sh.seg_max[g]);
+        m = block_max(m);
+        if (m < kInf) break;
       }
       for (int g = threadIdx.x; g < segments; g += BLOCK)
         if (sh.seg_max[g] > -kInf) sh.seg_sum[g] *= weight(sh.seg_max[g], m, s.per_t);
       __syncthreads();
     } else {
-      // ---- the largest logit; the smallest finite one; the sum, relative to the lane's own largest
-      const bool by_k = s.k < a.n, by_p = s.p < 1.0, sums = by_p && !by_k;
-      float top, bottom;
-      double sum;
+      const bool by_k = s.k < a.n, by_p = s.p < 1.0, sums = by_p && !by_k, far_k = by_k && s.k > BLOCK;
+      // ---- 1: the largest logit, the estimate of the sum, and where it is wanted the smallest finite one
+      float top, bottom, estimate;
+      const float per_t = fminf((float)s.per_t, 3e38f);
 #pragma unroll 1
-      for (;; inf_row = true) {
-      top = -kInf;
-      bottom = kInf;
-      sum = 0.0;
-      each([&](int, bool, int, const float* x) {
-        const float here = largest(x);
+      for (;; mode++) {
+        top = -kInf;
+        bottom = kInf;
+        estimate = 0.0f;
+        each([&](int, bool, int, const float* x) {
+          float here = x[0];
 #pragma unroll
-        for (int j = 0; j < kLaneRun; j++) bottom = fminf(bottom, x[j] > -kInf ? x[j] : kInf);
-        if (here > top) {
-          if (sums) sum *= weight(top, here, s.per_t);
-          top = here;
-        }
-        if (sums && top > -kInf)
+          for (int j = 1; j < kRun; j++) here = larger_of(here, x[j]);
+          if (far_k)
 #pragma unroll
-          for (int j = 0; j < kLaneRun; j++) sum += weight(x[j], top, s.per_t);
-      });
-      m = block_max(top, 0);
-      if (m < kInf) break;
-      }
-      bottom = -block_max(-bottom, 1);
-      double s1 = sums ? block_sum(top > -kInf ? sum * weight(top, m, s.per_t) : 0.0) : 0.0;
-      if (m > -kInf) {
-        // ---- a bound below everything that can be kept.  Weights below exp(-745) are 0.
-        double bound = (double)m - 745.0 / s.inv_t;
-        if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * s1 / (double)a.n, 1e-320)) / s.inv_t);
-        if (!by_k && s.q > 0.0) bound = fmax(bound, (double)m + log(s.q) / s.inv_t);
-        float from = fminf(m, fmaxf(bottom, (float)(bound - fabs(bound) * 1e-6)));
-        if (by_k && s.k <= BLOCK) {
-          // a value that k lanes' largest reach: halving between the smallest and the largest
-          float low = from, high = m;
-          for (int step = 0; step < 14; step++) {
-            const float mid = low + (high - low) * 0.5f;
-            if (!(mid > low && mid < high)) break;
-            if (__syncthreads_count(top >= mid) >= s.k) low = mid; else high = mid;
+            for (int j = 0; j < kRun; j++) bottom = x[j] > -kInf && x[j] < bottom ? x[j] : bottom;
+          if (sums) {
+            if (here > top) estimate *= __builtin_amdgcn_exp2f(fmaxf((top - here) * per_t, -150.0f));
+            top = larger_of(top, here);
+            if (top > -kInf)
+#pragma unroll
+              for (int j = 0; j < kRun; j++) estimate += __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f((x[j] - top) * per_t, -150.0f, 0.0f));
+          } else {
+            top = larger_of(top, here);
           }
-          if (__syncthreads_count(top >= low) >= s.k) from = low;
+        });
+        m = block_max(top);
+        if (m < kInf) break;
+      }
+      if (m > -kInf) {
+        if (far_k) bottom = -block_max(-bottom);
+        double s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;
+        // ---- 2: a bound below everything that can be kept (weights below exp(-745) are 0) ...
+        double bound = (double)m - 745.0 / s.inv_t;
+        if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * s1 * 0.99 / (double)a.n, 1e-320)) / s.inv_t);
+        if (!by_k && s.q > 0.0) bound = fmax(bound, (double)m + log(s.q) / s.inv_t);
+        float from = fminf(m, fmaxf((float)(bound - fabs(bound) * 1e-6), -3.402823466e38f));
+        if (far_k) from = fminf(m, fmaxf(bottom, from));
+        if (by_k && !far_k) {
+          // a value that k lanes' largest reach: halving between the bound and the largest, one wave's work
+          sh.list_x[threadIdx.x] = top;
+          __syncthreads();
+          if (wave == 0) {
+            float v[kWaves], low = from, high = m;
+#pragma unroll
+            for (int q = 0; q < kWaves; q++) v[q] = sh.list_x[q * 64 + lane];
+            auto reach = [&](float x) {
+              int c = 0;
+#pragma unroll
+              for (int q = 0; q < kWaves; q++) c += __popcll(__ballot(v[q] >= x));
+              return c;
+            };
+            const bool some = reach(low) >= s.k;
+#pragma unroll 1
+            for (int step = 0; some && step < 14; step++) {
+              const float mid = low + (high - low) * 0.5f;
+              if (!(mid > low && mid < high)) break;
+              if (reach(mid) >= s.k) low = mid; else high = mid;
+            }
+            if (lane == 0) sh.bound = low;
+          }
+          __syncthreads();
+          from = sh.bound;
         }
-        // ---- bins
-        // masses as integers: the sum (at most k, or n, where it is not known) below 2^62
-        const int scale_bits = 61 - __builtin_amdgcn_frexp_exp(sums ? s1 : (double)s.k);
+        // ---- ... and the bins
         const float per = m > from ? (float)(BINS - 1) / (m - from) : 0.0f;
         auto bin_of = [&](float x) { return (int)fminf((m - x) * per, (float)(BINS - 1)); };
-        const uint32_t key_from = key_of(from), key_m = key_of(m);
-        auto put_in = [&](int b, float x) {
-          atomicAdd(&sh.count[b], 1u);
-          atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(weight(x, m, s.per_t), scale_bits));
+        const uint32_t key_from = key_of(from + 0.0f), key_m = key_of(m + 0.0f);
+        // the smallest key whose bin is below b (one past the largest where b is 0): bin_of falls as the key rises.  The
+        // wave's lanes try 64 keys at once.
+        auto first_key_below = [&](int b) {
+          if (b <= 0) return key_m + 1;
+          uint32_t l = key_from, h = key_m;  // h's bin is 0
+#pragma unroll 1
+          while (l < h) {
+            const uint32_t step = (h - l) / 64 + 1, rest = h - l, off = (uint32_t)lane * step, at = l + (off < rest ? off : rest);
+            const unsigned long long yes = __ballot(bin_of(value_of(at)) < b);
+            const uint32_t hit = yes ? (uint32_t)__ffsll(yes) - 1 : 64;
+            const uint32_t below = hit * step, before = (hit - 1) * step;
+            if (hit < 64) h = l + (below < rest ? below : rest);
+            if (hit > 0) l = l + (before < rest ? before : rest) + 1;
+          }
+          return h;
         };
+        constexpr uint32_t kKeyMinusZero = 0x7FFFFFFFu;
+        auto low_value = [&](uint32_t key) { return value_of(key == kKeyMinusZero ? key + 1 : key); };
+        auto high_value = [&](uint32_t key) { return value_of(key == kKeyMinusZero ? key - 1 : key); };
+        // masses as integers: their sum (at most n where it is not known) stays below 2^62
+        int scale_bits = 61 - __builtin_amdgcn_frexp_exp(sums ? fmax(s1, 1.0) * 1.01 : (double)a.n);
         // the border by counts or by masses: the first bin where what lies up to its end reaches the target
         auto find_bin = [&](bool mass, uint32_t want_count, unsigned long long want_mass) {
           constexpr int kEach = BINS / BLOCK;
@@ -713,40 +767,47 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         };
         bool cut = false;                          // the border is known
         bool by_mass = !by_k;                      // top-k first, then top-p of what that left
+        bool first = true, exact = !sums;          // no round yet; masses and s1 are exact
+        bool list = false;                         // the list holds all that is kept but what lies above it
+        double above = 0.0;                        // that
         uint32_t want_count = (uint32_t)s.k;
-        unsigned long long want_mass = sums ? (unsigned long long)ceil(s.p * __builtin_ldexp(s1, scale_bits)) : 0;
+        unsigned long long want_mass = 0;
         uint32_t k_lo = 0, k_hi = 0;               // top-k's border
         int k_ties = 0;
         bool k_cut = false, k_ordered = false;
-        // Each round: all elements from `from` on into coarse bins (level 0), then the border's bin into finer ones
+        // Each round: everything from `from` on into coarse bins (level 0), then the border's bin into finer ones.
 #pragma unroll 1
-        for (bool first = true;; first = false) {
-          uint32_t below_lo = key_from, below_hi = 0xFFFFFFFFu;  // the keys that are binned
+        for (;;) {
+          uint32_t key_lo = key_from, key_hi = key_m;  // what is binned
           int shift = 0;
           uint32_t above_count = 0;
           unsigned long long above_mass = 0;
           bool found = true;
+          if (sums) want_mass = (unsigned long long)fmax(1.0, ceil(s.p * __builtin_ldexp(s1, scale_bits)));
 #pragma unroll 1
           for (int level = 0;; level++) {
-            if (first && threadIdx.x == 0 && level == 0) sh.listed = 0;
+            const bool listing = first && level == 0;
+            if (threadIdx.x == 0 && listing) sh.listed = 0;
             for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = 0; sh.mass[b] = 0; }
             __syncthreads();
+            const float x_lo = low_value(key_lo), x_hi = high_value(key_hi);
             each([&](int, bool, int i, const float* x) {
-              uint32_t in = 0;  // which of the eight
+              uint32_t in = 0;  // which of the run
 #pragma unroll
-              for (int j = 0; j < kLaneRun; j++) {
-                const uint32_t key = key_of(x[j]);
-                in |= key >= below_lo && key <= below_hi ? 1u << j : 0u;
-              }
+              for (int j = 0; j < kRun; j++) in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
 #pragma unroll 1
               while (in) {
                 const int j = __ffs(in) - 1;
                 in &= in - 1;
                 float v = x[0];
 #pragma unroll
-                for (int k = 1; k < kLaneRun; k++) v = j == k ? x[k] : v;
-                put_in(level ? (int)((below_hi - key_of(v)) >> shift) : bin_of(v), v);
-                if (first && level == 0 && sh.listed <= (uint32_t)BLOCK) {
+                for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
+                const int b = level ? (int)((key_hi - key_of(v + 0.0f)) >> shift) : bin_of(v);
+                // an estimate has 24 bits: enough to find the bin, or the one beside it
+                const double w = exact ? weight(v, m, s.per_t) : (double)__builtin_amdgcn_exp2f(fmaxf((v - m) * per_t, -150.0f));
+                atomicAdd(&sh.count[b], 1u);
+                atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(w, scale_bits));
+                if (listing && sh.listed <= (uint32_t)BLOCK) {
                   const uint32_t at = atomicAdd(&sh.listed, 1u);
                   if (at < (uint32_t)BLOCK) {
                     sh.list_x[at] = v;
@@ -756,96 +817,135 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
               }
             });
             __syncthreads();
-            if (first && level == 0 && (sh.listed <= (uint32_t)BLOCK || (!by_k && !by_p))) {
-              done = sh.listed <= (uint32_t)BLOCK;
-              found = false;
-              break;
-            }
+            if (listing) list = sh.listed <= (uint32_t)BLOCK;
             if (level == 0) {
-              found = find_bin(by_mass, want_count, want_mass > 0 ? want_mass : 1) >= 0;
+              if (list || (!by_k && !by_p)) {
+                found = false;
+                break;
+              }
+              found = find_bin(by_mass, want_count, want_mass) >= 0;
               if (!found) break;
-              // the keys of the bin: bin_of falls as the key rises
-              const int b = sh.bin;
-              uint32_t l = key_from, h = key_m;
-              while (l < h) {  // the smallest key whose bin is at most b
-                const uint32_t mid = l + (h - l) / 2;
-                if (bin_of(value_of(mid)) <= b) h = mid; else l = mid + 1;
-              }
-              below_lo = l;
-              h = key_m;
-              while (l < h) {  // the largest whose bin is at least b
-                const uint32_t mid = l + (h - l + 1) / 2;
-                if (bin_of(value_of(mid)) >= b) l = mid; else h = mid - 1;
-              }
-              below_hi = l;
+              if (!exact) break;
+              key_lo = first_key_below(sh.bin + 1);
+              key_hi = first_key_below(sh.bin) - 1;
             } else {
-              (void)find_bin(by_mass, want_count - above_count, (want_mass > 0 ? want_mass : 1) - above_mass);
-              below_hi -= (uint32_t)sh.bin << shift;
-              const uint32_t low = below_hi - ((1u << shift) - 1);
-              below_lo = low > below_lo && low <= below_hi ? low : below_lo;
+              (void)find_bin(by_mass, want_count - above_count, want_mass - above_mass);
+              key_hi -= (uint32_t)sh.bin << shift;
+              const uint32_t low = key_hi - ((1u << shift) - 1);
+              key_lo = low > key_lo && low <= key_hi ? low : key_lo;
             }
             above_count += sh.above_count;
             above_mass += sh.above_mass;
-            if (sh.bin_count == 1 || !((below_hi - below_lo) >> kFixedBits<T>)) break;  // one action, or one value
-            const int width = 32 - __clz(below_hi - below_lo);
+            if (sh.bin_count == 1 || !((key_hi - key_lo) >> kFixedBits<T>)) break;  // one action, or one value
+            const int width = 32 - __clz(key_hi - key_lo);
             shift = width > __builtin_ctz(BINS) ? width - __builtin_ctz(BINS) : 0;
             __syncthreads();
           }
-          if (!found && (done || (!by_k && !by_p))) break;
+          const bool whole_list = first && list;
+          first = false;
+          if (!exact) {
+            // ---- 3: the exact sum; above the border's bin and its neighbours by segments, and those listed
+            float x_lo = kInf, x_hi = kInf;  // nothing
+            if (found) {
+              x_lo = low_value(first_key_below(sh.bin + 2));
+              x_hi = high_value(first_key_below(sh.bin - 1) - 1);
+            }
+            __syncthreads();
+            if (threadIdx.x == 0 && !whole_list) sh.listed = 0;
+            __syncthreads();
+            double sum = 0.0, here = 0.0;
+            each([&](int g, bool end, int i, const float* x) {
+              uint32_t in = 0;
+#pragma unroll
+              for (int j = 0; j < kRun; j++) {
+                const double w = weight(x[j], m, s.per_t);
+                sum += w;
+                here += x[j] > x_hi ? w : 0.0;  // above min-p's bound too, which no bin lies below
+                in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
+              }
+#pragma unroll 1
+              while (in) {
+                const int j = __ffs(in) - 1;
+                in &= in - 1;
+                float v = x[0];
+#pragma unroll
+                for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
+                if (sh.listed <= (uint32_t)BLOCK) {
+                  const uint32_t at = atomicAdd(&sh.listed, 1u);
+                  if (at < (uint32_t)BLOCK) {
+                    sh.list_x[at] = v;
+                    sh.list_i[at] = i + j;
+                  }
+                }
+              }
+              if (end) {
+                here = wave_sum(here);
+                if (lane == 0) sh.seg_sum[g] = here;
+                here = 0.0;
+              }
+            });
+            s1 = block_sum(sum);
+            exact = true;
+            if (whole_list) break;
+            if (found && sh.listed <= (uint32_t)BLOCK) {
+              double mine = 0.0;
+              for (int g = threadIdx.x; g < segments; g += BLOCK) mine += sh.seg_sum[g];
+              above = block_sum(mine);
+              const float v = threadIdx.x < sh.listed ? sh.list_x[threadIdx.x] : -kInf;
+              const double within = block_sum(weight(v, m, s.per_t)), target = s.p * s1;
+              list = above < target && target <= above + within;
+            }
+            if (list) break;
+            scale_bits = 61 - __builtin_amdgcn_frexp_exp(s1);
+            continue;
+          }
+          if (whole_list || (!by_k && !by_p)) break;
           const uint32_t bin_count = sh.bin_count;
           const double one = found ? (double)sh.bin_mass / (double)bin_count : 0.0;
           if (!by_mass) {
             k_cut = found;
-            k_lo = below_lo;
-            k_hi = below_hi;
+            k_lo = key_lo;
+            k_hi = key_hi;
             k_ties = (int)(want_count - above_count);
             k_ordered = (uint32_t)k_ties < bin_count;
-            if (!by_p) {
-              cut = found;
-              lo = k_lo; hi = k_hi; ties = k_ties; ordered = k_ordered;
-              break;
+            if (by_p) {
+              // top-p's share of the first k, or of all there are
+              const unsigned long long all = found ? above_mass + (unsigned long long)(one * (double)k_ties) : all_mass();
+              want_mass = (unsigned long long)fmax(1.0, ceil(s.p * (double)all));
+              by_mass = true;
+              __syncthreads();
+              continue;
             }
-            // top-p's share of the first k, or of all there are
-            const unsigned long long all = found ? above_mass + (unsigned long long)(one * (double)k_ties) : all_mass();
-            want_mass = (unsigned long long)ceil(s.p * (double)all);
-            by_mass = true;
-            __syncthreads();
-            continue;
+            cut = found;
+            key_lo = k_lo; key_hi = k_hi; ties = k_ties; ordered = k_ordered;
+          } else {
+            const double need = ceil((double)(want_mass - above_mass) / one);
+            cut = found;
+            ties = need < (double)bin_count ? (need > 1.0 ? (int)need : 1) : (int)bin_count;
+            ordered = (uint32_t)ties < bin_count;
+            // the border by mass counts only where it is the stricter one
+            if (k_cut && (!found || key_hi < k_hi || (key_hi == k_hi && ties > k_ties))) {
+              cut = true;
+              key_lo = k_lo; key_hi = k_hi; ties = k_ties; ordered = k_ordered;
+            }
           }
-          const double need = ceil((double)((want_mass > 0 ? want_mass : 1) - above_mass) / one);
-          cut = found;
-          lo = below_lo;
-          hi = below_hi;
-          ties = need < (double)bin_count ? (need > 1.0 ? (int)need : 1) : (int)bin_count;
-          ordered = (uint32_t)ties < bin_count;
-          // the border by mass counts only where it is the stricter one
-          if (k_cut && (!found || hi < k_hi || (hi == k_hi && ties > k_ties))) {
-            cut = true;
-            lo = k_lo; hi = k_hi; ties = k_ties; ordered = k_ordered;
+          if (cut) {
+            lo = low_value(key_lo);
+            hi = high_value(key_hi);
+            if (ordered) {
+              // the one value in there, by the type's fixed bits
+              const uint32_t mask = (1u << kFixedBits<T>) - 1;
+              lo = hi = value_of(key_hi & 0x80000000u ? key_hi & ~mask : (key_hi - mask) | mask);
+            }
           }
           break;
         }
         __syncthreads();
-        if (done) {
-          // ---- little is left: an action a thread, sorted by value where an order is asked for, then by index
+        if (list) {
+          // ---- 4: an action a thread, sorted by value where an order is asked for, then by index
           const int n = (int)sh.listed, me = threadIdx.x;
           int left = n;  // of them, still in
           auto size_for = [](int count) { return count <= 64 ? 64 : 1 << (32 - __clz(count - 1)); };
-          // running sums over the threads, the own included
-          auto block_running = [&](double v, double* all) {
-            double run = running_sum<64>(v);
-            if (lane == 63) sh.wave_f64[wave] = run;
-            __syncthreads();
-            double total = 0.0;
-#pragma unroll
-            for (int q = 0; q < kWaves; q++) {
-              if (q == wave) run += total;
-              total += sh.wave_f64[q];
-            }
-            __syncthreads();
-            *all = total;
-            return run;
-          };
           float x = me < n ? sh.list_x[me] : -kInf;
           int i = me < n ? sh.list_i[me] : 0;
           double w = 0.0;
@@ -853,7 +953,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll 1
           for (int round = by_k || by_p ? 0 : 1; round < 2; round++) {
             const bool in = me < left;
-            const unsigned long long mine = round == 0 ? (unsigned long long)key_of(x) << 32 | (uint32_t)~i : (unsigned long long)(uint32_t)~i << 32 | key_of(x);
+            const unsigned long long mine = round == 0 ? (unsigned long long)key_of(x + 0.0f) << 32 | (uint32_t)~i : (unsigned long long)(uint32_t)~i << 32 | key_of(x + 0.0f);
             const unsigned long long key = block_sort<BLOCK>(in ? mine : 0, size_for(left), sh.mass);
             x = value_of(round == 0 ? (uint32_t)(key >> 32) : (uint32_t)key);
             i = (int)~(round == 0 ? (uint32_t)key : (uint32_t)(key >> 32));
@@ -861,49 +961,73 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             if (round == 0) {
               if (me >= s.k) w = 0.0;
               double all;
-              const double ahead = block_running(w, &all) - w;
-              const bool keep = in && me < s.k && (me == 0 || !by_p || ahead < s.p * (by_k ? all : s1));
+              const double ahead = above + (block_running(w, &all) - w);
+              const bool keep = in && me < s.k && ((me == 0 && above == 0.0) || !by_p || ahead < s.p * (by_k ? all : s1));
               left = __syncthreads_count(keep);  // a beginning of the order
+              if (me == left - 1) {
+                sh.list_x[0] = x;
+                sh.list_i[0] = i;
+              }
+              __syncthreads();
+              lo = hi = sh.list_x[0];
+              tie_index = sh.list_i[0];
+              __syncthreads();
             }
           }
           if (w < s.q) w = 0.0;
-          double total;
-          const double c = block_running(w, &total);
-          // the first past the border; rounding may have put that at the total: then the last one kept
-          const unsigned long long past = __ballot(w > 0.0 && c > s.u * total), kept = __ballot(w > 0.0);
-          if (lane == 0) {
-            sh.wave_u32[wave] = past ? wave * 64 + __ffsll(past) - 1 : BLOCK;
-            sh.wave_kept[wave] = kept ? wave * 64 + 63 - __clzll(kept) : -1;
-          }
-          __syncthreads();
-          int chosen = BLOCK, last = 0;
+          if (above == 0.0) {
+            double total;
+            const double c = block_running(w, &total);
+            // the first past the border; rounding may have put that at the total: then the last one kept
+            const unsigned long long past = __ballot(w > 0.0 && c > s.u * total), kept = __ballot(w > 0.0);
+            if (lane == 0) {
+              sh.wave_u32[wave] = past ? wave * 64 + __ffsll(past) - 1 : BLOCK;
+              sh.wave_kept[wave] = kept ? wave * 64 + 63 - __clzll(kept) : -1;
+            }
+            __syncthreads();
+            int chosen = BLOCK, last = 0;
 #pragma unroll
-          for (int q = 0; q < kWaves; q++) {
-            chosen = min(chosen, (int)sh.wave_u32[q]);
-            last = max(last, sh.wave_kept[q]);
+            for (int q = 0; q < kWaves; q++) {
+              chosen = min(chosen, (int)sh.wave_u32[q]);
+              last = max(last, sh.wave_kept[q]);
+            }
+            if (me == (chosen < BLOCK ? chosen : last)) write_result(a, r, i, x, m, s.inv_t, total);
+            done = true;
+          } else {
+            // what is kept of the list joins its segments: the first of each segment adds up that segment's
+            double* ws = reinterpret_cast<double*>(sh.mass);
+            ws[me] = w;
+            sh.list_i[me] = me < left ? i : 0x7FFFFFFF;
+            __syncthreads();
+            const int g = i / seg_len;
+            if (me < left && (me == 0 || sh.list_i[me - 1] / seg_len != g)) {
+              double sum = 0.0;
+              for (int j = me; j < left && sh.list_i[j] / seg_len == g; j++) sum += ws[j];
+              sh.seg_sum[g] += sum;
+            }
+            by_index = true;
           }
-          if (me == (chosen < BLOCK ? chosen : last)) write_result(a, r, i, x, m, s.inv_t, total);
         } else {
-          if (!cut) {  // everything above the bound
-            lo = key_from;
-            hi = key_from - 1;
-            ties = 0;
+          if (!cut) {  // everything from the bound on
+            lo = from;
+            hi = m;
             ordered = false;
           }
           // ---- what is kept, by segments
           double sum_here = 0.0;
           int ties_here = 0;
           each([&](int g, bool end, int, const float* x) {
+            bool some = false;
 #pragma unroll
-            for (int j = 0; j < kLaneRun; j++) {
-              const uint32_t key = key_of(x[j]);
-              const bool tie = key >= lo && key <= hi;
-              ties_here += tie ? 1 : 0;
-              if (key > hi || (tie && !ordered)) {
+            for (int j = 0; j < kRun; j++) some |= x[j] >= lo;
+            if (__any(some))
+#pragma unroll
+              for (int j = 0; j < kRun; j++) {
+                const bool tie = x[j] >= lo && x[j] <= hi;
+                ties_here += tie ? 1 : 0;
                 const double w = weight(x[j], m, s.per_t);
-                sum_here += w >= s.q ? w : 0.0;
+                sum_here += (x[j] > hi || (tie && !ordered)) && w >= s.q ? w : 0.0;
               }
-            }
             if (end) {
               sum_here = wave_sum(sum_here);
               if (ordered) ties_here = wave_sum(ties_here);
@@ -931,20 +1055,11 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         double tie_weight = 0.0;
         int tie_before = 0;
         if (CUT && ordered) {
-          // the value in [lo, hi]: by the type's fixed bits, or (one binary32 value) lo = hi
-          const uint32_t mask = (1u << kFixedBits<T>) - 1;
-          const float t = value_of(hi & 0x80000000u ? hi & ~mask : (hi - mask) | mask);
-          tie_weight = weight(t, m, s.per_t);
+          tie_weight = weight(hi, m, s.per_t);
           if (tie_weight < s.q) tie_weight = 0.0;
           int mine = 0;
           for (int g = g0; g < g1; g++) mine += sh.seg_ties[g];
-          int run = mine;
-#pragma unroll
-          for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(run, d, 64);
-            if (lane >= d) run += o;
-          }
-          tie_before = run - mine;
+          tie_before = running_sum<64>(mine) - mine;
         }
         auto kept_ties = [&](int before, int here) { return before >= ties ? 0 : min(here, ties - before); };
         double sum = 0.0;
@@ -977,42 +1092,30 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           if (CUT && ordered) tb += sh.seg_ties[g];
         }
         const unsigned long long over = __ballot(past >= 0), any = __ballot(last >= 0);
-        const int from_lane = over ? __ffsll(over) - 1 : 63 - __clzll(any);
-        const int seg = __shfl(over ? past : last, from_lane, 64);
+        const int from_lane = over ? __ffsll(over) - 1 : (any ? 63 - __clzll(any) : 0);
+        const int seg = max(0, __shfl(over ? past : last, from_lane, 64));
         int seen = __shfl(over ? past_ties : last_ties, from_lane, 64);
         // (rounding may have put the border at the total: then the last action of the last segment)
-        double base = over ? __hiloint2double(__shfl(__double2hiint(past_before), from_lane, 64), __shfl(__double2loint(past_before), from_lane, 64))
-                           : -__builtin_inf();
+        double base = over ? shfl_f64(past_before, from_lane) : -__builtin_inf();
         bool found = false;
 #pragma unroll 1
         for (int t = 0; t < turns && !found; t++) {
-          const int at = seg * seg_len + t * kSegment + lane * kLaneRun, i = start(at);
-          float x[kLaneRun];
-          double w[kLaneRun], mine = 0.0;
+          const int at = seg * seg_len + t * kTurn + lane * kRun, i = start(at);
+          float x[kRun];
+          double w[kRun], mine = 0.0;
           values(load(at), at, x);
           int equal = 0;
 #pragma unroll
-          for (int j = 0; j < kLaneRun; j++) {
-            const uint32_t key = key_of(x[j]);
-            equal += CUT && key >= lo && key <= hi ? 1 : 0;
-          }
-          int run = equal;
-          if (CUT && ordered) {
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-              const int o = __shfl_up(run, d, 64);
-              if (lane >= d) run += o;
-            }
-          }
+          for (int j = 0; j < kRun; j++) equal += CUT && x[j] >= lo && x[j] <= hi ? 1 : 0;
+          const int run = running_sum<64>(equal);
           int rank = seen + run - equal;
-          if (CUT && ordered) seen += __shfl(run, 63, 64);
+          seen += __shfl(run, 63, 64);
 #pragma unroll
-          for (int j = 0; j < kLaneRun; j++) {
-            const uint32_t key = key_of(x[j]);
+          for (int j = 0; j < kRun; j++) {
             bool in = x[j] > -kInf;
             if (CUT) {
-              const bool tie = key >= lo && key <= hi;
-              in = key > hi || (tie && (!ordered || rank < ties));
+              const bool tie = x[j] >= lo && x[j] <= hi;
+              in = x[j] > hi || (tie && (by_index ? i + j <= tie_index : !ordered || rank < ties));
               rank += tie ? 1 : 0;
             }
             w[j] = in ? weight(x[j], m, s.per_t) : 0.0;
@@ -1023,7 +1126,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           int p_at = -1, l_at = -1;
           float p_x = 0.0f, l_x = 0.0f;
 #pragma unroll
-          for (int j = 0; j < kLaneRun; j++) {
+          for (int j = 0; j < kRun; j++) {
             b += w[j];
             if (w[j] > 0.0) {
               l_at = i + j;
