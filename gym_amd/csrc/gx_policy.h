@@ -63,6 +63,14 @@ template <int M> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
   else if constexpr (M == 32) return (uint32_t)__shfl_xor((int)v, 32, 64);
   else return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, M << 10 | 0x1F);
 }
+// a value that is the same in every lane, in scalar registers
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ double uniform(double v) { return __hiloint2double(uniform(__double2hiint(v)), uniform(__double2loint(v))); }
+__device__ __forceinline__ unsigned long long uniform(unsigned long long v) {
+  return (unsigned long long)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v);
+}
 // running sums over 16 or 64 lanes, the lane's own included.  Within a row of 16 by shifts that bring zeros in; then the
 // last lane of a row into the next (rows 1 and 3), and lane 31 into the upper half.
 template <int CTRL, int ROWS> __device__ __forceinline__ double moved_f64(double v) {

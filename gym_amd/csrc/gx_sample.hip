@@ -14,10 +14,13 @@
 #include "gx_policy.h"
 
 #ifndef GX_WB
-#define GX_WB 1024
+#define GX_WB 512
+#endif
+#ifndef GX_RB
+#define GX_RB 32
 #endif
 #ifndef GX_AHEAD
-#define GX_AHEAD 4
+#define GX_AHEAD 2
 #endif
 namespace gx {
 
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 // binary64, so step 3 is the only one that takes them of every action.  What runs for few elements is a loop: unrolled,
 // the kernel outgrew the instruction cache and took three times as long.
 constexpr int kWideSmall = 4096;
-constexpr int kAhead = 2;
+constexpr int kAhead = GX_AHEAD;
 
 // low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
 template <class T> constexpr int kFixedBits = 0;
@@ -447,35 +450,70 @@ template <int BLOCK, int BINS, int SEGMENTS> struct WideShared {
   unsigned long long bin_mass, above_mass;
 };
 
-// One value a thread, the first `size` of them (a power of two) sorted downwards; `swap` holds a value a thread.
+// One value a thread, the first `size` of them (a power of two, at least 64) sorted downwards; `swap` holds a value a thread.
+template <int D> __device__ __forceinline__ unsigned long long sort_step(unsigned long long v, bool larger) {
+  const unsigned long long o = (unsigned long long)xor_lane<D>((uint32_t)(v >> 32)) << 32 | xor_lane<D>((uint32_t)v);
+  return (v > o) == larger ? v : o;
+}
 template <int BLOCK> __device__ __forceinline__ unsigned long long block_sort(unsigned long long v, int size, unsigned long long* swap) {
   const int me = threadIdx.x;
 #pragma unroll 1
   for (int block = 2; block <= size; block <<= 1) {
+    const bool down = !(me & block);
+    if (block > 64) {
 #pragma unroll 1
-    for (int d = block >> 1; d >= 1; d >>= 1) {
-      unsigned long long o;
-      if (d >= 64) {
+      for (int d = block >> 1; d >= 64; d >>= 1) {
         __syncthreads();
         swap[me] = v;
         __syncthreads();
-        o = swap[me ^ d];
-      } else {
-        o = __shfl_xor(v, d, 64);
+        const unsigned long long o = swap[me ^ d];
+        v = (v > o) == (!(me & d) == down) ? v : o;
       }
-      const bool larger = !(me & d) == !(me & block);
-      v = (v > o) == larger ? v : o;
     }
+    // within a wave
+    if (block > 32) v = sort_step<32>(v, !(me & 32) == down);
+    if (block > 16) v = sort_step<16>(v, !(me & 16) == down);
+    if (block > 8) v = sort_step<8>(v, !(me & 8) == down);
+    if (block > 4) v = sort_step<4>(v, !(me & 4) == down);
+    if (block > 2) v = sort_step<2>(v, !(me & 2) == down);
+    v = sort_step<1>(v, !(me & 1) == down);
   }
   __syncthreads();
   return v;
 }
 
+// The largest of a run of words of logits, without unpacking them: as signed integers of their width, positive numbers
+// are in order and negative ones in reverse, below them.  So it is the largest integer, or where that is negative the
+// smallest.  (NaN: see `mode`.)
+template <int W> __device__ __forceinline__ float run_largest_32(const uint32_t* w) {
+  float v = __uint_as_float(w[0]);
+#pragma unroll
+  for (int j = 1; j < W; j++) v = __builtin_amdgcn_fmed3f(v, __uint_as_float(w[j]), kInf);
+  return v;
+}
+typedef short Half2 __attribute__((ext_vector_type(2)));
+template <class T, int W> __device__ __forceinline__ float run_largest_16(const uint32_t* w) {
+  Half2 hi = __builtin_bit_cast(Half2, w[0]), lo = hi;
+#pragma unroll
+  for (int j = 1; j < W; j++) {
+    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(Half2, w[j]));
+    lo = __builtin_elementwise_min(lo, __builtin_bit_cast(Half2, w[j]));
+  }
+  const short h = hi.x > hi.y ? hi.x : hi.y, l = lo.x < lo.y ? lo.x : lo.y;
+  const uint32_t one = (uint16_t)(h < 0 ? l : h);
+  const float v = word_value<T>(&one, 0);
+  return h >= 0 && v != v ? kInf : v;
+}
+template <class T, int W> __device__ __forceinline__ float run_largest(const uint32_t* w) {
+  if constexpr (sizeof(T) == 4) return run_largest_32<W>(w);
+  else return run_largest_16<T, W>(w);
+}
+
 template <class T, int BLOCK, int BINS, int SEGMENTS, bool CUT, bool PACKED>
 __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
-  constexpr int kWaves = BLOCK / 64, kRun = 32 / sizeof(T), kTurn = 64 * kRun;
+  constexpr int kWaves = BLOCK / 64, kRun = PACKED ? GX_RB / (int)sizeof(T) : 8, kTurn = 64 * kRun;
   __shared__ WideShared<BLOCK, BINS, SEGMENTS> sh;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
   // turns a segment takes, so that SEGMENTS are enough
   const int turns = (a.n + kTurn * SEGMENTS - 1) / (kTurn * SEGMENTS), seg_len = kTurn * turns;
   const int segments = (a.n + seg_len - 1) / seg_len;
@@ -483,13 +521,14 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
-    const RowParams s = row_params<CUT>(a, r);
+    RowParams s = row_params<CUT>(a, r);
+    s.inv_t = uniform(s.inv_t); s.per_t = uniform(s.per_t); s.p = uniform(s.p); s.q = uniform(s.q); s.k = uniform(s.k); s.u = uniform(s.u);
     // 0: logits as they are.  A NaN is then no more than any bound and weighs nothing; where the largest comes out as +inf
     // (some NaN can make it that) the row is read again with 1: NaN as -inf, and if that was not it 2: +inf in finite terms
     int mode = 0;
     // A run of logits from c on, as words.  c is i, or the last run of the row where i is closer to its end: those before
     // i are the lane's before and are taken out of the values.
-    struct Run { uint32_t w[8]; };
+    struct Run { uint32_t w[kRun * sizeof(T) / 4]; };
     auto start = [&](int i) { return min(i, a.n - kRun); };
     auto load = [&](int i) {
       Run e;
@@ -514,8 +553,8 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < kRun; j++) x[j] = j < before ? -kInf : x[j];
     };
-    // f(segment, whether this was its last turn, index of the lane's first logit, its logits) over the wave's share of the
-    // row, the next loads under way
+    // f(segment, whether this was its last turn, the lane's place in the row, its words) over the wave's share of the row,
+    // the next loads under way
     auto each = [&](auto f) {
       int g = wave, t = 0;            // of the turn at hand
       int load_g = wave, load_t = 0;  // of the next one to load
@@ -530,22 +569,28 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll
       for (int k = 0; k < kAhead; k++) e[k] = next();
 #pragma unroll 1
-      for (int q = 0; q < units; q += kAhead)
+      for (int q = 0; q < units; q++) {  // (moving the words along costs less than a body for each place)
+        const int i = g * seg_len + t * kTurn + lane * kRun;
+        const Run now = e[0];
 #pragma unroll
-        for (int k = 0; k < kAhead; k++)
-          if (q + k < units) {
-            const int i = g * seg_len + t * kTurn + lane * kRun;
-            float x[kRun];
-            values(e[k], i, x);
-            e[k] = next();
-            const bool end = t == turns - 1;
-            f(g, end, start(i), x);
-            t = end ? 0 : t + 1;
-            g += end ? kWaves : 0;
-          }
+        for (int k = 0; k + 1 < kAhead; k++) e[k] = e[k + 1];
+        e[kAhead - 1] = next();
+        const bool end = t == turns - 1;
+        f(g, end, i, now);
+        t = end ? 0 : t + 1;
+        g += end ? kWaves : 0;
+      }
     };
     // the larger of two in one instruction: their median with +inf
     auto larger_of = [](float x, float y) { return __builtin_amdgcn_fmed3f(x, y, kInf); };
+    auto largest = [&](const Run& e, int i) {
+      if (mode == 0 && !__any(i > start(i))) return run_largest<T, sizeof e.w / 4>(e.w);
+      float x[kRun], v = -kInf;
+      values(e, i, x);
+#pragma unroll
+      for (int j = 0; j < kRun; j++) v = larger_of(v, x[j]);
+      return v;
+    };
     auto block_max = [&](float v) {
       v = group_max<64>(v);
       if (lane == 0) sh.wave_f32[wave] = v;
@@ -554,7 +599,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll
       for (int w = 1; w < kWaves; w++) v = fmaxf(v, sh.wave_f32[w]);
       __syncthreads();
-      return v;
+      return uniform(v);
     };
     // running sums over the threads, the own included, and the sum of all
     auto block_running = [&](double v, double* all) {
@@ -568,7 +613,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         total += sh.wave_f64[q];
       }
       __syncthreads();
-      *all = total;
+      *all = uniform(total);
       return run;
     };
     auto block_sum = [&](double v) {
@@ -590,10 +635,10 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
       for (;; mode++) {
         float top = -kInf;
         double sum = 0.0;
-        each([&](int g, bool end, int, const float* x) {
-          float here = x[0];
-#pragma unroll
-          for (int j = 1; j < kRun; j++) here = larger_of(here, x[j]);
+        each([&](int g, bool end, int i, const Run& e) {
+          const float here = largest(e, i);
+          float x[kRun];
+          values(e, i, x);
           if (here > top) {
             sum *= weight(top, here, s.per_t);
             top = here;
@@ -631,14 +676,17 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         top = -kInf;
         bottom = kInf;
         estimate = 0.0f;
-        each([&](int, bool, int, const float* x) {
-          float here = x[0];
-#pragma unroll
-          for (int j = 1; j < kRun; j++) here = larger_of(here, x[j]);
-          if (far_k)
+        each([&](int, bool, int i, const Run& e) {
+          const float here = largest(e, i);
+          if (far_k) {
+            float x[kRun];
+            values(e, i, x);
 #pragma unroll
             for (int j = 0; j < kRun; j++) bottom = x[j] > -kInf && x[j] < bottom ? x[j] : bottom;
+          }
           if (sums) {
+            float x[kRun];
+            values(e, i, x);
             if (here > top) estimate *= __builtin_amdgcn_exp2f(fmaxf((top - here) * per_t, -150.0f));
             top = larger_of(top, here);
             if (top > -kInf)
@@ -684,12 +732,13 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             if (lane == 0) sh.bound = low;
           }
           __syncthreads();
-          from = sh.bound;
+          from = uniform(sh.bound);
         }
         // ---- ... and the bins
+        from = uniform(from);
         const float per = m > from ? (float)(BINS - 1) / (m - from) : 0.0f;
         auto bin_of = [&](float x) { return (int)fminf((m - x) * per, (float)(BINS - 1)); };
-        const uint32_t key_from = key_of(from + 0.0f), key_m = key_of(m + 0.0f);
+        const uint32_t key_from = uniform(key_of(from + 0.0f)), key_m = uniform(key_of(m + 0.0f));
         // the smallest key whose bin is below b (one past the largest where b is 0): bin_of falls as the key rises.  The
         // wave's lanes try 64 keys at once.
         auto first_key_below = [&](int b) {
@@ -699,7 +748,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           while (l < h) {
             const uint32_t step = (h - l) / 64 + 1, rest = h - l, off = (uint32_t)lane * step, at = l + (off < rest ? off : rest);
             const unsigned long long yes = __ballot(bin_of(value_of(at)) < b);
-            const uint32_t hit = yes ? (uint32_t)__ffsll(yes) - 1 : 64;
+            const uint32_t hit = uniform(yes ? (uint32_t)__ffsll(yes) - 1 : 64u);
             const uint32_t below = hit * step, before = (hit - 1) * step;
             if (hit < 64) h = l + (below < rest ? below : rest);
             if (hit > 0) l = l + (before < rest ? before : rest) + 1;
@@ -710,16 +759,23 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         auto low_value = [&](uint32_t key) { return value_of(key == kKeyMinusZero ? key + 1 : key); };
         auto high_value = [&](uint32_t key) { return value_of(key == kKeyMinusZero ? key - 1 : key); };
         // masses as integers: their sum (at most n where it is not known) stays below 2^62
+        bool exact = !sums;                        // s1 and the masses (else binary32 estimates in the same place)
+        // (of 31 bits, in the counts' place)
+        const int guess_shift = 30;
         int scale_bits = 61 - __builtin_amdgcn_frexp_exp(sums ? fmax(s1, 1.0) * 1.01 : (double)a.n);
         // the border by counts or by masses: the first bin where what lies up to its end reaches the target
+        const float guess_bits = (float)(scale_bits - guess_shift);
         auto find_bin = [&](bool mass, uint32_t want_count, unsigned long long want_mass) {
           constexpr int kEach = BINS / BLOCK;
           uint32_t c = 0;
           unsigned long long w = 0;
+          auto mass_of = [&](int b) {
+            return exact ? sh.mass[b] : (unsigned long long)sh.count[b] << guess_shift;
+          };
 #pragma unroll
           for (int e = 0; e < kEach; e++) {
             c += sh.count[threadIdx.x * kEach + e];
-            w += sh.mass[threadIdx.x * kEach + e];
+            w += mass_of(threadIdx.x * kEach + e);
           }
           uint32_t rc = c;
           unsigned long long rw = w;
@@ -738,9 +794,9 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll
           for (int e = 0; e < kEach; e++) {
             const uint32_t bc = sh.count[threadIdx.x * kEach + e];
-            const unsigned long long bw = sh.mass[threadIdx.x * kEach + e];
+            const unsigned long long bw = mass_of(threadIdx.x * kEach + e);
             const bool before = mass ? rw < want_mass : rc < want_count, after = mass ? rw + bw >= want_mass : rc + bc >= want_count;
-            if (bc && before && after) {
+            if ((bc || bw) && before && after) {
               sh.bin = threadIdx.x * kEach + e;
               sh.bin_count = bc;
               sh.bin_mass = bw;
@@ -751,7 +807,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             rw += bw;
           }
           __syncthreads();
-          return sh.bin;
+          return uniform(sh.bin);
         };
         auto all_mass = [&]() {
           unsigned long long all = 0;
@@ -763,11 +819,11 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           all = 0;
           for (int v = 0; v < kWaves; v++) all += sh.wave_u64[v];
           __syncthreads();
-          return all;
+          return uniform(all);
         };
         bool cut = false;                          // the border is known
         bool by_mass = !by_k;                      // top-k first, then top-p of what that left
-        bool first = true, exact = !sums;          // no round yet; masses and s1 are exact
+        bool first = true;                         // no round yet
         bool list = false;                         // the list holds all that is kept but what lies above it
         double above = 0.0;                        // that
         uint32_t want_count = (uint32_t)s.k;
@@ -777,7 +833,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         bool k_cut = false, k_ordered = false;
         // Each round: everything from `from` on into coarse bins (level 0), then the border's bin into finer ones.
 #pragma unroll 1
-        for (;;) {
+        while (by_k || by_p) {
           uint32_t key_lo = key_from, key_hi = key_m;  // what is binned
           int shift = 0;
           uint32_t above_count = 0;
@@ -790,11 +846,22 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             if (threadIdx.x == 0 && listing) sh.listed = 0;
             for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = 0; sh.mass[b] = 0; }
             __syncthreads();
-            const float x_lo = low_value(key_lo), x_hi = high_value(key_hi);
-            each([&](int, bool, int i, const float* x) {
+            const float x_lo = uniform(low_value(key_lo)), x_hi = uniform(high_value(key_hi));
+            each([&](int, bool, int i, const Run& e) {
+              if (!__any(largest(e, i) >= x_lo)) return;
+              float x[kRun];
+              values(e, i, x);
               uint32_t in = 0;  // which of the run
 #pragma unroll
               for (int j = 0; j < kRun; j++) in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
+              const bool append = listing && sh.listed <= (uint32_t)BLOCK;
+              if (!exact) {
+                // estimates: 24 bits are enough to find the bin, or the one beside it
+#pragma unroll
+                for (int j = 0; j < kRun; j++)
+                  if (x[j] >= x_lo) atomicAdd(&sh.count[bin_of(x[j])], (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - m, per_t, guess_bits)) + 0.5f));
+                if (!append) return;
+              }
 #pragma unroll 1
               while (in) {
                 const int j = __ffs(in) - 1;
@@ -802,41 +869,41 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
                 float v = x[0];
 #pragma unroll
                 for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
-                const int b = level ? (int)((key_hi - key_of(v + 0.0f)) >> shift) : bin_of(v);
-                // an estimate has 24 bits: enough to find the bin, or the one beside it
-                const double w = exact ? weight(v, m, s.per_t) : (double)__builtin_amdgcn_exp2f(fmaxf((v - m) * per_t, -150.0f));
-                atomicAdd(&sh.count[b], 1u);
-                atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(w, scale_bits));
-                if (listing && sh.listed <= (uint32_t)BLOCK) {
+                if (exact) {
+                  const int b = level ? (int)((key_hi - key_of(v + 0.0f)) >> shift) : bin_of(v);
+                  atomicAdd(&sh.count[b], 1u);
+                  atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(weight(v, m, s.per_t), scale_bits));
+                }
+                if (append) {
                   const uint32_t at = atomicAdd(&sh.listed, 1u);
                   if (at < (uint32_t)BLOCK) {
                     sh.list_x[at] = v;
-                    sh.list_i[at] = i + j;
+                    sh.list_i[at] = start(i) + j;
                   }
                 }
               }
             });
             __syncthreads();
-            if (listing) list = sh.listed <= (uint32_t)BLOCK;
+            if (listing) list = uniform(sh.listed) <= (uint32_t)BLOCK;
             if (level == 0) {
-              if (list || (!by_k && !by_p)) {
+              if (list) {
                 found = false;
                 break;
               }
               found = find_bin(by_mass, want_count, want_mass) >= 0;
               if (!found) break;
               if (!exact) break;
-              key_lo = first_key_below(sh.bin + 1);
-              key_hi = first_key_below(sh.bin) - 1;
+              key_lo = first_key_below(uniform(sh.bin) + 1);
+              key_hi = first_key_below(uniform(sh.bin)) - 1;
             } else {
               (void)find_bin(by_mass, want_count - above_count, want_mass - above_mass);
-              key_hi -= (uint32_t)sh.bin << shift;
+              key_hi -= (uint32_t)uniform(sh.bin) << shift;
               const uint32_t low = key_hi - ((1u << shift) - 1);
               key_lo = low > key_lo && low <= key_hi ? low : key_lo;
             }
-            above_count += sh.above_count;
-            above_mass += sh.above_mass;
-            if (sh.bin_count == 1 || !((key_hi - key_lo) >> kFixedBits<T>)) break;  // one action, or one value
+            above_count += uniform(sh.above_count);
+            above_mass += uniform(sh.above_mass);
+            if (uniform(sh.bin_count) == 1 || !((key_hi - key_lo) >> kFixedBits<T>)) break;  // one action, or one value
             const int width = 32 - __clz(key_hi - key_lo);
             shift = width > __builtin_ctz(BINS) ? width - __builtin_ctz(BINS) : 0;
             __syncthreads();
@@ -847,14 +914,16 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             // ---- 3: the exact sum; above the border's bin and its neighbours by segments, and those listed
             float x_lo = kInf, x_hi = kInf;  // nothing
             if (found) {
-              x_lo = low_value(first_key_below(sh.bin + 2));
-              x_hi = high_value(first_key_below(sh.bin - 1) - 1);
+              x_lo = uniform(low_value(first_key_below(uniform(sh.bin) + 2)));
+              x_hi = uniform(high_value(first_key_below(uniform(sh.bin) - 1) - 1));
             }
             __syncthreads();
             if (threadIdx.x == 0 && !whole_list) sh.listed = 0;
             __syncthreads();
             double sum = 0.0, here = 0.0;
-            each([&](int g, bool end, int i, const float* x) {
+            each([&](int g, bool end, int i, const Run& e) {
+              float x[kRun];
+              values(e, i, x);
               uint32_t in = 0;
 #pragma unroll
               for (int j = 0; j < kRun; j++) {
@@ -874,7 +943,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
                   const uint32_t at = atomicAdd(&sh.listed, 1u);
                   if (at < (uint32_t)BLOCK) {
                     sh.list_x[at] = v;
-                    sh.list_i[at] = i + j;
+                    sh.list_i[at] = start(i) + j;
                   }
                 }
               }
@@ -899,9 +968,9 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             scale_bits = 61 - __builtin_amdgcn_frexp_exp(s1);
             continue;
           }
-          if (whole_list || (!by_k && !by_p)) break;
-          const uint32_t bin_count = sh.bin_count;
-          const double one = found ? (double)sh.bin_mass / (double)bin_count : 0.0;
+          if (whole_list) break;
+          const uint32_t bin_count = uniform(sh.bin_count);
+          const double one = found ? uniform((double)sh.bin_mass / (double)bin_count) : 0.0;
           if (!by_mass) {
             k_cut = found;
             k_lo = key_lo;
@@ -942,8 +1011,8 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         }
         __syncthreads();
         if (list) {
-          // ---- 4: an action a thread, sorted by value where an order is asked for, then by index
-          const int n = (int)sh.listed, me = threadIdx.x;
+          // ---- 4: an action a thread, sorted by value, then what is kept by index
+          const int n = uniform((int)sh.listed), me = threadIdx.x;
           int left = n;  // of them, still in
           auto size_for = [](int count) { return count <= 64 ? 64 : 1 << (32 - __clz(count - 1)); };
           float x = me < n ? sh.list_x[me] : -kInf;
@@ -951,7 +1020,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           double w = 0.0;
           // first round: by value, and the cuts; second: by index
 #pragma unroll 1
-          for (int round = by_k || by_p ? 0 : 1; round < 2; round++) {
+          for (int round = 0; round < 2; round++) {
             const bool in = me < left;
             const unsigned long long mine = round == 0 ? (unsigned long long)key_of(x + 0.0f) << 32 | (uint32_t)~i : (unsigned long long)(uint32_t)~i << 32 | key_of(x + 0.0f);
             const unsigned long long key = block_sort<BLOCK>(in ? mine : 0, size_for(left), sh.mass);
@@ -969,8 +1038,8 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
                 sh.list_i[0] = i;
               }
               __syncthreads();
-              lo = hi = sh.list_x[0];
-              tie_index = sh.list_i[0];
+              lo = hi = uniform(sh.list_x[0]);
+              tie_index = uniform(sh.list_i[0]);
               __syncthreads();
             }
           }
@@ -1016,11 +1085,10 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           // ---- what is kept, by segments
           double sum_here = 0.0;
           int ties_here = 0;
-          each([&](int g, bool end, int, const float* x) {
-            bool some = false;
-#pragma unroll
-            for (int j = 0; j < kRun; j++) some |= x[j] >= lo;
-            if (__any(some))
+          each([&](int g, bool end, int i, const Run& e) {
+            if (__any(largest(e, i) >= lo)) {
+              float x[kRun];
+              values(e, i, x);
 #pragma unroll
               for (int j = 0; j < kRun; j++) {
                 const bool tie = x[j] >= lo && x[j] <= hi;
@@ -1028,6 +1096,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
                 const double w = weight(x[j], m, s.per_t);
                 sum_here += (x[j] > hi || (tie && !ordered)) && w >= s.q ? w : 0.0;
               }
+            }
             if (end) {
               sum_here = wave_sum(sum_here);
               if (ordered) ties_here = wave_sum(ties_here);
