@@ -8,20 +8,11 @@
 //
 // Three forms, by the number of actions:
 //   up to 8      a lane a row, every pair of actions compared (row_kernel)
-//   up to 256    16 or 64 lanes a row, the row sorted in registers where top-k or top-p ask for it (group_kernel)
+//   up to 1024   16 or 64 lanes a row, the row sorted in registers where top-k or top-p ask for it (group_kernel)
 //   more         a workgroup a row; the border of the kept set is found by histograms, never by a sort (wide_kernel)
 #include "gx_launch.h"
 #include "gx_policy.h"
 
-#ifndef GX_WB
-#define GX_WB 512
-#endif
-#ifndef GX_RB
-#define GX_RB 32
-#endif
-#ifndef GX_AHEAD
-#define GX_AHEAD 2
-#endif
 namespace gx {
 
 namespace {
@@ -184,43 +175,49 @@ __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
       double s1 = 0.0, ahead[N] = {};
 #pragma unroll
       for (int i = 0; i < N; i++) s1 += w[i];
-      const double target = s.p < 1.0 ? s.p * s1 : __builtin_inf();
+      // (never 0: what has nothing ahead of it is kept)
+      const double target = s.p < 1.0 ? fmax(s.p * s1, 1e-290) : __builtin_inf();
 #pragma unroll
       for (int i = 0; i < N; i++)
 #pragma unroll
         for (int j = i + 1; j < N; j++) {
+          // a weight or, without its upper half, something below 1e-307: as good as 0 here
           const bool later = x[j] > x[i];
-          ahead[i] += later ? w[j] : 0.0;
-          ahead[j] += later ? 0.0 : w[i];
+          ahead[i] += __hiloint2double(later ? __double2hiint(w[j]) : 0, __double2loint(w[j]));
+          ahead[j] += __hiloint2double(later ? 0 : __double2hiint(w[i]), __double2loint(w[i]));
         }
-      // nothing lies ahead of the first alone
 #pragma unroll
-      for (int i = 0; i < N; i++) w[i] = (ahead[i] < target || ahead[i] == 0.0) && w[i] >= s.q ? w[i] : 0.0;
+      for (int i = 0; i < N; i++) w[i] = ahead[i] < target ? w[i] : 0.0;
+      if (__any(s.q > 0.0))
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = w[i] >= s.q ? w[i] : 0.0;
     }
     double total = 0.0;
 #pragma unroll
     for (int i = 0; i < N; i++) total += w[i];
     const double stop = s.u * total;
-    int action = -1;
-    float chosen = 0.0f;
+    // the first past the border: as many as are not
+    int action = 0;
     double c = 0.0;
-    bool open = true;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       c += w[i];
-      // the first past the border; until one is, the last that is kept (where rounding put the border at the total)
-      if (open && w[i] > 0.0) {
-        action = i;
-        chosen = x[i];
-        open = !(c > stop);
-      }
+      action += c > stop ? 0 : 1;
     }
+    if (__any(action == N) && action == N) {  // rounding put the border at the total: the last one kept
+      action = 0;
+#pragma unroll
+      for (int i = 0; i < N; i++) action = w[i] > 0.0 ? i : action;
+    }
+    float chosen = x[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) chosen = action == i ? x[i] : chosen;
     if (m == -kInf) action = -1;
     write_result(a, r, action, chosen, m, s.inv_t, total);
   }
 }
 
-// ----------------------------------------------------- up to 256 actions ---
+// ---------------------------------------------------- up to 1024 actions ---
 // G lanes a row (16: four rows a wave), E consecutive actions a lane.  Bound by instructions.  With top-k or top-p the
 // row's values are sorted in registers (a bitonic network: the values alone, not their indices, for t and j are all that
 // is wanted), weighed in that order and summed along it; the draw then goes over the row as it lies.
@@ -315,54 +312,54 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       for (int e = 0; e < E; e++) x[e] = without_inf(x[e]);
       m = 0.0f;
     }
+    // kept: above t, and the first `ties` of those equal to it
+    float t = -kInf;
+    int ties = 0, before = 0;  // (before: at lower indices than the lane's)
+    if (CUT && __any(s.k < a.n || s.p < 1.0)) {
+      uint32_t v[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) v[e] = key_of(x[e]);
+      group_sort<G, E>(v);
+      double sw[E], sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        sw[e] = first + e < s.k ? weight(value_of(v[e]), m, s.per_t) : 0.0;
+        sum += sw[e];
+      }
+      double s1, ahead = group_before<G>(sum, &s1);
+      const double target = s.p < 1.0 ? s.p * s1 : __builtin_inf();
+      // kept: a beginning of the order.  The last one kept is t.
+      uint32_t mine = 0;
+      int kept = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const bool in = first + e == 0 || (first + e < s.k && ahead < target && sw[e] > 0.0);
+        ahead += sw[e];
+        mine = in ? v[e] : mine;
+        kept += in ? 1 : 0;
+      }
+      const unsigned long long some = group_ballot<G>(kept > 0);
+      const int last_lane = 63 - __clzll(some);
+      t = value_of((uint32_t)__shfl((int)mine, last_lane, G));
+      const int count = last_lane * E + __shfl(kept, last_lane, G);  // the lanes before it keep all of theirs
+      int above = 0, equal = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        above += __popcll(group_ballot<G>(x[e] > t));
+        equal += x[e] == t ? 1 : 0;
+      }
+      before = running_sum<G>(equal) - equal;
+      ties = count - above;
+    }
     double w[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) w[e] = weight(x[e], m, s.per_t);
-    if (CUT) {
-      if (__any(s.k < a.n || s.p < 1.0)) {
-        uint32_t key[E], v[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) key[e] = v[e] = key_of(x[e]);
-        group_sort<G, E>(v);
-        double sw[E], sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          sw[e] = first + e < s.k ? weight(value_of(v[e]), m, s.per_t) : 0.0;
-          sum += sw[e];
-        }
-        double s1, ahead = group_before<G>(sum, &s1);
-        const double target = s.p < 1.0 ? s.p * s1 : __builtin_inf();
-        // kept: a beginning of the order.  The last one kept is t.
-        uint32_t mine = 0;
-        int kept = 0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const bool in = first + e == 0 || (first + e < s.k && ahead < target && sw[e] > 0.0);
-          ahead += sw[e];
-          mine = in ? v[e] : mine;
-          kept += in ? 1 : 0;
-        }
-        const unsigned long long some = group_ballot<G>(kept > 0);
-        const int last_lane = 63 - __clzll(some);
-        const uint32_t t = (uint32_t)__shfl((int)mine, last_lane, G);
-        const int count = last_lane * E + __shfl(kept, last_lane, G);  // the lanes before it keep all of theirs
-        int above = 0, equal = 0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          above += __popcll(group_ballot<G>(key[e] > t));
-          equal += key[e] == t ? 1 : 0;
-        }
-        int before = running_sum<G>(equal) - equal;  // ties at lower indices
-        const int ties = count - above;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const bool tie = key[e] == t;
-          w[e] = key[e] > t || (tie && before < ties) ? w[e] : 0.0;
-          before += tie ? 1 : 0;
-        }
+    for (int e = 0; e < E; e++) {
+      w[e] = weight(x[e], m, s.per_t);
+      if (CUT) {
+        const bool tie = x[e] == t;
+        w[e] = (x[e] > t || (tie && before < ties)) && w[e] >= s.q ? w[e] : 0.0;
+        before += tie ? 1 : 0;
       }
-#pragma unroll
-      for (int e = 0; e < E; e++) w[e] = w[e] >= s.q ? w[e] : 0.0;
     }
     double sum = 0.0, total;
 #pragma unroll
@@ -393,7 +390,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
   }
 }
 
-// --------------------------------------------------- more than 256 actions ---
+// -------------------------------------------------- more than 1024 actions ---
 // A workgroup a row, which it reads from memory once and again from the caches.  The row is cut into at most SEGMENTS
 // stretches, a wave each, 32 bytes of consecutive logits a lane and turn.
 //
@@ -411,7 +408,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 // binary64, so step 3 is the only one that takes them of every action.  What runs for few elements is a loop: unrolled,
 // the kernel outgrew the instruction cache and took three times as long.
 constexpr int kWideSmall = 4096;
-constexpr int kAhead = GX_AHEAD;
+constexpr int kAhead = 2;
 
 // low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
 template <class T> constexpr int kFixedBits = 0;
@@ -509,9 +506,9 @@ template <class T, int W> __device__ __forceinline__ float run_largest(const uin
   else return run_largest_16<T, W>(w);
 }
 
-template <class T, int BLOCK, int BINS, int SEGMENTS, bool CUT, bool PACKED>
+template <class T, int BLOCK, int BINS, int SEGMENTS, int RUN_BYTES, bool CUT, bool PACKED>
 __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
-  constexpr int kWaves = BLOCK / 64, kRun = PACKED ? GX_RB / (int)sizeof(T) : 8, kTurn = 64 * kRun;
+  constexpr int kWaves = BLOCK / 64, kRun = PACKED ? RUN_BYTES / (int)sizeof(T) : 8, kTurn = 64 * kRun;
   __shared__ WideShared<BLOCK, BINS, SEGMENTS> sh;
   const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
   // turns a segment takes, so that SEGMENTS are enough
@@ -1245,10 +1242,10 @@ template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArg
     hipLaunchKernelGGL((group_kernel<T, G, E, CUT, PACKED>), grid(kBlock / G), dim3(kBlock), 0, stream, a);                   \
     return hipGetLastError();                                                                                                 \
   }
-  GX_GROUP(16, 1) GX_GROUP(16, 2) GX_GROUP(16, 4) GX_GROUP(64, 2) GX_GROUP(64, 4)
+  GX_GROUP(16, 1) GX_GROUP(16, 2) GX_GROUP(16, 4) GX_GROUP(64, 2) GX_GROUP(64, 4) GX_GROUP(64, 8) GX_GROUP(64, 16)
 #undef GX_GROUP
-  if (a.n <= kWideSmall) hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, CUT, PACKED>), grid(1), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((wide_kernel<T, GX_WB, 2048, 1024, CUT, PACKED>), grid(1), dim3(GX_WB), 0, stream, a);
+  if (a.n <= kWideSmall) hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED>), grid(1), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((wide_kernel<T, 512, 2048, 1024, 32, CUT, PACKED>), grid(1), dim3(512), 0, stream, a);
   return hipGetLastError();
 }
 
