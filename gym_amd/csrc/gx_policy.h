@@ -71,33 +71,24 @@ __device__ __forceinline__ double uniform(double v) { return __hiloint2double(un
 __device__ __forceinline__ unsigned long long uniform(unsigned long long v) {
   return (unsigned long long)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v);
 }
-// running sums over 16 or 64 lanes, the lane's own included.  Within a row of 16 by shifts that bring zeros in; then the
-// last lane of a row into the next (rows 1 and 3), and lane 31 into the upper half.
-template <int CTRL, int ROWS> __device__ __forceinline__ double moved_f64(double v) {
-  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, true);
-  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, true);
-  return __hiloint2double(hi, lo);
+// Running sums over groups of G lanes, the lane's own included.  Within a row of 16 by shifts that bring zeros in (and
+// where a group is less than a row, nothing from the group before); then the last lane of a row into the next (rows 1
+// and 3), and lane 31 into the upper half.
+template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true); }
+template <int CTRL, int ROWS> __device__ __forceinline__ double moved(double v) {
+  return __hiloint2double(moved<CTRL, ROWS>(__double2hiint(v)), moved<CTRL, ROWS>(__double2loint(v)));
 }
-template <int G> __device__ __forceinline__ double running_sum(double v) {
-  v += moved_f64<0x111, 0xF>(v);
-  v += moved_f64<0x112, 0xF>(v);
-  v += moved_f64<0x114, 0xF>(v);
-  v += moved_f64<0x118, 0xF>(v);
-  if constexpr (G == 64) {
-    v += moved_f64<0x142, 0xA>(v);  // row_bcast 15
-    v += moved_f64<0x143, 0xC>(v);  // row_bcast 31
-  }
-  return v;
+template <int G, int D, class T> __device__ __forceinline__ T shifted_in(T v) {
+  const T o = moved<0x110 + D, 0xF>(v);
+  return G >= 16 || (threadIdx.x & (G - 1)) >= D ? o : (T)0;
 }
-template <int G> __device__ __forceinline__ int running_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  if constexpr (G == 64) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);
-  }
+template <int G, class T> __device__ __forceinline__ T running_sum(T v) {
+  if constexpr (G > 1) v += shifted_in<G, 1>(v);
+  if constexpr (G > 2) v += shifted_in<G, 2>(v);
+  if constexpr (G > 4) v += shifted_in<G, 4>(v);
+  if constexpr (G > 8) v += shifted_in<G, 8>(v);
+  if constexpr (G > 16) v += moved<0x142, 0xA>(v);  // row_bcast 15
+  if constexpr (G > 32) v += moved<0x143, 0xC>(v);  // row_bcast 31
   return v;
 }
 __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {

@@ -221,30 +221,33 @@ __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
 // G lanes a row (16: four rows a wave), E consecutive actions a lane.  Bound by instructions.  With top-k or top-p the
 // row's values are sorted in registers (a bitonic network: the values alone, not their indices, for t and j are all that
 // is wanted), weighed in that order and summed along it; the draw then goes over the row as it lies.
-template <int M> struct Bit { static constexpr int value = M; };
+template <int M> __device__ __forceinline__ float max_with(float v) { return fmaxf(v, __uint_as_float(xor_lane<M>(__float_as_uint(v)))); }
 template <int G> __device__ __forceinline__ float group_max(float v) {
-  auto other = [](float f, auto m) { return __uint_as_float(xor_lane<decltype(m)::value>(__float_as_uint(f))); };
-  v = fmaxf(v, other(v, Bit<1>()));
-  v = fmaxf(v, other(v, Bit<2>()));
-  v = fmaxf(v, other(v, Bit<4>()));
-  v = fmaxf(v, other(v, Bit<8>()));
-  if (G == 64) {
-    v = fmaxf(v, other(v, Bit<16>()));
-    v = fmaxf(v, other(v, Bit<32>()));
-  }
+  if constexpr (G > 1) v = max_with<1>(v);
+  if constexpr (G > 2) v = max_with<2>(v);
+  if constexpr (G > 4) v = max_with<4>(v);
+  if constexpr (G > 8) v = max_with<8>(v);
+  if constexpr (G > 16) v = max_with<16>(v);
+  if constexpr (G > 32) v = max_with<32>(v);
   return v;
 }
 // sums over the lanes of a group before this one
 template <int G> __device__ __forceinline__ double group_before(double v, double* all) {
+  if constexpr (G == 1) {
+    *all = v;
+    return 0.0;
+  }
   const double run = running_sum<G>(v);
   *all = shfl_f64(run, G - 1, G);
-  const double before = moved_f64<0x138, 0xF>(run);  // from the lane before, of all 64
+  const double before = moved<0x138, 0xF>(run);  // from the lane before, of all 64
   return threadIdx.x & (G - 1) ? before : 0.0;
 }
 template <int G> __device__ __forceinline__ unsigned long long group_ballot(bool b) {
+  if constexpr (G == 1) return b ? 1 : 0;
   const unsigned long long m = __ballot(b);
   return G == 64 ? m : (m >> (threadIdx.x & 63 & ~(G - 1))) & ((1ull << (G & 63)) - 1);
 }
+template <int G> __device__ __forceinline__ int group_lane(int v, int lane) { return G == 1 ? v : __shfl(v, lane, G); }
 
 __device__ __forceinline__ uint32_t med3(uint32_t a, uint32_t b, uint32_t c) {
   return max(min(a, b), min(max(a, b), c));
@@ -340,8 +343,8 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       }
       const unsigned long long some = group_ballot<G>(kept > 0);
       const int last_lane = 63 - __clzll(some);
-      t = value_of((uint32_t)__shfl((int)mine, last_lane, G));
-      const int count = last_lane * E + __shfl(kept, last_lane, G);  // the lanes before it keep all of theirs
+      t = value_of((uint32_t)group_lane<G>((int)mine, last_lane));
+      const int count = last_lane * E + group_lane<G>(kept, last_lane);  // the lanes before it keep all of theirs
       int above = 0, equal = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
@@ -1242,7 +1245,7 @@ template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArg
     hipLaunchKernelGGL((group_kernel<T, G, E, CUT, PACKED>), grid(kBlock / G), dim3(kBlock), 0, stream, a);                   \
     return hipGetLastError();                                                                                                 \
   }
-  GX_GROUP(16, 1) GX_GROUP(16, 2) GX_GROUP(16, 4) GX_GROUP(64, 2) GX_GROUP(64, 4) GX_GROUP(64, 8) GX_GROUP(64, 16)
+  GX_GROUP(1, 16) GX_GROUP(2, 16) GX_GROUP(4, 16) GX_GROUP(8, 16) GX_GROUP(16, 16) GX_GROUP(32, 16) GX_GROUP(64, 16)
 #undef GX_GROUP
   if (a.n <= kWideSmall) hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED>), grid(1), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((wide_kernel<T, 512, 2048, 1024, 32, CUT, PACKED>), grid(1), dim3(512), 0, stream, a);
