@@ -410,8 +410,35 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 // then the segment u falls into, and in it the action.  The passes are bound by instructions: 20 an exponential in
 // binary64, so step 3 is the only one that takes them of every action.  What runs for few elements is a loop: unrolled,
 // the kernel outgrew the instruction cache and took three times as long.
+//
+// Few rows leave most of the card idle, so each is split among several workgroups (parts), and the steps become launches
+// that hand their results on in the workspace: kPartMax is step 1, kPartList step 2 (and for min-p alone the segments'
+// sums), kPartExact step 3, kPartJoin the rest, by one workgroup a row.  Where a step says that the row needs more than
+// that (a list too long, +inf among the logits, k above kListMost), kPartJoin goes through the row by itself.
 constexpr int kWideSmall = 4096;
 constexpr int kAhead = 2;
+#ifndef GX_PA
+#define GX_PA 8192
+#endif
+constexpr int kPartActions = GX_PA;  // actions a part has at least
+enum Part { kWhole = 0, kPartMax = 1, kPartList = 2, kPartExact = 3, kPartJoin = 4 };
+constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock;
+
+struct SplitRow {
+  double sum[kMostParts];       // of each part: exact, and estimated relative to its largest logit
+  double estimate[kMostParts];
+  float top[kMostParts];        // its largest logit
+  float bound[kMostParts];      // what k of its lanes' largest reach, or -inf
+  float share[kMostParts];      // what 2 k / parts of them reach: half the parts together have k that reach their median
+  uint32_t listed, around;      // lengths of the lists; more than kListMost: not kept
+  float list_x[kListMost];      // what may be kept
+  int list_i[kListMost];
+  float around_x[kListMost];    // what lies around top-p's border
+  int around_i[kListMost];
+  uint32_t bins[kWideBins];     // estimates
+  double seg_sum[kWideSegments];
+  float seg_max[kWideSegments];
+};
 
 // low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
 template <class T> constexpr int kFixedBits = 0;
@@ -509,17 +536,24 @@ template <class T, int W> __device__ __forceinline__ float run_largest(const uin
   else return run_largest_16<T, W>(w);
 }
 
-template <class T, int BLOCK, int BINS, int SEGMENTS, int RUN_BYTES, bool CUT, bool PACKED>
-__global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
+__host__ __device__ __forceinline__ int share_of(int k, int parts) { return (2 * k + parts - 1) / parts; }
+
+template <class T, int BLOCK, int BINS, int SEGMENTS, int RUN_BYTES, bool CUT, bool PACKED, Part PART>
+__global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, SplitRow* split) {
+  constexpr bool kOnePart = PART == kPartMax || PART == kPartList || PART == kPartExact;  // of a row, not all of it
   constexpr int kWaves = BLOCK / 64, kRun = PACKED ? RUN_BYTES / (int)sizeof(T) : 8, kTurn = 64 * kRun;
   __shared__ WideShared<BLOCK, BINS, SEGMENTS> sh;
   const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
   // turns a segment takes, so that SEGMENTS are enough
   const int turns = (a.n + kTurn * SEGMENTS - 1) / (kTurn * SEGMENTS), seg_len = kTurn * turns;
   const int segments = (a.n + seg_len - 1) / seg_len;
-  const int units = ((segments - wave + kWaves - 1) / kWaves) * turns;  // turns of this wave
-
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  for (uint64_t item = blockIdx.x; item < (kOnePart ? a.rows * (uint64_t)parts : a.rows); item += gridDim.x) {
+    const uint64_t r = kOnePart ? item / (uint64_t)parts : item;
+    const int part = kOnePart ? (int)(item % (uint64_t)parts) : 0;
+    // its segments, and the turns of this wave among them
+    const int g_first = kOnePart ? (int)((int64_t)segments * part / parts) : 0, g_last = kOnePart ? (int)((int64_t)segments * (part + 1) / parts) : segments;
+    const int units = max(0, (g_last - g_first - wave + kWaves - 1) / kWaves) * turns;
+    SplitRow* const sr = split + (PART == kWhole ? 0 : r);
     const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
     RowParams s = row_params<CUT>(a, r);
     s.inv_t = uniform(s.inv_t); s.per_t = uniform(s.per_t); s.p = uniform(s.p); s.q = uniform(s.q); s.k = uniform(s.k); s.u = uniform(s.u);
@@ -556,8 +590,8 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
     // f(segment, whether this was its last turn, the lane's place in the row, its words) over the wave's share of the row,
     // the next loads under way
     auto each = [&](auto f) {
-      int g = wave, t = 0;            // of the turn at hand
-      int load_g = wave, load_t = 0;  // of the next one to load
+      int g = g_first + wave, t = 0;            // of the turn at hand
+      int load_g = g_first + wave, load_t = 0;  // of the next one to load
       auto next = [&]() {
         const int i = load_g * seg_len + load_t * kTurn + lane * kRun;
         const bool end = load_t == turns - 1;
@@ -629,13 +663,23 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
     int ties = 0, tie_index = 0;
     bool ordered = false, by_index = false;
     bool done = false;  // the action is written
+    // the segments' results of an earlier launch
+    auto segments_of_split = [&]() {
+      for (int g = threadIdx.x; g < segments; g += BLOCK) {
+        sh.seg_sum[g] = sr->seg_sum[g];
+        if (!CUT) sh.seg_max[g] = sr->seg_max[g];
+      }
+      __syncthreads();
+    };
     if (!CUT) {
       // largest logit and sum of a segment: a lane's own first, then the wave's
+      bool have = PART == kPartJoin;
+      if (have) segments_of_split();
 #pragma unroll 1
-      for (;; mode++) {
+      for (;; mode += have ? 0 : 1, have = false) {
         float top = -kInf;
         double sum = 0.0;
-        each([&](int g, bool end, int i, const Run& e) {
+        if (!have) each([&](int g, bool end, int i, const Run& e) {
           const float here = largest(e, i);
           float x[kRun];
           values(e, i, x);
@@ -650,27 +694,84 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             const float seg_top = group_max<64>(top);
             sum = wave_sum(top > -kInf ? sum * weight(top, seg_top, s.per_t) : 0.0);
             if (lane == 0) {
-              sh.seg_max[g] = seg_top;
-              sh.seg_sum[g] = sum;
+              (kOnePart ? sr->seg_max : sh.seg_max)[g] = seg_top;
+              (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = sum;
             }
             top = -kInf;
             sum = 0.0;
           }
         });
+        if (kOnePart) break;
         __syncthreads();
         m = -kInf;
         for (int g = threadIdx.x; g < segments; g += BLOCK) m = fmaxf(m, sh.seg_max[g]);
         m = block_max(m);
         if (m < kInf) break;
       }
+      if (kOnePart) continue;
       for (int g = threadIdx.x; g < segments; g += BLOCK)
         if (sh.seg_max[g] > -kInf) sh.seg_sum[g] *= weight(sh.seg_max[g], m, s.per_t);
       __syncthreads();
     } else {
       const bool by_k = s.k < a.n, by_p = s.p < 1.0, sums = by_p && !by_k, far_k = by_k && s.k > BLOCK;
-      // ---- 1: the largest logit, the estimate of the sum, and where it is wanted the smallest finite one
-      float top, bottom, estimate;
       const float per_t = fminf((float)s.per_t, 3e38f);
+      bool list = false;    // the list holds all that is kept but what lies above it
+      bool summed = false;  // the segments' sums of what is kept are there
+      bool taken = false;   // either, by earlier launches
+      double above = 0.0;   // what lies above the list
+      double s1 = 0.0;      // the sum (of all; for top-p alone)
+      float split_bound = -kInf;
+      if (PART >= kPartList) {
+        const bool mine = (int)threadIdx.x < parts;
+        m = block_max(mine ? sr->top[threadIdx.x] : -kInf);
+        if (kOnePart && (far_k || m == kInf || m == -kInf || (PART == kPartExact && !sums))) continue;
+        if (m < kInf && m > -kInf) {
+          if (PART != kPartJoin) {
+            if (sums) s1 = block_sum(mine ? sr->estimate[threadIdx.x] * weight(sr->top[threadIdx.x], m, s.per_t) : 0.0);
+            if (by_k) {
+              // what one part's lanes reach alone; or what enough parts reach with their share (see kPartMax)
+              split_bound = block_max(mine ? sr->bound[threadIdx.x] : -kInf);
+              const int share = min(share_of(s.k, parts), s.k), need = (s.k + share - 1) / share;
+              const float b = lane < parts ? sr->share[lane] : -kInf;
+              int rank = 0;
+              for (int j = 0; j < parts; j++) {
+                const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(b), j));
+                rank += o > b || (o == b && j < lane) ? 1 : 0;
+              }
+              const unsigned long long who = __ballot(lane < parts && rank == need - 1);
+              split_bound = fmaxf(split_bound, __shfl(b, __ffsll(who) - 1, 64));
+            }
+          } else if (!far_k) {
+            const uint32_t listed = uniform(sr->listed), around = uniform(sr->around);
+            if (sums) s1 = block_sum(mine ? sr->sum[threadIdx.x] : 0.0);
+            list = taken = (by_k || by_p) && listed <= (uint32_t)kListMost;
+            if (list) {
+              if (threadIdx.x == 0) sh.listed = listed;
+              sh.list_x[threadIdx.x] = sr->list_x[threadIdx.x];
+              sh.list_i[threadIdx.x] = sr->list_i[threadIdx.x];
+              __syncthreads();
+            } else if (sums && around <= (uint32_t)kListMost) {
+              segments_of_split();
+              double sum = 0.0;
+              for (int g = threadIdx.x; g < segments; g += BLOCK) sum += sh.seg_sum[g];
+              above = block_sum(sum);
+              if (threadIdx.x == 0) sh.listed = around;
+              const float v = threadIdx.x < around ? sr->around_x[threadIdx.x] : -kInf;
+              sh.list_x[threadIdx.x] = v;
+              sh.list_i[threadIdx.x] = sr->around_i[threadIdx.x];
+              const double within = block_sum(weight(v, m, s.per_t));
+              list = taken = above < s.p * s1 && s.p * s1 <= above + within;
+              if (!list) above = 0.0;
+            } else if (!by_k && !by_p) {
+              segments_of_split();
+              summed = taken = true;
+            }
+          }
+        }
+      }
+      // ---- 1: the largest logit, the estimate of the sum, and where it is wanted the smallest finite one
+      float top = -kInf, bottom = kInf, estimate = 0.0f;
+      if ((PART == kWhole || PART == kPartMax || PART == kPartJoin) && !taken)
 #pragma unroll 1
       for (;; mode++) {
         top = -kInf;
@@ -697,23 +798,38 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           }
         });
         m = block_max(top);
-        if (m < kInf) break;
+        if (m < kInf || PART == kPartMax) break;
+      }
+      if (PART == kPartMax) {
+        s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;  // (beside +inf: unused)
+        if (part == 0)
+          for (int b = threadIdx.x; b < kWideBins; b += BLOCK) sr->bins[b] = 0;
+        if (threadIdx.x == 0) {
+          sr->top[part] = m;
+          sr->estimate[part] = s1;
+          sr->bound[part] = sr->share[part] = -kInf;
+          if (part == 0) sr->listed = sr->around = 0;
+        }
+        if (!by_k || far_k || !(m > -kInf && m < kInf)) continue;
       }
       if (m > -kInf) {
-        if (far_k) bottom = -block_max(-bottom);
-        double s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;
+        if (!kOnePart && !taken) {
+          if (far_k) bottom = -block_max(-bottom);
+          s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;
+        }
         // ---- 2: a bound below everything that can be kept (weights below exp(-745) are 0) ...
         double bound = (double)m - 745.0 / s.inv_t;
         if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * s1 * 0.99 / (double)a.n, 1e-320)) / s.inv_t);
         if (!by_k && s.q > 0.0) bound = fmax(bound, (double)m + log(s.q) / s.inv_t);
         float from = fminf(m, fmaxf((float)(bound - fabs(bound) * 1e-6), -3.402823466e38f));
         if (far_k) from = fminf(m, fmaxf(bottom, from));
-        if (by_k && !far_k) {
+        if (by_k && !far_k && (PART == kPartList || PART == kPartExact)) from = fminf(m, fmaxf(from, split_bound));
+        if (by_k && !far_k && !taken && (!kOnePart || PART == kPartMax)) {
           // a value that k lanes' largest reach: halving between the bound and the largest, one wave's work
           sh.list_x[threadIdx.x] = top;
           __syncthreads();
           if (wave == 0) {
-            float v[kWaves], low = from, high = m;
+            float v[kWaves];
 #pragma unroll
             for (int q = 0; q < kWaves; q++) v[q] = sh.list_x[q * 64 + lane];
             auto reach = [&](float x) {
@@ -722,18 +838,31 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
               for (int q = 0; q < kWaves; q++) c += __popcll(__ballot(v[q] >= x));
               return c;
             };
-            const bool some = reach(low) >= s.k;
+            auto reached_by = [&](int count, float low) {
+              if (reach(low) < count) return -kInf;
+              float high = m;
 #pragma unroll 1
-            for (int step = 0; some && step < 14; step++) {
-              const float mid = low + (high - low) * 0.5f;
-              if (!(mid > low && mid < high)) break;
-              if (reach(mid) >= s.k) low = mid; else high = mid;
+              for (int step = 0; step < 14; step++) {
+                const float mid = low + (high - low) * 0.5f;
+                if (!(mid > low && mid < high)) break;
+                if (reach(mid) >= count) low = mid; else high = mid;
+              }
+              return low;
+            };
+            const float b = reached_by(s.k, from);
+            const float share = PART == kPartMax ? reached_by(min(share_of(s.k, parts), s.k), from) : 0.0f;
+            if (lane == 0) {
+              sh.bound = fmaxf(from, b);
+              if (PART == kPartMax) {
+                sr->bound[part] = b;
+                sr->share[part] = share;
+              }
             }
-            if (lane == 0) sh.bound = low;
           }
           __syncthreads();
           from = uniform(sh.bound);
         }
+        if (PART == kPartMax) continue;
         // ---- ... and the bins
         from = uniform(from);
         const float per = m > from ? (float)(BINS - 1) / (m - from) : 0.0f;
@@ -821,11 +950,21 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           __syncthreads();
           return uniform(all);
         };
+        // those of a list of this workgroup's that is not too long, into the row's
+        auto hand_on = [&](uint32_t* count, float* to_x, int* to_i) {
+          const uint32_t n = uniform(sh.listed);
+          if (threadIdx.x == 0) sh.bin = (int)atomicAdd(count, n <= (uint32_t)kListMost ? n : (uint32_t)kListMost + 1);
+          __syncthreads();
+          const uint32_t at = (uint32_t)sh.bin + threadIdx.x;
+          if (n <= (uint32_t)kListMost && threadIdx.x < n && at < (uint32_t)kListMost) {
+            to_x[at] = sh.list_x[threadIdx.x];
+            to_i[at] = sh.list_i[threadIdx.x];
+          }
+          __syncthreads();
+        };
         bool cut = false;                          // the border is known
         bool by_mass = !by_k;                      // top-k first, then top-p of what that left
         bool first = true;                         // no round yet
-        bool list = false;                         // the list holds all that is kept but what lies above it
-        double above = 0.0;                        // that
         uint32_t want_count = (uint32_t)s.k;
         unsigned long long want_mass = 0;
         uint32_t k_lo = 0, k_hi = 0;               // top-k's border
@@ -833,7 +972,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
         bool k_cut = false, k_ordered = false;
         // Each round: everything from `from` on into coarse bins (level 0), then the border's bin into finer ones.
 #pragma unroll 1
-        while (by_k || by_p) {
+        while ((by_k || by_p) && !taken) {
           uint32_t key_lo = key_from, key_hi = key_m;  // what is binned
           int shift = 0;
           uint32_t above_count = 0;
@@ -843,11 +982,11 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 #pragma unroll 1
           for (int level = 0;; level++) {
             const bool listing = first && level == 0;
-            if (threadIdx.x == 0 && listing) sh.listed = 0;
-            for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = 0; sh.mass[b] = 0; }
+            if (threadIdx.x == 0 && listing) sh.listed = PART == kPartExact ? sr->listed : 0;
+            for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = PART == kPartExact ? sr->bins[b] : 0; sh.mass[b] = 0; }
             __syncthreads();
             const float x_lo = uniform(low_value(key_lo)), x_hi = uniform(high_value(key_hi));
-            each([&](int, bool, int i, const Run& e) {
+            if (PART != kPartExact) each([&](int, bool, int i, const Run& e) {
               if (!__any(largest(e, i) >= x_lo)) return;
               float x[kRun];
               values(e, i, x);
@@ -884,6 +1023,13 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
               }
             });
             __syncthreads();
+            if (PART == kPartList) {
+              hand_on(&sr->listed, sr->list_x, sr->list_i);
+              if (sums)
+                for (int b = threadIdx.x; b < BINS; b += BLOCK)
+                  if (sh.count[b]) atomicAdd(&sr->bins[b], sh.count[b]);
+              break;
+            }
             if (listing) list = uniform(sh.listed) <= (uint32_t)BLOCK;
             if (level == 0) {
               if (list) {
@@ -908,6 +1054,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             shift = width > __builtin_ctz(BINS) ? width - __builtin_ctz(BINS) : 0;
             __syncthreads();
           }
+          if (PART == kPartList) break;
           const bool whole_list = first && list;
           first = false;
           if (!exact) {
@@ -949,12 +1096,21 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
               }
               if (end) {
                 here = wave_sum(here);
-                if (lane == 0) sh.seg_sum[g] = here;
+                if (lane == 0) (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = here;
                 here = 0.0;
               }
             });
             s1 = block_sum(sum);
             exact = true;
+            if (PART == kPartExact) {
+              if (threadIdx.x == 0) {
+                sr->sum[part] = s1;
+                if (!found && !whole_list) sh.listed = kListMost + 1;  // no border: kPartJoin is to find it
+              }
+              __syncthreads();
+              if (!whole_list) hand_on(&sr->around, sr->around_x, sr->around_i);
+              break;
+            }
             if (whole_list) break;
             if (found && sh.listed <= (uint32_t)BLOCK) {
               double mine = 0.0;
@@ -1010,6 +1166,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
           break;
         }
         __syncthreads();
+        if (PART == kPartExact || (PART == kPartList && (by_k || by_p))) continue;
         if (list) {
           // ---- 4: an action a thread, sorted by value, then what is kept by index
           const int n = uniform((int)sh.listed), me = threadIdx.x;
@@ -1082,6 +1239,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
             hi = m;
             ordered = false;
           }
+          if (!summed) {
           // ---- what is kept, by segments
           double sum_here = 0.0;
           int ties_here = 0;
@@ -1101,17 +1259,19 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
               sum_here = wave_sum(sum_here);
               if (ordered) ties_here = wave_sum(ties_here);
               if (lane == 0) {
-                sh.seg_sum[g] = sum_here;
+                (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = sum_here;
                 sh.seg_ties[g] = ties_here;
               }
               sum_here = 0.0;
               ties_here = 0;
             }
           });
+          }
         }
         __syncthreads();
       }
     }
+    if (kOnePart) continue;
 
     // ---- the segment, and in it the action: one wave's work
     if (wave == 0 && !done) {
@@ -1224,11 +1384,21 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a) {
 
 }  // namespace
 
-size_t sample_workspace(const SampleArgs&, int) { return 0; }
+namespace {
+// Workgroups a row of the large form takes: more than one where the rows alone would leave half the card idle.
+int split_parts(const SampleArgs& a, int num_cus) {
+  if (a.n <= kWideSmall || a.rows * 2 > (uint64_t)num_cus) return 1;
+  const int by_rows = num_cus / (int)a.rows, by_size = a.n / kPartActions;
+  const int parts = by_rows < by_size ? by_rows : by_size;
+  return parts < kMostParts ? parts : kMostParts;
+}
+}  // namespace
+
+size_t sample_workspace(const SampleArgs& a, int num_cus) { return a.rows && split_parts(a, num_cus) > 1 ? a.rows * sizeof(SplitRow) : 0; }
 
 namespace {
 
-template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArgs& a, int num_cus, hipStream_t stream) {
+template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArgs& a, SplitRow* split, int num_cus, hipStream_t stream) {
   // a launch has fewer than 2^32 threads, and grids beyond what the card holds gain nothing: the workgroups go round
   auto grid = [&](uint64_t per_group) {
     const uint64_t groups = (a.rows + per_group - 1) / per_group, most = (uint64_t)num_cus * 64;
@@ -1247,25 +1417,44 @@ template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArg
   }
   GX_GROUP(1, 16) GX_GROUP(2, 16) GX_GROUP(4, 16) GX_GROUP(8, 16) GX_GROUP(16, 16) GX_GROUP(32, 16) GX_GROUP(64, 16)
 #undef GX_GROUP
-  if (a.n <= kWideSmall) hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED>), grid(1), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((wide_kernel<T, 512, 2048, 1024, 32, CUT, PACKED>), grid(1), dim3(512), 0, stream, a);
+  if (a.n <= kWideSmall) {
+    hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED, kWhole>), grid(1), dim3(256), 0, stream, a, 1, nullptr);
+    return hipGetLastError();
+  }
+#define GX_WIDE(PART, GRID) \
+  hipLaunchKernelGGL((wide_kernel<T, kWideBlock, kWideBins, kWideSegments, 32, CUT, PACKED, PART>), GRID, dim3(kWideBlock), 0, stream, a, parts, split)
+  const int parts = split_parts(a, num_cus);
+  if (parts < 2) {
+    GX_WIDE(kWhole, grid(1));
+    return hipGetLastError();
+  }
+  const dim3 all((unsigned)(a.rows * (uint64_t)parts));
+  GX_WIDE(kPartMax, all);
+  if constexpr (CUT) {
+    GX_WIDE(kPartList, all);
+    const bool top_p_alone = (a.top_p || a.top_p_all < 1.0f) && (a.top_k || a.top_k_all <= 0 || a.top_k_all >= a.n);
+    if (top_p_alone) GX_WIDE(kPartExact, all);
+  }
+  GX_WIDE(kPartJoin, grid(1));
+#undef GX_WIDE
   return hipGetLastError();
 }
 
-template <class T> hipError_t launch_typed(const SampleArgs& a, int num_cus, hipStream_t stream) {
+template <class T> hipError_t launch_typed(const SampleArgs& a, SplitRow* split, int num_cus, hipStream_t stream) {
   const bool cut = a.temperature || a.top_k || a.top_p || a.min_p || a.greedy_all || (a.top_k_all > 0 && a.top_k_all < a.n) ||
                    a.top_p_all < 1.0f || a.min_p_all > 0.0f;
   const bool packed = a.col_stride == 1;
-  if (cut) return packed ? launch_rows<T, true, true>(a, num_cus, stream) : launch_rows<T, true, false>(a, num_cus, stream);
-  return packed ? launch_rows<T, false, true>(a, num_cus, stream) : launch_rows<T, false, false>(a, num_cus, stream);
+  if (cut) return packed ? launch_rows<T, true, true>(a, split, num_cus, stream) : launch_rows<T, true, false>(a, split, num_cus, stream);
+  return packed ? launch_rows<T, false, true>(a, split, num_cus, stream) : launch_rows<T, false, false>(a, split, num_cus, stream);
 }
 
 }  // namespace
 
-hipError_t launch_sample_logits(const SampleArgs& a, int dtype, void*, int num_cus, hipStream_t stream) {
-  if (dtype == GX_F32) return launch_typed<float>(a, num_cus, stream);
-  if (dtype == GX_F16) return launch_typed<f16>(a, num_cus, stream);
-  return launch_typed<bf16>(a, num_cus, stream);
+hipError_t launch_sample_logits(const SampleArgs& a, int dtype, void* workspace, int num_cus, hipStream_t stream) {
+  SplitRow* split = static_cast<SplitRow*>(workspace);
+  if (dtype == GX_F32) return launch_typed<float>(a, split, num_cus, stream);
+  if (dtype == GX_F16) return launch_typed<f16>(a, split, num_cus, stream);
+  return launch_typed<bf16>(a, split, num_cus, stream);
 }
 
 }  // namespace gx
