@@ -417,10 +417,9 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 // that (a list too long, +inf among the logits, k above kListMost), kPartJoin goes through the row by itself.
 constexpr int kWideSmall = 4096;
 constexpr int kAhead = 2;
-#ifndef GX_PA
-#define GX_PA 8192
-#endif
-constexpr int kPartActions = GX_PA;  // actions a part has at least
+// Actions a part has at least.  One row of 131 072, top-p: 46 us with 8 192, 50 with 16 384, 44 with 4 096, whose 32 parts
+// find their lists too long sooner.
+constexpr int kPartActions = 8192;
 enum Part { kWhole = 0, kPartMax = 1, kPartList = 2, kPartExact = 3, kPartJoin = 4 };
 constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock;
 
@@ -803,7 +802,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
       if (PART == kPartMax) {
         s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;  // (beside +inf: unused)
         if (part == 0)
-          for (int b = threadIdx.x; b < kWideBins; b += BLOCK) sr->bins[b] = 0;
+          for (int b = threadIdx.x; b < BINS; b += BLOCK) sr->bins[b] = 0;
         if (threadIdx.x == 0) {
           sr->top[part] = m;
           sr->estimate[part] = s1;
@@ -825,10 +824,11 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
         if (far_k) from = fminf(m, fmaxf(bottom, from));
         if (by_k && !far_k && (PART == kPartList || PART == kPartExact)) from = fminf(m, fmaxf(from, split_bound));
         if (by_k && !far_k && !taken && (!kOnePart || PART == kPartMax)) {
-          // a value that k lanes' largest reach: halving between the bound and the largest, one wave's work
+          // a value that k lanes' largest reach: halving between the bound and the largest, one wave's work (and of a part
+          // what its share of k reach, another's)
           sh.list_x[threadIdx.x] = top;
           __syncthreads();
-          if (wave == 0) {
+          if (wave == 0 || (PART == kPartMax && wave == 1)) {
             float v[kWaves];
 #pragma unroll
             for (int q = 0; q < kWaves; q++) v[q] = sh.list_x[q * 64 + lane];
@@ -849,18 +849,14 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
               }
               return low;
             };
-            const float b = reached_by(s.k, from);
-            const float share = PART == kPartMax ? reached_by(min(share_of(s.k, parts), s.k), from) : 0.0f;
+            const float b = reached_by(wave == 0 ? s.k : min(share_of(s.k, parts), s.k), from);
             if (lane == 0) {
-              sh.bound = fmaxf(from, b);
-              if (PART == kPartMax) {
-                sr->bound[part] = b;
-                sr->share[part] = share;
-              }
+              if (PART == kPartMax) (wave == 0 ? sr->bound : sr->share)[part] = b;
+              else sh.bound = fmaxf(from, b);
             }
           }
           __syncthreads();
-          from = uniform(sh.bound);
+          if (PART != kPartMax) from = uniform(sh.bound);
         }
         if (PART == kPartMax) continue;
         // ---- ... and the bins

@@ -58,7 +58,8 @@ def check_sample(x, u, got=None, **par):
 # ------------------------------------------------------------------- sampling ---
 CUTS = [dict(), dict(temperature=0.6), dict(top_k=1), dict(top_k=3), dict(top_p=0.9), dict(min_p=0.1),
         dict(temperature=1.7, top_k=40, top_p=0.8, min_p=0.02), dict(temperature=0.0)]
-SIZES = [1, 2, 3, 4, 5, 6, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 1000, 1025, 4099]
+SIZES = [1, 2, 3, 4, 5, 6, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1000, 1024, 1025, 2500, 4096, 4097,
+         8200, 16_400]
 
 
 @pytest.mark.parametrize("n", SIZES)
@@ -81,6 +82,36 @@ def test_vocabulary(n, dtype):
         check_sample(x, u, **cut)
 
 
+def test_a_workgroup_a_row():
+    """large rows, too many of them to be split (compare with the few of test_vocabulary)"""
+    for i, (n, dtype, spread, cut) in enumerate([
+            (20_011, BF16, 2.5, dict(temperature=0.8, top_k=50, top_p=0.95)), (20_011, F32, 2.5, dict(top_p=0.9)), (20_011, F16, 2.5, dict()),
+            (9_000, F32, 0.02, dict(top_p=0.7)), (9_001, BF16, 0.05, dict(top_p=0.5)), (9_002, F32, 1.0, dict(top_k=3000, top_p=0.9)),
+            (9_003, F16, 2.0, dict(min_p=0.02)), (9_004, F32, 1.0, dict(top_k=700)), (9_005, BF16, 0.0, dict(top_k=100, top_p=0.25)),
+            (9_006, BF16, 1.0, dict(top_p=0.9, min_p=0.1)), (9_007, F32, 8.0, dict(top_p=0.99999))]):
+        x, u = make_logits(150, n, dtype, n + i, spread=spread, masked=0.2 if i % 3 == 0 else 0.0)
+        check_sample(x, u, **cut)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40, 128, 129])
+def test_split_rows(rows):
+    """the same rows split and whole give the same actions; and both the plain form's"""
+    n = 33_000
+    for i, (dtype, spread, cut) in enumerate([
+            (BF16, 2.5, dict(temperature=0.8, top_k=50, top_p=0.95)), (F32, 2.5, dict(top_p=0.9)), (F16, 2.5, dict()), (F32, 0.0, dict(top_k=7, top_p=0.5)),
+            (BF16, 0.05, dict(top_p=0.6)), (F32, 2.5, dict(min_p=0.01)), (F32, 1.0, dict(top_k=1500)), (BF16, 2.5, dict(top_k=512)),
+            (F32, 2.5, dict(top_p=0.9, min_p=0.2)), (F16, 3.0, dict(temperature=0.0))]):
+        x, u = make_logits(rows, n, dtype, 7 * rows + i, spread=spread, masked=0.1 if i % 2 else 0.0)
+        if i % 3 == 0:
+            x[:, :100] += 6  # most of what counts in one part
+        got = policy.sample_logits(x, u, **cut)
+        many, um = x.repeat(1 + 300 // rows, 1), u.repeat(1 + 300 // rows)
+        a, lp = policy.sample_logits(many, um, **cut)
+        assert torch.equal(a[:rows], got[0]) and torch.all((lp[:rows] - got[1]).abs() <= 2.0**-23 * lp[:rows].abs() + 1e-10)
+        few = slice(0, min(rows, 6))
+        check_sample(x[few], u[few], got=(got[0][few], got[1][few]), **cut)
+
+
 def test_many_rows():
     """more rows than any grid has lanes for, small action spaces: a sample of them in binary64, the rest by two runs"""
     for n, cut in [(2, {}), (4, dict(temperature=0.7, top_p=0.95)), (6, dict(top_k=3)), (17, dict(top_p=0.5))]:
@@ -98,7 +129,7 @@ def test_many_rows():
 
 
 def test_parameters_by_row():
-    for n in (4, 7, 100, 255, 700, 5000):
+    for n in (4, 7, 100, 255, 700, 3000, 5000, 30_000):
         rows = 53
         x, u = make_logits(rows, n, F32, n, masked=0.1)
         g = gen(n)
@@ -115,7 +146,7 @@ def test_parameters_by_row():
         check_sample(x, u, got=policy.sample_logits(x, u, temperature=t, top_k=k, top_p=p, min_p=q), **want)
 
 
-@pytest.mark.parametrize("n", [3, 8, 13, 40, 200, 300, 3000])
+@pytest.mark.parametrize("n", [3, 8, 13, 20, 40, 100, 200, 300, 700, 3000, 5000, 40_000])
 def test_special_values(n):
     low = {F32: torch.finfo(F32).min, F16: torch.finfo(F16).min, BF16: torch.finfo(BF16).min}
     for dtype in TYPES:
@@ -153,7 +184,7 @@ def test_random_numbers_at_their_ends(n):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n", [4, 6, 33, 200, 2050])
+@pytest.mark.parametrize("n", [4, 6, 12, 33, 200, 2050, 17_000])
 def test_strides(n, dtype):
     """column-major (the batch's own layout), padded and shifted rows, every second element, one row for all"""
     rows = 70
