@@ -1055,68 +1055,90 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
           first = false;
           if (!exact) {
             // ---- 3: the exact sum; above the border's bin and its neighbours by segments, and those listed
-            float x_lo = kInf, x_hi = kInf;  // nothing
-            if (found) {
-              x_lo = uniform(low_value(first_key_below(uniform(sh.bin) + 2)));
-              x_hi = uniform(high_value(first_key_below(uniform(sh.bin) - 1) - 1));
-            }
-            __syncthreads();
-            if (threadIdx.x == 0 && !whole_list) sh.listed = 0;
-            __syncthreads();
-            double sum = 0.0, here = 0.0;
-            each([&](int g, bool end, int i, const Run& e) {
-              float x[kRun];
-              values(e, i, x);
-              uint32_t in = 0;
-#pragma unroll
-              for (int j = 0; j < kRun; j++) {
-                const double w = weight(x[j], m, s.per_t);
-                sum += w;
-                here += x[j] > x_hi ? w : 0.0;  // above min-p's bound too, which no bin lies below
-                in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
-              }
+            int b = uniform(sh.bin);
 #pragma unroll 1
-              while (in) {
-                const int j = __ffs(in) - 1;
-                in &= in - 1;
-                float v = x[0];
-#pragma unroll
-                for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
-                if (sh.listed <= (uint32_t)BLOCK) {
-                  const uint32_t at = atomicAdd(&sh.listed, 1u);
-                  if (at < (uint32_t)BLOCK) {
-                    sh.list_x[at] = v;
-                    sh.list_i[at] = start(i) + j;
-                  }
+            for (int attempt = 0;; attempt++) {
+              float x_lo = kInf, x_hi = kInf;  // nothing
+              int beside = 0;
+              if (found) {
+                // as many bins on either side as the list should hold, at least one (logits of 16 bits may leave some empty)
+                const float one = __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits);  // a logit's weight there
+                auto in_bin = [&](int at) { return at >= 0 && at < BINS ? (float)sh.count[at] : 0.0f; };
+                float in_list = in_bin(b);
+                for (; beside < 8; beside++) {
+                  const float more = in_bin(b - beside - 1) + in_bin(b + beside + 1);
+                  if (beside > 0 && in_list + more > one * (float)(BLOCK * 5 / 8)) break;
+                  in_list += more;
                 }
-              }
-              if (end) {
-                here = wave_sum(here);
-                if (lane == 0) (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = here;
-                here = 0.0;
-              }
-            });
-            s1 = block_sum(sum);
-            exact = true;
-            if (PART == kPartExact) {
-              if (threadIdx.x == 0) {
-                sr->sum[part] = s1;
-                if (!found && !whole_list) sh.listed = kListMost + 1;  // no border: kPartJoin is to find it
+                x_lo = uniform(low_value(first_key_below(b + uniform(beside) + 1)));
+                x_hi = uniform(high_value(first_key_below(b - uniform(beside)) - 1));
               }
               __syncthreads();
-              if (!whole_list) hand_on(&sr->around, sr->around_x, sr->around_i);
+              if (threadIdx.x == 0 && !whole_list) sh.listed = 0;
+              __syncthreads();
+              double sum = 0.0, here = 0.0;
+              each([&](int g, bool end, int i, const Run& e) {
+                float x[kRun];
+                values(e, i, x);
+                uint32_t in = 0;
+#pragma unroll
+                for (int j = 0; j < kRun; j++) {
+                  const double w = weight(x[j], m, s.per_t);
+                  sum += w;
+                  here += x[j] > x_hi ? w : 0.0;  // above min-p's bound too, which no bin lies below
+                  in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
+                }
+#pragma unroll 1
+                while (in) {
+                  const int j = __ffs(in) - 1;
+                  in &= in - 1;
+                  float v = x[0];
+#pragma unroll
+                  for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
+                  if (sh.listed <= (uint32_t)BLOCK) {
+                    const uint32_t at = atomicAdd(&sh.listed, 1u);
+                    if (at < (uint32_t)BLOCK) {
+                      sh.list_x[at] = v;
+                      sh.list_i[at] = start(i) + j;
+                    }
+                  }
+                }
+                if (end) {
+                  here = wave_sum(here);
+                  if (lane == 0) (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = here;
+                  here = 0.0;
+                }
+              });
+              s1 = block_sum(sum);
+              exact = true;
+              if (PART == kPartExact) {
+                if (threadIdx.x == 0) {
+                  sr->sum[part] = s1;
+                  if (!found && !whole_list) sh.listed = kListMost + 1;  // no border: kPartJoin is to find it
+                }
+                __syncthreads();
+                if (!whole_list) hand_on(&sr->around, sr->around_x, sr->around_i);
+                break;
+              }
+              if (!whole_list && found && sh.listed <= (uint32_t)BLOCK) {
+                double mine = 0.0;
+                for (int g = threadIdx.x; g < segments; g += BLOCK) mine += sh.seg_sum[g];
+                above = block_sum(mine);
+                const float v = threadIdx.x < sh.listed ? sh.list_x[threadIdx.x] : -kInf;
+                const double within = block_sum(weight(v, m, s.per_t)), target = s.p * s1;
+                list = above < target && target <= above + within;
+                if (!list) {
+                  // next to it then: the nearest bin with anything in it, once
+                  const int way = target <= above ? -1 : 1;
+                  above = 0.0;
+                  b = uniform(b + way * (beside + 1));
+                  while (b >= 0 && b < BINS && !sh.count[b]) b += way;
+                  if (attempt == 0 && b >= 0 && b < BINS) continue;
+                }
+              }
               break;
             }
-            if (whole_list) break;
-            if (found && sh.listed <= (uint32_t)BLOCK) {
-              double mine = 0.0;
-              for (int g = threadIdx.x; g < segments; g += BLOCK) mine += sh.seg_sum[g];
-              above = block_sum(mine);
-              const float v = threadIdx.x < sh.listed ? sh.list_x[threadIdx.x] : -kInf;
-              const double within = block_sum(weight(v, m, s.per_t)), target = s.p * s1;
-              list = above < target && target <= above + within;
-            }
-            if (list) break;
+            if (PART == kPartExact || list) break;
             scale_bits = 61 - __builtin_amdgcn_frexp_exp(s1);
             continue;
           }
