@@ -15,7 +15,7 @@ LIB = os.path.join(HERE, "lib", "libgymx.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["gx_api.cpp", "gx_classic.hip", "gx_acrobot.hip", "gx_classic64.hip", "gx_acrobot64.hip", "gx_tabular.hip", "gx_blackjack.hip", "gx_pong.hip", "gx_breakout.hip", "gx_invaders.hip",
-           "gx_stats.hip", "gx_hostpath.hip", "gx_sample.hip", "gx_embed.hip"]
+           "gx_stats.hip", "gx_hostpath.hip", "gx_sample.hip", "gx_sample_f16.hip", "gx_sample_bf16.hip", "gx_embed.hip"]
 # -ffp-contract=off: EXACT mode is operation-for-operation binary32; fused
 # multiply-adds are written out explicitly where they are wanted.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

@@ -627,8 +627,14 @@ int launch_step(gx_vec* v, const void* d_actions, int k_steps, uint64_t action_s
   v->state_dirty = false;
   v->sweep_parity ^= 1u;
   if (stream != v->ctx->compute && (a.forced_draws || (has_error_flag(v) && policy == GX_POLICY_DEVICE_ACTIONS))) {
-    HIP_TRY(hipEventRecord(v->ev_foreign, stream));
-    v->foreign_pending = true;
+    // (a step that is being recorded into a graph runs when that is replayed: an event recorded here would belong to the
+    // graph, and waiting for it would fail)
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(stream, &capture));
+    if (capture == hipStreamCaptureStatusNone) {
+      HIP_TRY(hipEventRecord(v->ev_foreign, stream));
+      v->foreign_pending = true;
+    }
   }
   return GX_OK;
 }

@@ -1,1478 +1,18 @@
-// Actions from a policy's logits: temperature, top-k, top-p, min-p and a draw by a given random number (gx_sample).
-//
-// The kept set is a beginning of the order "logit descending, equal logits by index", so it is described by one logit t
-// and a count j: everything above t, and the first j (by index) of those equal to t.  Weights exp((x - m) / T) and their
-// sums are binary64 (or integers of 62 bits) throughout: which action u falls on is a border in a sum of up to 2^24 terms,
-// and a sum in binary32 would move it past one action in a thousand.  The vector units do as many binary64 operations a
-// cycle as binary32 ones, so this costs registers, not time.
-//
-// Three forms, by the number of actions:
-//   up to 8      a lane a row, every pair of actions compared (row_kernel)
-//   up to 1024   16 or 64 lanes a row, the row sorted in registers where top-k or top-p ask for it (group_kernel)
-//   more         a workgroup a row; the border of the kept set is found by histograms, never by a sort (wide_kernel)
-#include "gx_launch.h"
-#include "gx_policy.h"
+// Actions from a policy's logits, binary32 logits and the choice of the type (see gx_sample_kernel.h; a translation unit a
+// type, so that they compile side by side).
+#include "gx_sample_kernel.h"
 
 namespace gx {
 
-namespace {
-
-constexpr float kInf = __builtin_inff();
-
-// ordered bits: a < b as numbers <=> key(a) < key(b); -0 and +0 are one, NaN is -inf
-__device__ __forceinline__ float clean(float x) { return x != x ? -kInf : x + 0.0f; }
-__device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float value_of(uint32_t k) {
-  return __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu));
-}
-
-template <class T, int N> struct Elements { T v[N]; };
-// N consecutive logits, at whatever address: gfx950 loads vectors at any alignment
-template <class T, int N> __device__ __forceinline__ void load_logits(const T* p, float* x) {
-  Elements<T, N> e;
-  __builtin_memcpy(&e, p, sizeof e);
-#pragma unroll
-  for (int j = 0; j < N; j++) x[j] = clean(to_f32(e.v[j]));
-}
-
-// A row's parameters, read as the interface says.
-struct RowParams {
-  double inv_t;  // 1 / T
-  double per_t;  // log2(e) / T
-  double p, q;   // p = 1: no cut
-  int32_t k;     // 1 .. n
-  double u;
-};
-
-// CUT: top-k, top-p or min-p may leave something out
-template <bool CUT> __device__ __forceinline__ RowParams row_params(const SampleArgs& a, uint64_t r) {
-  RowParams s;
-  bool greedy = a.greedy_all;
-  s.inv_t = a.inv_t_all;
-  if (a.temperature) {
-    const float t = a.temperature[r];
-    greedy = !(t > 0.0f);  // T = 0, and what reads as it
-    s.inv_t = greedy ? 1.0 : 1.0 / (double)t;
-  }
-  s.per_t = s.inv_t * 1.4426950408889634;
-  s.k = a.n;
-  s.p = 1.0;
-  s.q = 0.0;
-  if (CUT) {
-    const int32_t k = a.top_k ? a.top_k[r] : a.top_k_all;
-    const float p = a.top_p ? a.top_p[r] : a.top_p_all;
-    const float q = a.min_p ? a.min_p[r] : a.min_p_all;
-    if (k > 0 && k < a.n) s.k = k;
-    if (greedy) s.k = 1;
-    s.p = p < 1.0f ? (p > 0.0f ? (double)p : 0.0) : 1.0;  // NaN: no cut
-    s.q = q > 0.0f ? (q < 1.0f ? (double)q : 1.0) : 0.0;
-  }
-  if (a.u) {
-    const float u = a.u[r];
-    s.u = u > 0.0f ? (u < 1.0f ? (double)u : 1.0 - 0x1.0p-53) : 0.0;
-  } else {
-    s.u = word_uniform(policy_word(policy_block(a.seed_lo, a.seed_hi, a.tick, a.env_index_base + r), a.tick));
-  }
-  return s;
-}
-
-// 2^t, t <= 0: t = k + f, |f| <= 1/2, and a polynomial for 2^f with a relative error below 1.5e-13 (an equal-ripple fit
-// of degree 9, exact at f = 0)
-__device__ __forceinline__ double exp2_neg(double t) {
-  t = fmax(t, -1100.0);  // 2^t is 0 there, and for a NaN
-  const double k = rint(t), f = t - k;
-  double e = 0x1.89efabdef686ep-24;
-  e = __builtin_fma(e, f, 0x1.63c688cf3cab8p-20);
-  e = __builtin_fma(e, f, 0x1.fffb62b51cef6p-17);
-  e = __builtin_fma(e, f, 0x1.4308b503274e4p-13);
-  e = __builtin_fma(e, f, 0x1.5d87ed72fbd66p-10);
-  e = __builtin_fma(e, f, 0x1.3b2ab71455231p-7);
-  e = __builtin_fma(e, f, 0x1.c6b08d793b970p-5);
-  e = __builtin_fma(e, f, 0x1.ebfbdff8256ebp-3);
-  e = __builtin_fma(e, f, 0x1.62e42fefa11f3p-1);
-  e = __builtin_fma(e, f, 1.0);
-  return __builtin_ldexp(e, (int)k);
-}
-
-// log(c), c >= 1, to 1e-13: c = 2^k g, g in [sqrt(1/2), sqrt(2)), log g = 2 atanh((g - 1) / (g + 1))
-__device__ __forceinline__ double log_from_one(double c) {
-  int k;
-  double g = __builtin_frexp(c, &k);
-  if (g < 0.70710678118654752) {
-    g += g;
-    k -= 1;
-  }
-  const double d = g + 1.0;
-  double r = __builtin_amdgcn_rcp(d);  // 2^-14 or better, doubled twice
-  r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
-  r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
-  const double s = (g - 1.0) * r, s2 = s * s;
-  double e = 1.0 / 17.0;
-  e = __builtin_fma(e, s2, 1.0 / 15.0);
-  e = __builtin_fma(e, s2, 1.0 / 13.0);
-  e = __builtin_fma(e, s2, 1.0 / 11.0);
-  e = __builtin_fma(e, s2, 1.0 / 9.0);
-  e = __builtin_fma(e, s2, 1.0 / 7.0);
-  e = __builtin_fma(e, s2, 1.0 / 5.0);
-  e = __builtin_fma(e, s2, 1.0 / 3.0);
-  e = __builtin_fma(e, s2, 1.0);
-  return __builtin_fma((double)k, 0.69314718055994531, 2.0 * s * e);
-}
-
-// The weight of a logit beside the largest, which is finite (see without_inf): 1 for that, 0 for -inf.  `per_t` is
-// log2(e) / T.  (-inf / inf is a NaN on the way and 0 in the end.)
-__device__ __forceinline__ double weight(float x, float m, double per_t) { return exp2_neg(((double)x - (double)m) * per_t); }
-
-// Beside +inf every finite logit weighs nothing, and those that are +inf weigh the same: 0 and -inf say that in finite terms.
-__device__ __forceinline__ float without_inf(float x) { return x == kInf ? 0.0f : -kInf; }
-
-__device__ __forceinline__ void write_result(const SampleArgs& a, uint64_t r, int action, float x, float m, double inv_t, double total) {
-  a.actions[r] = action;
-  if (a.logprob) a.logprob[r] = action < 0 ? -kInf : (float)(((double)x - (double)m) * inv_t - log_from_one(total));
-}
-
-// ------------------------------------------------------- up to 8 actions ---
-// A lane a row.  Bound by the arithmetic about as much as by memory: N exponentials, and with a cut every pair of
-// actions: the rank of an action and the mass ahead of it, which are all that the definition asks for.
-template <class T, int N, bool CUT, bool PACKED>
-__global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
-  for (uint64_t r = (uint64_t)blockIdx.x * kBlock + threadIdx.x; r < a.rows; r += (uint64_t)gridDim.x * kBlock) {
-    const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
-    float x[N];
-    if (PACKED) load_logits<T, N>(row, x);
-    else
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] = clean(to_f32(row[(int64_t)i * a.col_stride]));
-    const RowParams s = row_params<CUT>(a, r);
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) m = fmaxf(m, x[i]);
-    if (__any(m == kInf) && m == kInf) {
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] = without_inf(x[i]);
-      m = 0.0f;
-    }
-    double w[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) w[i] = weight(x[i], m, s.per_t);
-    if (CUT) {
-      if (__any(s.k < N)) {
-        int rank[N] = {};
-#pragma unroll
-        for (int i = 0; i < N; i++)
-#pragma unroll
-          for (int j = i + 1; j < N; j++) {
-            const bool later = x[j] > x[i];  // equal: the lower index first
-            rank[i] += later ? 1 : 0;
-            rank[j] += later ? 0 : 1;
-          }
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = rank[i] < s.k ? w[i] : 0.0;
-      }
-      double s1 = 0.0, ahead[N] = {};
-#pragma unroll
-      for (int i = 0; i < N; i++) s1 += w[i];
-      // (never 0: what has nothing ahead of it is kept)
-      const double target = s.p < 1.0 ? fmax(s.p * s1, 1e-290) : __builtin_inf();
-#pragma unroll
-      for (int i = 0; i < N; i++)
-#pragma unroll
-        for (int j = i + 1; j < N; j++) {
-          // a weight or, without its upper half, something below 1e-307: as good as 0 here
-          const bool later = x[j] > x[i];
-          ahead[i] += __hiloint2double(later ? __double2hiint(w[j]) : 0, __double2loint(w[j]));
-          ahead[j] += __hiloint2double(later ? 0 : __double2hiint(w[i]), __double2loint(w[i]));
-        }
-#pragma unroll
-      for (int i = 0; i < N; i++) w[i] = ahead[i] < target ? w[i] : 0.0;
-      if (__any(s.q > 0.0))
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = w[i] >= s.q ? w[i] : 0.0;
-    }
-    double total = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; i++) total += w[i];
-    const double stop = s.u * total;
-    // the first past the border: as many as are not
-    int action = 0;
-    double c = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      c += w[i];
-      action += c > stop ? 0 : 1;
-    }
-    if (__any(action == N) && action == N) {  // rounding put the border at the total: the last one kept
-      action = 0;
-#pragma unroll
-      for (int i = 0; i < N; i++) action = w[i] > 0.0 ? i : action;
-    }
-    float chosen = x[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) chosen = action == i ? x[i] : chosen;
-    if (m == -kInf) action = -1;
-    write_result(a, r, action, chosen, m, s.inv_t, total);
-  }
-}
-
-// ---------------------------------------------------- up to 1024 actions ---
-// G lanes a row (16: four rows a wave), E consecutive actions a lane.  Bound by instructions.  With top-k or top-p the
-// row's values are sorted in registers (a bitonic network: the values alone, not their indices, for t and j are all that
-// is wanted), weighed in that order and summed along it; the draw then goes over the row as it lies.
-template <int M> __device__ __forceinline__ float max_with(float v) { return fmaxf(v, __uint_as_float(xor_lane<M>(__float_as_uint(v)))); }
-template <int G> __device__ __forceinline__ float group_max(float v) {
-  if constexpr (G > 1) v = max_with<1>(v);
-  if constexpr (G > 2) v = max_with<2>(v);
-  if constexpr (G > 4) v = max_with<4>(v);
-  if constexpr (G > 8) v = max_with<8>(v);
-  if constexpr (G > 16) v = max_with<16>(v);
-  if constexpr (G > 32) v = max_with<32>(v);
-  return v;
-}
-// sums over the lanes of a group before this one
-template <int G> __device__ __forceinline__ double group_before(double v, double* all) {
-  if constexpr (G == 1) {
-    *all = v;
-    return 0.0;
-  }
-  const double run = running_sum<G>(v);
-  *all = shfl_f64(run, G - 1, G);
-  const double before = moved<0x138, 0xF>(run);  // from the lane before, of all 64
-  return threadIdx.x & (G - 1) ? before : 0.0;
-}
-template <int G> __device__ __forceinline__ unsigned long long group_ballot(bool b) {
-  if constexpr (G == 1) return b ? 1 : 0;
-  const unsigned long long m = __ballot(b);
-  return G == 64 ? m : (m >> (threadIdx.x & 63 & ~(G - 1))) & ((1ull << (G & 63)) - 1);
-}
-template <int G> __device__ __forceinline__ int group_lane(int v, int lane) { return G == 1 ? v : __shfl(v, lane, G); }
-
-__device__ __forceinline__ uint32_t med3(uint32_t a, uint32_t b, uint32_t c) {
-  return max(min(a, b), min(max(a, b), c));
-}
-// Descending over index lane * E + e, of ordered keys.  A step gives a lane the larger or the smaller of two: the median of
-// them and a bound, which is one instruction.
-template <int D, int E> __device__ __forceinline__ void sort_across(uint32_t* v, uint32_t bound) {
-#pragma unroll
-  for (int e = 0; e < E; e++) v[e] = med3(v[e], xor_lane<D>(v[e]), bound);
-}
-template <int G, int E> __device__ __forceinline__ void group_sort(uint32_t* v) {
-  const int lane = threadIdx.x & (G - 1);
-#pragma unroll
-  for (int size = 2; size <= G * E; size <<= 1) {
-#pragma unroll
-    for (int d = size >> 1; d >= 1; d >>= 1) {
-      // a block of `size` is sorted downwards if its number is even, the last one of all downwards
-      if (d >= E) {
-        const bool low = !(lane & (d / E)), down = size == G * E || !(lane & (size / E));
-        const uint32_t bound = low == down ? 0xFFFFFFFFu : 0u;
-        switch (d / E) {
-          case 1: sort_across<1, E>(v, bound); break;
-          case 2: sort_across<2, E>(v, bound); break;
-          case 4: sort_across<4, E>(v, bound); break;
-          case 8: sort_across<8, E>(v, bound); break;
-          case 16: sort_across<16, E>(v, bound); break;
-          default: sort_across<32, E>(v, bound); break;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; e++)
-          if (!(e & d)) {
-            const bool down = size == G * E || (size >= E ? !(lane & (size / E)) : !(e & size));
-            const uint32_t bound = down ? 0xFFFFFFFFu : 0u, x = v[e], y = v[e + d];
-            v[e] = med3(x, y, bound);
-            v[e + d] = med3(x, y, ~bound);
-          }
-      }
-    }
-  }
-}
-
-template <class T, int G, int E, bool CUT, bool PACKED>
-__global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
-  constexpr int kRows = kBlock / G;
-  const int lane = threadIdx.x & (G - 1), first = lane * E;
-  // (a group whose rows are done goes on with the last row, unwritten: its wave's other groups need its lanes)
-  for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (uint64_t)gridDim.x * kRows) {
-    const uint64_t mine = r0 + threadIdx.x / G;
-    const bool live = mine < a.rows;
-    const uint64_t r = live ? mine : a.rows - 1;
-    const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
-    float x[E];
-    if (PACKED && first + E <= a.n) load_logits<T, E>(row + first, x);
-    else
-#pragma unroll
-      for (int e = 0; e < E; e++) x[e] = first + e < a.n ? clean(to_f32(row[(int64_t)(first + e) * a.col_stride])) : -kInf;
-    const RowParams s = row_params<CUT>(a, r);
-    float m = x[0];
-#pragma unroll
-    for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
-    m = group_max<G>(m);
-    if (__any(m == kInf) && m == kInf) {
-#pragma unroll
-      for (int e = 0; e < E; e++) x[e] = without_inf(x[e]);
-      m = 0.0f;
-    }
-    // kept: above t, and the first `ties` of those equal to it
-    float t = -kInf;
-    int ties = 0, before = 0;  // (before: at lower indices than the lane's)
-    if (CUT && __any(s.k < a.n || s.p < 1.0)) {
-      uint32_t v[E];
-#pragma unroll
-      for (int e = 0; e < E; e++) v[e] = key_of(x[e]);
-      group_sort<G, E>(v);
-      double sw[E], sum = 0.0;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        sw[e] = first + e < s.k ? weight(value_of(v[e]), m, s.per_t) : 0.0;
-        sum += sw[e];
-      }
-      double s1, ahead = group_before<G>(sum, &s1);
-      const double target = s.p < 1.0 ? s.p * s1 : __builtin_inf();
-      // kept: a beginning of the order.  The last one kept is t.
-      uint32_t mine = 0;
-      int kept = 0;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const bool in = first + e == 0 || (first + e < s.k && ahead < target && sw[e] > 0.0);
-        ahead += sw[e];
-        mine = in ? v[e] : mine;
-        kept += in ? 1 : 0;
-      }
-      const unsigned long long some = group_ballot<G>(kept > 0);
-      const int last_lane = 63 - __clzll(some);
-      t = value_of((uint32_t)group_lane<G>((int)mine, last_lane));
-      const int count = last_lane * E + group_lane<G>(kept, last_lane);  // the lanes before it keep all of theirs
-      int above = 0, equal = 0;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        above += __popcll(group_ballot<G>(x[e] > t));
-        equal += x[e] == t ? 1 : 0;
-      }
-      before = running_sum<G>(equal) - equal;
-      ties = count - above;
-    }
-    double w[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      w[e] = weight(x[e], m, s.per_t);
-      if (CUT) {
-        const bool tie = x[e] == t;
-        w[e] = (x[e] > t || (tie && before < ties)) && w[e] >= s.q ? w[e] : 0.0;
-        before += tie ? 1 : 0;
-      }
-    }
-    double sum = 0.0, total;
-#pragma unroll
-    for (int e = 0; e < E; e++) sum += w[e];
-    double c = group_before<G>(sum, &total);
-    const double stop = s.u * total;
-    int past = -1, last = -1;  // this lane's first action past the border, its last one kept
-    float x_past = 0.0f, x_last = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      c += w[e];
-      if (w[e] > 0.0) {
-        last = first + e;
-        x_last = x[e];
-        if (past < 0 && c > stop) {
-          past = last;
-          x_past = x_last;
-        }
-      }
-    }
-    const unsigned long long over = group_ballot<G>(past >= 0), kept = group_ballot<G>(last >= 0);
-    // rounding may have put the border at the total: the last one kept then
-    const int chosen_lane = over ? __ffsll(over) - 1 : (kept ? 63 - __clzll(kept) : 0);
-    if (live && lane == chosen_lane) {
-      const bool none = m == -kInf;
-      write_result(a, r, none ? -1 : (over ? past : last), over ? x_past : x_last, m, s.inv_t, total);
-    }
-  }
-}
-
-// -------------------------------------------------- more than 1024 actions ---
-// A workgroup a row, which it reads from memory once and again from the caches.  The row is cut into at most SEGMENTS
-// stretches, a wave each, 32 bytes of consecutive logits a lane and turn.
-//
-// Without a cut, one pass: each segment's largest logit and the sum of its weights relative to that.  With one:
-//   1  the largest logit, and for top-p alone the sum of the weights, estimated in binary32
-//   2  a lower bound on what can be kept (the k-th largest of the lanes' largest logits; the weight below which all
-//      actions together weigh less than 1 - p of the sum; min-p's own); what is above goes into BINS bins by m - x, and is
-//      listed while the list is short
-//   3  for top-p alone: the exact sum, the exact sums of the segments above the bins where the estimates put the border,
-//      and the list of what lies in those
-//   4  a short list is sorted: it ends with the border.  Where it is too long, or the estimate was wrong, the border's bin
-//      goes into finer and finer bins with integer masses (whose order of adding changes nothing) until it holds one
-//      value, and a last pass adds up what is kept by segments
-// then the segment u falls into, and in it the action.  The passes are bound by instructions: 20 an exponential in
-// binary64, so step 3 is the only one that takes them of every action.  What runs for few elements is a loop: unrolled,
-// the kernel outgrew the instruction cache and took three times as long.
-//
-// Few rows leave most of the card idle, so each is split among several workgroups (parts), and the steps become launches
-// that hand their results on in the workspace: kPartMax is step 1, kPartList step 2 (and for min-p alone the segments'
-// sums), kPartExact step 3, kPartJoin the rest, by one workgroup a row.  Where a step says that the row needs more than
-// that (a list too long, +inf among the logits, k above kListMost), kPartJoin goes through the row by itself.
-constexpr int kWideSmall = 4096;
-constexpr int kAhead = 2;
-// Actions a part has at least.  One row of 131 072, top-p: 46 us with 8 192, 50 with 16 384, 44 with 4 096, whose 32 parts
-// find their lists too long sooner.
-constexpr int kPartActions = 8192;
-enum Part { kWhole = 0, kPartMax = 1, kPartList = 2, kPartExact = 3, kPartJoin = 4 };
-constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock;
-
-struct SplitRow {
-  double sum[kMostParts];       // of each part: exact, and estimated relative to its largest logit
-  double estimate[kMostParts];
-  float top[kMostParts];        // its largest logit
-  float bound[kMostParts];      // what k of its lanes' largest reach, or -inf
-  float share[kMostParts];      // what 2 k / parts of them reach: half the parts together have k that reach their median
-  uint32_t listed, around;      // lengths of the lists; more than kListMost: not kept
-  float list_x[kListMost];      // what may be kept
-  int list_i[kListMost];
-  float around_x[kListMost];    // what lies around top-p's border
-  int around_i[kListMost];
-  uint32_t bins[kWideBins];     // estimates
-  double seg_sum[kWideSegments];
-  float seg_max[kWideSegments];
-};
-
-// low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
-template <class T> constexpr int kFixedBits = 0;
-template <> constexpr int kFixedBits<f16> = 13;
-template <> constexpr int kFixedBits<bf16> = 16;
-
-// logit j of a run of words
-template <class T> __device__ __forceinline__ float word_value(const uint32_t* w, int j);
-template <> __device__ __forceinline__ float word_value<float>(const uint32_t* w, int j) { return __uint_as_float(w[j]); }
-template <> __device__ __forceinline__ float word_value<bf16>(const uint32_t* w, int j) {
-  return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
-}
-template <> __device__ __forceinline__ float word_value<f16>(const uint32_t* w, int j) {
-  return (float)__builtin_bit_cast(f16, (uint16_t)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]));
-}
-
-template <int BLOCK, int BINS, int SEGMENTS> struct WideShared {
-  double seg_sum[SEGMENTS];
-  float seg_max[SEGMENTS];
-  int seg_ties[SEGMENTS];
-  unsigned long long mass[BINS];
-  uint32_t count[BINS];
-  double wave_f64[BLOCK / 64];
-  unsigned long long wave_u64[BLOCK / 64];
-  float wave_f32[BLOCK / 64];
-  uint32_t wave_u32[BLOCK / 64];
-  int wave_kept[BLOCK / 64];
-  // what may be kept, or the border's surroundings, if that is little
-  float list_x[BLOCK];
-  int list_i[BLOCK];
-  uint32_t listed;
-  float bound;
-  // the border's bin
-  int bin;
-  uint32_t bin_count, above_count;
-  unsigned long long bin_mass, above_mass;
-};
-
-// One value a thread, the first `size` of them (a power of two, at least 64) sorted downwards; `swap` holds a value a thread.
-template <int D> __device__ __forceinline__ unsigned long long sort_step(unsigned long long v, bool larger) {
-  const unsigned long long o = (unsigned long long)xor_lane<D>((uint32_t)(v >> 32)) << 32 | xor_lane<D>((uint32_t)v);
-  return (v > o) == larger ? v : o;
-}
-template <int BLOCK> __device__ __forceinline__ unsigned long long block_sort(unsigned long long v, int size, unsigned long long* swap) {
-  const int me = threadIdx.x;
-#pragma unroll 1
-  for (int block = 2; block <= size; block <<= 1) {
-    const bool down = !(me & block);
-    if (block > 64) {
-#pragma unroll 1
-      for (int d = block >> 1; d >= 64; d >>= 1) {
-        __syncthreads();
-        swap[me] = v;
-        __syncthreads();
-        const unsigned long long o = swap[me ^ d];
-        v = (v > o) == (!(me & d) == down) ? v : o;
-      }
-    }
-    // within a wave
-    if (block > 32) v = sort_step<32>(v, !(me & 32) == down);
-    if (block > 16) v = sort_step<16>(v, !(me & 16) == down);
-    if (block > 8) v = sort_step<8>(v, !(me & 8) == down);
-    if (block > 4) v = sort_step<4>(v, !(me & 4) == down);
-    if (block > 2) v = sort_step<2>(v, !(me & 2) == down);
-    v = sort_step<1>(v, !(me & 1) == down);
-  }
-  __syncthreads();
-  return v;
-}
-
-// The largest of a run of words of logits, without unpacking them: as signed integers of their width, positive numbers
-// are in order and negative ones in reverse, below them.  So it is the largest integer, or where that is negative the
-// smallest.  (NaN: see `mode`.)
-template <int W> __device__ __forceinline__ float run_largest_32(const uint32_t* w) {
-  float v = __uint_as_float(w[0]);
-#pragma unroll
-  for (int j = 1; j < W; j++) v = __builtin_amdgcn_fmed3f(v, __uint_as_float(w[j]), kInf);
-  return v;
-}
-typedef short Half2 __attribute__((ext_vector_type(2)));
-template <class T, int W> __device__ __forceinline__ float run_largest_16(const uint32_t* w) {
-  Half2 hi = __builtin_bit_cast(Half2, w[0]), lo = hi;
-#pragma unroll
-  for (int j = 1; j < W; j++) {
-    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(Half2, w[j]));
-    lo = __builtin_elementwise_min(lo, __builtin_bit_cast(Half2, w[j]));
-  }
-  const short h = hi.x > hi.y ? hi.x : hi.y, l = lo.x < lo.y ? lo.x : lo.y;
-  const uint32_t one = (uint16_t)(h < 0 ? l : h);
-  const float v = word_value<T>(&one, 0);
-  return h >= 0 && v != v ? kInf : v;
-}
-template <class T, int W> __device__ __forceinline__ float run_largest(const uint32_t* w) {
-  if constexpr (sizeof(T) == 4) return run_largest_32<W>(w);
-  else return run_largest_16<T, W>(w);
-}
-
-__host__ __device__ __forceinline__ int share_of(int k, int parts) { return (2 * k + parts - 1) / parts; }
-
-template <class T, int BLOCK, int BINS, int SEGMENTS, int RUN_BYTES, bool CUT, bool PACKED, Part PART>
-__global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, SplitRow* split) {
-  constexpr bool kOnePart = PART == kPartMax || PART == kPartList || PART == kPartExact;  // of a row, not all of it
-  constexpr int kWaves = BLOCK / 64, kRun = PACKED ? RUN_BYTES / (int)sizeof(T) : 8, kTurn = 64 * kRun;
-  __shared__ WideShared<BLOCK, BINS, SEGMENTS> sh;
-  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
-  // turns a segment takes, so that SEGMENTS are enough
-  const int turns = (a.n + kTurn * SEGMENTS - 1) / (kTurn * SEGMENTS), seg_len = kTurn * turns;
-  const int segments = (a.n + seg_len - 1) / seg_len;
-  for (uint64_t item = blockIdx.x; item < (kOnePart ? a.rows * (uint64_t)parts : a.rows); item += gridDim.x) {
-    const uint64_t r = kOnePart ? item / (uint64_t)parts : item;
-    const int part = kOnePart ? (int)(item % (uint64_t)parts) : 0;
-    // its segments, and the turns of this wave among them
-    const int g_first = kOnePart ? (int)((int64_t)segments * part / parts) : 0, g_last = kOnePart ? (int)((int64_t)segments * (part + 1) / parts) : segments;
-    const int units = max(0, (g_last - g_first - wave + kWaves - 1) / kWaves) * turns;
-    SplitRow* const sr = split + (PART == kWhole ? 0 : r);
-    const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
-    RowParams s = row_params<CUT>(a, r);
-    s.inv_t = uniform(s.inv_t); s.per_t = uniform(s.per_t); s.p = uniform(s.p); s.q = uniform(s.q); s.k = uniform(s.k); s.u = uniform(s.u);
-    // 0: logits as they are.  A NaN is then no more than any bound and weighs nothing; where the largest comes out as +inf
-    // (some NaN can make it that) the row is read again with 1: NaN as -inf, and if that was not it 2: +inf in finite terms
-    int mode = 0;
-    // A run of logits from c on, as words.  c is i, or the last run of the row where i is closer to its end: those before
-    // i are the lane's before and are taken out of the values.
-    struct Run { uint32_t w[kRun * sizeof(T) / 4]; };
-    auto start = [&](int i) { return min(i, a.n - kRun); };
-    auto load = [&](int i) {
-      Run e;
-      const T* at = row + (PACKED ? (int64_t)start(i) : (int64_t)start(i) * a.col_stride);
-      if (PACKED) __builtin_memcpy(&e, at, sizeof e);
-      else {
-        T v[kRun];
-#pragma unroll
-        for (int j = 0; j < kRun; j++) v[j] = at[j * a.col_stride];
-        __builtin_memcpy(&e, v, sizeof e);
-      }
-      return e;
-    };
-    auto values = [&](const Run& e, int i, float* x) {
-#pragma unroll
-      for (int j = 0; j < kRun; j++) x[j] = word_value<T>(e.w, j);
-      if (mode)
-#pragma unroll
-        for (int j = 0; j < kRun; j++) x[j] = mode == 2 ? without_inf(clean(x[j])) : clean(x[j]);
-      const int before = i - start(i);
-      if (__any(before > 0))
-#pragma unroll
-        for (int j = 0; j < kRun; j++) x[j] = j < before ? -kInf : x[j];
-    };
-    // f(segment, whether this was its last turn, the lane's place in the row, its words) over the wave's share of the row,
-    // the next loads under way
-    auto each = [&](auto f) {
-      int g = g_first + wave, t = 0;            // of the turn at hand
-      int load_g = g_first + wave, load_t = 0;  // of the next one to load
-      auto next = [&]() {
-        const int i = load_g * seg_len + load_t * kTurn + lane * kRun;
-        const bool end = load_t == turns - 1;
-        load_t = end ? 0 : load_t + 1;
-        load_g += end ? kWaves : 0;
-        return load(i);
-      };
-      Run e[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; k++) e[k] = next();
-#pragma unroll 1
-      for (int q = 0; q < units; q++) {  // (moving the words along costs less than a body for each place)
-        const int i = g * seg_len + t * kTurn + lane * kRun;
-        const Run now = e[0];
-#pragma unroll
-        for (int k = 0; k + 1 < kAhead; k++) e[k] = e[k + 1];
-        e[kAhead - 1] = next();
-        const bool end = t == turns - 1;
-        f(g, end, i, now);
-        t = end ? 0 : t + 1;
-        g += end ? kWaves : 0;
-      }
-    };
-    // the larger of two in one instruction: their median with +inf
-    auto larger_of = [](float x, float y) { return __builtin_amdgcn_fmed3f(x, y, kInf); };
-    auto largest = [&](const Run& e, int i) {
-      if (mode == 0 && !__any(i > start(i))) return run_largest<T, sizeof e.w / 4>(e.w);
-      float x[kRun], v = -kInf;
-      values(e, i, x);
-#pragma unroll
-      for (int j = 0; j < kRun; j++) v = larger_of(v, x[j]);
-      return v;
-    };
-    auto block_max = [&](float v) {
-      v = group_max<64>(v);
-      if (lane == 0) sh.wave_f32[wave] = v;
-      __syncthreads();
-      v = sh.wave_f32[0];
-#pragma unroll
-      for (int w = 1; w < kWaves; w++) v = fmaxf(v, sh.wave_f32[w]);
-      __syncthreads();
-      return uniform(v);
-    };
-    // running sums over the threads, the own included, and the sum of all
-    auto block_running = [&](double v, double* all) {
-      double run = running_sum<64>(v);
-      if (lane == 63) sh.wave_f64[wave] = run;
-      __syncthreads();
-      double total = 0.0;
-#pragma unroll
-      for (int q = 0; q < kWaves; q++) {
-        if (q == wave) run += total;
-        total += sh.wave_f64[q];
-      }
-      __syncthreads();
-      *all = uniform(total);
-      return run;
-    };
-    auto block_sum = [&](double v) {
-      double all;
-      (void)block_running(v, &all);
-      return all;
-    };
-
-    float m = -kInf;
-    // What is kept: logits above `hi`, and of those in [lo, hi] all, or (ordered) the first `ties` by index, or (listed)
-    // those up to the index `tie_index`.
-    float lo = 0.0f, hi = 0.0f;
-    int ties = 0, tie_index = 0;
-    bool ordered = false, by_index = false;
-    bool done = false;  // the action is written
-    // the segments' results of an earlier launch
-    auto segments_of_split = [&]() {
-      for (int g = threadIdx.x; g < segments; g += BLOCK) {
-        sh.seg_sum[g] = sr->seg_sum[g];
-        if (!CUT) sh.seg_max[g] = sr->seg_max[g];
-      }
-      __syncthreads();
-    };
-    if (!CUT) {
-      // largest logit and sum of a segment: a lane's own first, then the wave's
-      bool have = PART == kPartJoin;
-      if (have) segments_of_split();
-#pragma unroll 1
-      for (;; mode += have ? 0 : 1, have = false) {
-        float top = -kInf;
-        double sum = 0.0;
-        if (!have) each([&](int g, bool end, int i, const Run& e) {
-          const float here = largest(e, i);
-          float x[kRun];
-          values(e, i, x);
-          if (here > top) {
-            sum *= weight(top, here, s.per_t);
-            top = here;
-          }
-          if (__any(top > -kInf))
-#pragma unroll
-            for (int j = 0; j < kRun; j++) sum += weight(x[j], top, s.per_t);
-          if (end) {
-            const float seg_top = group_max<64>(top);
-            sum = wave_sum(top > -kInf ? sum * weight(top, seg_top, s.per_t) : 0.0);
-            if (lane == 0) {
-              (kOnePart ? sr->seg_max : sh.seg_max)[g] = seg_top;
-              (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = sum;
-            }
-            top = -kInf;
-            sum = 0.0;
-          }
-        });
-        if (kOnePart) break;
-        __syncthreads();
-        m = -kInf;
-        for (int g = threadIdx.x; g < segments; g += BLOCK) m = fmaxf(m, sh.seg_max[g]);
-        m = block_max(m);
-        if (m < kInf) break;
-      }
-      if (kOnePart) continue;
-      for (int g = threadIdx.x; g < segments; g += BLOCK)
-        if (sh.seg_max[g] > -kInf) sh.seg_sum[g] *= weight(sh.seg_max[g], m, s.per_t);
-      __syncthreads();
-    } else {
-      const bool by_k = s.k < a.n, by_p = s.p < 1.0, sums = by_p && !by_k, far_k = by_k && s.k > BLOCK;
-      const float per_t = fminf((float)s.per_t, 3e38f);
-      bool list = false;    // the list holds all that is kept but what lies above it
-      bool summed = false;  // the segments' sums of what is kept are there
-      bool taken = false;   // either, by earlier launches
-      double above = 0.0;   // what lies above the list
-      double s1 = 0.0;      // the sum (of all; for top-p alone)
-      float split_bound = -kInf;
-      if (PART >= kPartList) {
-        const bool mine = (int)threadIdx.x < parts;
-        m = block_max(mine ? sr->top[threadIdx.x] : -kInf);
-        if (kOnePart && (far_k || m == kInf || m == -kInf || (PART == kPartExact && !sums))) continue;
-        if (m < kInf && m > -kInf) {
-          if (PART != kPartJoin) {
-            if (sums) s1 = block_sum(mine ? sr->estimate[threadIdx.x] * weight(sr->top[threadIdx.x], m, s.per_t) : 0.0);
-            if (by_k) {
-              // what one part's lanes reach alone; or what enough parts reach with their share (see kPartMax)
-              split_bound = block_max(mine ? sr->bound[threadIdx.x] : -kInf);
-              const int share = min(share_of(s.k, parts), s.k), need = (s.k + share - 1) / share;
-              const float b = lane < parts ? sr->share[lane] : -kInf;
-              int rank = 0;
-              for (int j = 0; j < parts; j++) {
-                const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(b), j));
-                rank += o > b || (o == b && j < lane) ? 1 : 0;
-              }
-              const unsigned long long who = __ballot(lane < parts && rank == need - 1);
-              split_bound = fmaxf(split_bound, __shfl(b, __ffsll(who) - 1, 64));
-            }
-          } else if (!far_k) {
-            const uint32_t listed = uniform(sr->listed), around = uniform(sr->around);
-            if (sums) s1 = block_sum(mine ? sr->sum[threadIdx.x] : 0.0);
-            list = taken = (by_k || by_p) && listed <= (uint32_t)kListMost;
-            if (list) {
-              if (threadIdx.x == 0) sh.listed = listed;
-              sh.list_x[threadIdx.x] = sr->list_x[threadIdx.x];
-              sh.list_i[threadIdx.x] = sr->list_i[threadIdx.x];
-              __syncthreads();
-            } else if (sums && around <= (uint32_t)kListMost) {
-              segments_of_split();
-              double sum = 0.0;
-              for (int g = threadIdx.x; g < segments; g += BLOCK) sum += sh.seg_sum[g];
-              above = block_sum(sum);
-              if (threadIdx.x == 0) sh.listed = around;
-              const float v = threadIdx.x < around ? sr->around_x[threadIdx.x] : -kInf;
-              sh.list_x[threadIdx.x] = v;
-              sh.list_i[threadIdx.x] = sr->around_i[threadIdx.x];
-              const double within = block_sum(weight(v, m, s.per_t));
-              list = taken = above < s.p * s1 && s.p * s1 <= above + within;
-              if (!list) above = 0.0;
-            } else if (!by_k && !by_p) {
-              segments_of_split();
-              summed = taken = true;
-            }
-          }
-        }
-      }
-      // ---- 1: the largest logit, the estimate of the sum, and where it is wanted the smallest finite one
-      float top = -kInf, bottom = kInf, estimate = 0.0f;
-      if ((PART == kWhole || PART == kPartMax || PART == kPartJoin) && !taken)
-#pragma unroll 1
-      for (;; mode++) {
-        top = -kInf;
-        bottom = kInf;
-        estimate = 0.0f;
-        each([&](int, bool, int i, const Run& e) {
-          const float here = largest(e, i);
-          if (far_k) {
-            float x[kRun];
-            values(e, i, x);
-#pragma unroll
-            for (int j = 0; j < kRun; j++) bottom = x[j] > -kInf && x[j] < bottom ? x[j] : bottom;
-          }
-          if (sums) {
-            float x[kRun];
-            values(e, i, x);
-            if (here > top) estimate *= __builtin_amdgcn_exp2f(fmaxf((top - here) * per_t, -150.0f));
-            top = larger_of(top, here);
-            if (top > -kInf)
-#pragma unroll
-              for (int j = 0; j < kRun; j++) estimate += __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f((x[j] - top) * per_t, -150.0f, 0.0f));
-          } else {
-            top = larger_of(top, here);
-          }
-        });
-        m = block_max(top);
-        if (m < kInf || PART == kPartMax) break;
-      }
-      if (PART == kPartMax) {
-        s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;  // (beside +inf: unused)
-        if (part == 0)
-          for (int b = threadIdx.x; b < BINS; b += BLOCK) sr->bins[b] = 0;
-        if (threadIdx.x == 0) {
-          sr->top[part] = m;
-          sr->estimate[part] = s1;
-          sr->bound[part] = sr->share[part] = -kInf;
-          if (part == 0) sr->listed = sr->around = 0;
-        }
-        if (!by_k || far_k || !(m > -kInf && m < kInf)) continue;
-      }
-      if (m > -kInf) {
-        if (!kOnePart && !taken) {
-          if (far_k) bottom = -block_max(-bottom);
-          s1 = sums ? block_sum(top > -kInf ? (double)estimate * weight(top, m, s.per_t) : 0.0) : 0.0;
-        }
-        // ---- 2: a bound below everything that can be kept (weights below exp(-745) are 0) ...
-        double bound = (double)m - 745.0 / s.inv_t;
-        if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * s1 * 0.99 / (double)a.n, 1e-320)) / s.inv_t);
-        if (!by_k && s.q > 0.0) bound = fmax(bound, (double)m + log(s.q) / s.inv_t);
-        float from = fminf(m, fmaxf((float)(bound - fabs(bound) * 1e-6), -3.402823466e38f));
-        if (far_k) from = fminf(m, fmaxf(bottom, from));
-        if (by_k && !far_k && (PART == kPartList || PART == kPartExact)) from = fminf(m, fmaxf(from, split_bound));
-        if (by_k && !far_k && !taken && (!kOnePart || PART == kPartMax)) {
-          // a value that k lanes' largest reach: halving between the bound and the largest, one wave's work (and of a part
-          // what its share of k reach, another's)
-          sh.list_x[threadIdx.x] = top;
-          __syncthreads();
-          if (wave == 0 || (PART == kPartMax && wave == 1)) {
-            float v[kWaves];
-#pragma unroll
-            for (int q = 0; q < kWaves; q++) v[q] = sh.list_x[q * 64 + lane];
-            auto reach = [&](float x) {
-              int c = 0;
-#pragma unroll
-              for (int q = 0; q < kWaves; q++) c += __popcll(__ballot(v[q] >= x));
-              return c;
-            };
-            auto reached_by = [&](int count, float low) {
-              if (reach(low) < count) return -kInf;
-              float high = m;
-#pragma unroll 1
-              for (int step = 0; step < 14; step++) {
-                const float mid = low + (high - low) * 0.5f;
-                if (!(mid > low && mid < high)) break;
-                if (reach(mid) >= count) low = mid; else high = mid;
-              }
-              return low;
-            };
-            const float b = reached_by(wave == 0 ? s.k : min(share_of(s.k, parts), s.k), from);
-            if (lane == 0) {
-              if (PART == kPartMax) (wave == 0 ? sr->bound : sr->share)[part] = b;
-              else sh.bound = fmaxf(from, b);
-            }
-          }
-          __syncthreads();
-          if (PART != kPartMax) from = uniform(sh.bound);
-        }
-        if (PART == kPartMax) continue;
-        // ---- ... and the bins
-        from = uniform(from);
-        const float per = m > from ? (float)(BINS - 1) / (m - from) : 0.0f;
-        auto bin_of = [&](float x) { return (int)fminf((m - x) * per, (float)(BINS - 1)); };
-        const uint32_t key_from = uniform(key_of(from + 0.0f)), key_m = uniform(key_of(m + 0.0f));
-        // the smallest key whose bin is below b (one past the largest where b is 0): bin_of falls as the key rises.  The
-        // wave's lanes try 64 keys at once.
-        auto first_key_below = [&](int b) {
-          if (b <= 0) return key_m + 1;
-          uint32_t l = key_from, h = key_m;  // h's bin is 0
-#pragma unroll 1
-          while (l < h) {
-            const uint32_t step = (h - l) / 64 + 1, rest = h - l, off = (uint32_t)lane * step, at = l + (off < rest ? off : rest);
-            const unsigned long long yes = __ballot(bin_of(value_of(at)) < b);
-            const uint32_t hit = uniform(yes ? (uint32_t)__ffsll(yes) - 1 : 64u);
-            const uint32_t below = hit * step, before = (hit - 1) * step;
-            if (hit < 64) h = l + (below < rest ? below : rest);
-            if (hit > 0) l = l + (before < rest ? before : rest) + 1;
-          }
-          return h;
-        };
-        constexpr uint32_t kKeyMinusZero = 0x7FFFFFFFu;
-        auto low_value = [&](uint32_t key) { return value_of(key == kKeyMinusZero ? key + 1 : key); };
-        auto high_value = [&](uint32_t key) { return value_of(key == kKeyMinusZero ? key - 1 : key); };
-        // masses as integers: their sum (at most n where it is not known) stays below 2^62
-        bool exact = !sums;                        // s1 and the masses (else binary32 estimates in the same place)
-        // (of 31 bits, in the counts' place)
-        const int guess_shift = 30;
-        int scale_bits = 61 - __builtin_amdgcn_frexp_exp(sums ? fmax(s1, 1.0) * 1.01 : (double)a.n);
-        // the border by counts or by masses: the first bin where what lies up to its end reaches the target
-        const float guess_bits = (float)(scale_bits - guess_shift);
-        auto find_bin = [&](bool mass, uint32_t want_count, unsigned long long want_mass) {
-          constexpr int kEach = BINS / BLOCK;
-          uint32_t c = 0;
-          unsigned long long w = 0;
-          auto mass_of = [&](int b) {
-            return exact ? sh.mass[b] : (unsigned long long)sh.count[b] << guess_shift;
-          };
-#pragma unroll
-          for (int e = 0; e < kEach; e++) {
-            c += sh.count[threadIdx.x * kEach + e];
-            w += mass_of(threadIdx.x * kEach + e);
-          }
-          uint32_t rc = c;
-          unsigned long long rw = w;
-#pragma unroll
-          for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t oc = __shfl_up(rc, d, 64);
-            const unsigned long long ow = __shfl_up(rw, d, 64);
-            if (lane >= d) { rc += oc; rw += ow; }
-          }
-          if (lane == 63) { sh.wave_u32[wave] = rc; sh.wave_u64[wave] = rw; }
-          if (threadIdx.x == 0) sh.bin = -1;
-          __syncthreads();
-          rc -= c;
-          rw -= w;
-          for (int v = 0; v < wave; v++) { rc += sh.wave_u32[v]; rw += sh.wave_u64[v]; }
-#pragma unroll
-          for (int e = 0; e < kEach; e++) {
-            const uint32_t bc = sh.count[threadIdx.x * kEach + e];
-            const unsigned long long bw = mass_of(threadIdx.x * kEach + e);
-            const bool before = mass ? rw < want_mass : rc < want_count, after = mass ? rw + bw >= want_mass : rc + bc >= want_count;
-            if ((bc || bw) && before && after) {
-              sh.bin = threadIdx.x * kEach + e;
-              sh.bin_count = bc;
-              sh.bin_mass = bw;
-              sh.above_count = rc;
-              sh.above_mass = rw;
-            }
-            rc += bc;
-            rw += bw;
-          }
-          __syncthreads();
-          return uniform(sh.bin);
-        };
-        auto all_mass = [&]() {
-          unsigned long long all = 0;
-          for (int b = threadIdx.x; b < BINS; b += BLOCK) all += sh.mass[b];
-#pragma unroll
-          for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
-          if (lane == 0) sh.wave_u64[wave] = all;
-          __syncthreads();
-          all = 0;
-          for (int v = 0; v < kWaves; v++) all += sh.wave_u64[v];
-          __syncthreads();
-          return uniform(all);
-        };
-        // those of a list of this workgroup's that is not too long, into the row's
-        auto hand_on = [&](uint32_t* count, float* to_x, int* to_i) {
-          const uint32_t n = uniform(sh.listed);
-          if (threadIdx.x == 0) sh.bin = (int)atomicAdd(count, n <= (uint32_t)kListMost ? n : (uint32_t)kListMost + 1);
-          __syncthreads();
-          const uint32_t at = (uint32_t)sh.bin + threadIdx.x;
-          if (n <= (uint32_t)kListMost && threadIdx.x < n && at < (uint32_t)kListMost) {
-            to_x[at] = sh.list_x[threadIdx.x];
-            to_i[at] = sh.list_i[threadIdx.x];
-          }
-          __syncthreads();
-        };
-        bool cut = false;                          // the border is known
-        bool by_mass = !by_k;                      // top-k first, then top-p of what that left
-        bool first = true;                         // no round yet
-        uint32_t want_count = (uint32_t)s.k;
-        unsigned long long want_mass = 0;
-        uint32_t k_lo = 0, k_hi = 0;               // top-k's border
-        int k_ties = 0;
-        bool k_cut = false, k_ordered = false;
-        // Each round: everything from `from` on into coarse bins (level 0), then the border's bin into finer ones.
-#pragma unroll 1
-        while ((by_k || by_p) && !taken) {
-          uint32_t key_lo = key_from, key_hi = key_m;  // what is binned
-          int shift = 0;
-          uint32_t above_count = 0;
-          unsigned long long above_mass = 0;
-          bool found = true;
-          if (sums) want_mass = (unsigned long long)fmax(1.0, ceil(s.p * __builtin_ldexp(s1, scale_bits)));
-#pragma unroll 1
-          for (int level = 0;; level++) {
-            const bool listing = first && level == 0;
-            if (threadIdx.x == 0 && listing) sh.listed = PART == kPartExact ? sr->listed : 0;
-            for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = PART == kPartExact ? sr->bins[b] : 0; sh.mass[b] = 0; }
-            __syncthreads();
-            const float x_lo = uniform(low_value(key_lo)), x_hi = uniform(high_value(key_hi));
-            if (PART != kPartExact) each([&](int, bool, int i, const Run& e) {
-              if (!__any(largest(e, i) >= x_lo)) return;
-              float x[kRun];
-              values(e, i, x);
-              uint32_t in = 0;  // which of the run
-#pragma unroll
-              for (int j = 0; j < kRun; j++) in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
-              const bool append = listing && sh.listed <= (uint32_t)BLOCK;
-              if (!exact) {
-                // estimates: 24 bits are enough to find the bin, or the one beside it
-#pragma unroll
-                for (int j = 0; j < kRun; j++)
-                  if (x[j] >= x_lo) atomicAdd(&sh.count[bin_of(x[j])], (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - m, per_t, guess_bits)) + 0.5f));
-                if (!append) return;
-              }
-#pragma unroll 1
-              while (in) {
-                const int j = __ffs(in) - 1;
-                in &= in - 1;
-                float v = x[0];
-#pragma unroll
-                for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
-                if (exact) {
-                  const int b = level ? (int)((key_hi - key_of(v + 0.0f)) >> shift) : bin_of(v);
-                  atomicAdd(&sh.count[b], 1u);
-                  atomicAdd(&sh.mass[b], (unsigned long long)__builtin_ldexp(weight(v, m, s.per_t), scale_bits));
-                }
-                if (append) {
-                  const uint32_t at = atomicAdd(&sh.listed, 1u);
-                  if (at < (uint32_t)BLOCK) {
-                    sh.list_x[at] = v;
-                    sh.list_i[at] = start(i) + j;
-                  }
-                }
-              }
-            });
-            __syncthreads();
-            if (PART == kPartList) {
-              hand_on(&sr->listed, sr->list_x, sr->list_i);
-              if (sums)
-                for (int b = threadIdx.x; b < BINS; b += BLOCK)
-                  if (sh.count[b]) atomicAdd(&sr->bins[b], sh.count[b]);
-              break;
-            }
-            if (listing) list = uniform(sh.listed) <= (uint32_t)BLOCK;
-            if (level == 0) {
-              if (list) {
-                found = false;
-                break;
-              }
-              found = find_bin(by_mass, want_count, want_mass) >= 0;
-              if (!found) break;
-              if (!exact) break;
-              key_lo = first_key_below(uniform(sh.bin) + 1);
-              key_hi = first_key_below(uniform(sh.bin)) - 1;
-            } else {
-              (void)find_bin(by_mass, want_count - above_count, want_mass - above_mass);
-              key_hi -= (uint32_t)uniform(sh.bin) << shift;
-              const uint32_t low = key_hi - ((1u << shift) - 1);
-              key_lo = low > key_lo && low <= key_hi ? low : key_lo;
-            }
-            above_count += uniform(sh.above_count);
-            above_mass += uniform(sh.above_mass);
-            if (uniform(sh.bin_count) == 1 || !((key_hi - key_lo) >> kFixedBits<T>)) break;  // one action, or one value
-            const int width = 32 - __clz(key_hi - key_lo);
-            shift = width > __builtin_ctz(BINS) ? width - __builtin_ctz(BINS) : 0;
-            __syncthreads();
-          }
-          if (PART == kPartList) break;
-          const bool whole_list = first && list;
-          first = false;
-          if (!exact) {
-            // ---- 3: the exact sum; above the border's bin and its neighbours by segments, and those listed
-            int b = uniform(sh.bin);
-#pragma unroll 1
-            for (int attempt = 0;; attempt++) {
-              float x_lo = kInf, x_hi = kInf;  // nothing
-              int beside = 0;
-              if (found) {
-                // as many bins on either side as the list should hold, at least one (logits of 16 bits may leave some empty)
-                const float one = __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits);  // a logit's weight there
-                auto in_bin = [&](int at) { return at >= 0 && at < BINS ? (float)sh.count[at] : 0.0f; };
-                float in_list = in_bin(b);
-                for (; beside < 8; beside++) {
-                  const float more = in_bin(b - beside - 1) + in_bin(b + beside + 1);
-                  if (beside > 0 && in_list + more > one * (float)(BLOCK * 5 / 8)) break;
-                  in_list += more;
-                }
-                x_lo = uniform(low_value(first_key_below(b + uniform(beside) + 1)));
-                x_hi = uniform(high_value(first_key_below(b - uniform(beside)) - 1));
-              }
-              __syncthreads();
-              if (threadIdx.x == 0 && !whole_list) sh.listed = 0;
-              __syncthreads();
-              double sum = 0.0, here = 0.0;
-              each([&](int g, bool end, int i, const Run& e) {
-                float x[kRun];
-                values(e, i, x);
-                uint32_t in = 0;
-#pragma unroll
-                for (int j = 0; j < kRun; j++) {
-                  const double w = weight(x[j], m, s.per_t);
-                  sum += w;
-                  here += x[j] > x_hi ? w : 0.0;  // above min-p's bound too, which no bin lies below
-                  in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
-                }
-#pragma unroll 1
-                while (in) {
-                  const int j = __ffs(in) - 1;
-                  in &= in - 1;
-                  float v = x[0];
-#pragma unroll
-                  for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
-                  if (sh.listed <= (uint32_t)BLOCK) {
-                    const uint32_t at = atomicAdd(&sh.listed, 1u);
-                    if (at < (uint32_t)BLOCK) {
-                      sh.list_x[at] = v;
-                      sh.list_i[at] = start(i) + j;
-                    }
-                  }
-                }
-                if (end) {
-                  here = wave_sum(here);
-                  if (lane == 0) (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = here;
-                  here = 0.0;
-                }
-              });
-              s1 = block_sum(sum);
-              exact = true;
-              if (PART == kPartExact) {
-                if (threadIdx.x == 0) {
-                  sr->sum[part] = s1;
-                  if (!found && !whole_list) sh.listed = kListMost + 1;  // no border: kPartJoin is to find it
-                }
-                __syncthreads();
-                if (!whole_list) hand_on(&sr->around, sr->around_x, sr->around_i);
-                break;
-              }
-              if (!whole_list && found && sh.listed <= (uint32_t)BLOCK) {
-                double mine = 0.0;
-                for (int g = threadIdx.x; g < segments; g += BLOCK) mine += sh.seg_sum[g];
-                above = block_sum(mine);
-                const float v = threadIdx.x < sh.listed ? sh.list_x[threadIdx.x] : -kInf;
-                const double within = block_sum(weight(v, m, s.per_t)), target = s.p * s1;
-                list = above < target && target <= above + within;
-                if (!list) {
-                  // next to it then: the nearest bin with anything in it, once
-                  const int way = target <= above ? -1 : 1;
-                  above = 0.0;
-                  b = uniform(b + way * (beside + 1));
-                  while (b >= 0 && b < BINS && !sh.count[b]) b += way;
-                  if (attempt == 0 && b >= 0 && b < BINS) continue;
-                }
-              }
-              break;
-            }
-            if (PART == kPartExact || list) break;
-            scale_bits = 61 - __builtin_amdgcn_frexp_exp(s1);
-            continue;
-          }
-          if (whole_list) break;
-          const uint32_t bin_count = uniform(sh.bin_count);
-          const double one = found ? uniform((double)sh.bin_mass / (double)bin_count) : 0.0;
-          if (!by_mass) {
-            k_cut = found;
-            k_lo = key_lo;
-            k_hi = key_hi;
-            k_ties = (int)(want_count - above_count);
-            k_ordered = (uint32_t)k_ties < bin_count;
-            if (by_p) {
-              // top-p's share of the first k, or of all there are
-              const unsigned long long all = found ? above_mass + (unsigned long long)(one * (double)k_ties) : all_mass();
-              want_mass = (unsigned long long)fmax(1.0, ceil(s.p * (double)all));
-              by_mass = true;
-              __syncthreads();
-              continue;
-            }
-            cut = found;
-            key_lo = k_lo; key_hi = k_hi; ties = k_ties; ordered = k_ordered;
-          } else {
-            const double need = ceil((double)(want_mass - above_mass) / one);
-            cut = found;
-            ties = need < (double)bin_count ? (need > 1.0 ? (int)need : 1) : (int)bin_count;
-            ordered = (uint32_t)ties < bin_count;
-            // the border by mass counts only where it is the stricter one
-            if (k_cut && (!found || key_hi < k_hi || (key_hi == k_hi && ties > k_ties))) {
-              cut = true;
-              key_lo = k_lo; key_hi = k_hi; ties = k_ties; ordered = k_ordered;
-            }
-          }
-          if (cut) {
-            lo = low_value(key_lo);
-            hi = high_value(key_hi);
-            if (ordered) {
-              // the one value in there, by the type's fixed bits
-              const uint32_t mask = (1u << kFixedBits<T>) - 1;
-              lo = hi = value_of(key_hi & 0x80000000u ? key_hi & ~mask : (key_hi - mask) | mask);
-            }
-          }
-          break;
-        }
-        __syncthreads();
-        if (PART == kPartExact || (PART == kPartList && (by_k || by_p))) continue;
-        if (list) {
-          // ---- 4: an action a thread, sorted by value, then what is kept by index
-          const int n = uniform((int)sh.listed), me = threadIdx.x;
-          int left = n;  // of them, still in
-          auto size_for = [](int count) { return count <= 64 ? 64 : 1 << (32 - __clz(count - 1)); };
-          float x = me < n ? sh.list_x[me] : -kInf;
-          int i = me < n ? sh.list_i[me] : 0;
-          double w = 0.0;
-          // first round: by value, and the cuts; second: by index
-#pragma unroll 1
-          for (int round = 0; round < 2; round++) {
-            const bool in = me < left;
-            const unsigned long long mine = round == 0 ? (unsigned long long)key_of(x + 0.0f) << 32 | (uint32_t)~i : (unsigned long long)(uint32_t)~i << 32 | key_of(x + 0.0f);
-            const unsigned long long key = block_sort<BLOCK>(in ? mine : 0, size_for(left), sh.mass);
-            x = value_of(round == 0 ? (uint32_t)(key >> 32) : (uint32_t)key);
-            i = (int)~(round == 0 ? (uint32_t)key : (uint32_t)(key >> 32));
-            w = in ? weight(x, m, s.per_t) : 0.0;
-            if (round == 0) {
-              if (me >= s.k) w = 0.0;
-              double all;
-              const double ahead = above + (block_running(w, &all) - w);
-              const bool keep = in && me < s.k && ((me == 0 && above == 0.0) || !by_p || ahead < s.p * (by_k ? all : s1));
-              left = __syncthreads_count(keep);  // a beginning of the order
-              if (me == left - 1) {
-                sh.list_x[0] = x;
-                sh.list_i[0] = i;
-              }
-              __syncthreads();
-              lo = hi = uniform(sh.list_x[0]);
-              tie_index = uniform(sh.list_i[0]);
-              __syncthreads();
-            }
-          }
-          if (w < s.q) w = 0.0;
-          if (above == 0.0) {
-            double total;
-            const double c = block_running(w, &total);
-            // the first past the border; rounding may have put that at the total: then the last one kept
-            const unsigned long long past = __ballot(w > 0.0 && c > s.u * total), kept = __ballot(w > 0.0);
-            if (lane == 0) {
-              sh.wave_u32[wave] = past ? wave * 64 + __ffsll(past) - 1 : BLOCK;
-              sh.wave_kept[wave] = kept ? wave * 64 + 63 - __clzll(kept) : -1;
-            }
-            __syncthreads();
-            int chosen = BLOCK, last = 0;
-#pragma unroll
-            for (int q = 0; q < kWaves; q++) {
-              chosen = min(chosen, (int)sh.wave_u32[q]);
-              last = max(last, sh.wave_kept[q]);
-            }
-            if (me == (chosen < BLOCK ? chosen : last)) write_result(a, r, i, x, m, s.inv_t, total);
-            done = true;
-          } else {
-            // what is kept of the list joins its segments: the first of each segment adds up that segment's
-            double* ws = reinterpret_cast<double*>(sh.mass);
-            ws[me] = w;
-            sh.list_i[me] = me < left ? i : 0x7FFFFFFF;
-            __syncthreads();
-            const int g = i / seg_len;
-            if (me < left && (me == 0 || sh.list_i[me - 1] / seg_len != g)) {
-              double sum = 0.0;
-              for (int j = me; j < left && sh.list_i[j] / seg_len == g; j++) sum += ws[j];
-              sh.seg_sum[g] += sum;
-            }
-            by_index = true;
-          }
-        } else {
-          if (!cut) {  // everything from the bound on
-            lo = from;
-            hi = m;
-            ordered = false;
-          }
-          if (!summed) {
-          // ---- what is kept, by segments
-          double sum_here = 0.0;
-          int ties_here = 0;
-          each([&](int g, bool end, int i, const Run& e) {
-            if (__any(largest(e, i) >= lo)) {
-              float x[kRun];
-              values(e, i, x);
-#pragma unroll
-              for (int j = 0; j < kRun; j++) {
-                const bool tie = x[j] >= lo && x[j] <= hi;
-                ties_here += tie ? 1 : 0;
-                const double w = weight(x[j], m, s.per_t);
-                sum_here += (x[j] > hi || (tie && !ordered)) && w >= s.q ? w : 0.0;
-              }
-            }
-            if (end) {
-              sum_here = wave_sum(sum_here);
-              if (ordered) ties_here = wave_sum(ties_here);
-              if (lane == 0) {
-                (kOnePart ? sr->seg_sum : sh.seg_sum)[g] = sum_here;
-                sh.seg_ties[g] = ties_here;
-              }
-              sum_here = 0.0;
-              ties_here = 0;
-            }
-          });
-          }
-        }
-        __syncthreads();
-      }
-    }
-    if (kOnePart) continue;
-
-    // ---- the segment, and in it the action: one wave's work
-    if (wave == 0 && !done) {
-      int action = -1;
-      float chosen = 0.0f;
-      double total = 0.0;
-      if (m > -kInf) {
-        const int per_lane = (segments + 63) / 64, g0 = lane * per_lane, g1 = min(segments, g0 + per_lane);
-        // ties are kept by index: how many lie in the segments before.  They weigh the same.
-        double tie_weight = 0.0;
-        int tie_before = 0;
-        if (CUT && ordered) {
-          tie_weight = weight(hi, m, s.per_t);
-          if (tie_weight < s.q) tie_weight = 0.0;
-          int mine = 0;
-          for (int g = g0; g < g1; g++) mine += sh.seg_ties[g];
-          tie_before = running_sum<64>(mine) - mine;
-        }
-        auto kept_ties = [&](int before, int here) { return before >= ties ? 0 : min(here, ties - before); };
-        double sum = 0.0;
-        int tb = tie_before;
-        for (int g = g0; g < g1; g++) {
-          if (CUT && ordered) {
-            sh.seg_sum[g] += (double)kept_ties(tb, sh.seg_ties[g]) * tie_weight;
-            tb += sh.seg_ties[g];
-          }
-          sum += sh.seg_sum[g];
-        }
-        double c = group_before<64>(sum, &total);
-        const double stop = s.u * total;
-        // the lane's first segment past the border, and its last with anything kept
-        int past = -1, last = -1, past_ties = 0, last_ties = 0;
-        double past_before = 0.0;
-        tb = tie_before;
-        for (int g = g0; g < g1; g++) {
-          const double v = sh.seg_sum[g];
-          if (v > 0.0) {
-            last = g;
-            last_ties = tb;
-            if (past < 0 && c + v > stop) {
-              past = g;
-              past_ties = tb;
-              past_before = c;
-            }
-          }
-          c += v;
-          if (CUT && ordered) tb += sh.seg_ties[g];
-        }
-        const unsigned long long over = __ballot(past >= 0), any = __ballot(last >= 0);
-        const int from_lane = over ? __ffsll(over) - 1 : (any ? 63 - __clzll(any) : 0);
-        const int seg = max(0, __shfl(over ? past : last, from_lane, 64));
-        int seen = __shfl(over ? past_ties : last_ties, from_lane, 64);
-        // (rounding may have put the border at the total: then the last action of the last segment)
-        double base = over ? shfl_f64(past_before, from_lane) : -__builtin_inf();
-        bool found = false;
-#pragma unroll 1
-        for (int t = 0; t < turns && !found; t++) {
-          const int at = seg * seg_len + t * kTurn + lane * kRun, i = start(at);
-          float x[kRun];
-          double w[kRun], mine = 0.0;
-          values(load(at), at, x);
-          int equal = 0;
-#pragma unroll
-          for (int j = 0; j < kRun; j++) equal += CUT && x[j] >= lo && x[j] <= hi ? 1 : 0;
-          const int run = running_sum<64>(equal);
-          int rank = seen + run - equal;
-          seen += __shfl(run, 63, 64);
-#pragma unroll
-          for (int j = 0; j < kRun; j++) {
-            bool in = x[j] > -kInf;
-            if (CUT) {
-              const bool tie = x[j] >= lo && x[j] <= hi;
-              in = x[j] > hi || (tie && (by_index ? i + j <= tie_index : !ordered || rank < ties));
-              rank += tie ? 1 : 0;
-            }
-            w[j] = in ? weight(x[j], m, s.per_t) : 0.0;
-            if (CUT && w[j] < s.q) w[j] = 0.0;
-            mine += w[j];
-          }
-          double all, b = base + group_before<64>(mine, &all);
-          int p_at = -1, l_at = -1;
-          float p_x = 0.0f, l_x = 0.0f;
-#pragma unroll
-          for (int j = 0; j < kRun; j++) {
-            b += w[j];
-            if (w[j] > 0.0) {
-              l_at = i + j;
-              l_x = x[j];
-              if (p_at < 0 && b > stop) {
-                p_at = l_at;
-                p_x = l_x;
-              }
-            }
-          }
-          const unsigned long long o = __ballot(p_at >= 0), k = __ballot(l_at >= 0);
-          if (o || k) {  // until one is past the border, the last one kept so far
-            const int who = o ? __ffsll(o) - 1 : 63 - __clzll(k);
-            action = __shfl(o ? p_at : l_at, who, 64);
-            chosen = __shfl(o ? p_x : l_x, who, 64);
-            found = o != 0;
-          }
-          base += all;
-        }
-      }
-      if (lane == 0) write_result(a, r, action, chosen, m, s.inv_t, total);
-    }
-    __syncthreads();
-  }
-}
-
-}  // namespace
-
-namespace {
-// Workgroups a row of the large form takes: more than one where the rows alone would leave half the card idle.
-int split_parts(const SampleArgs& a, int num_cus) {
-  if (a.n <= kWideSmall || a.rows * 2 > (uint64_t)num_cus) return 1;
-  const int by_rows = num_cus / (int)a.rows, by_size = a.n / kPartActions;
-  const int parts = by_rows < by_size ? by_rows : by_size;
-  return parts < kMostParts ? parts : kMostParts;
-}
-}  // namespace
+hipError_t launch_sample_f16(const SampleArgs& a, void* workspace, int num_cus, hipStream_t stream);
+hipError_t launch_sample_bf16(const SampleArgs& a, void* workspace, int num_cus, hipStream_t stream);
 
 size_t sample_workspace(const SampleArgs& a, int num_cus) { return a.rows && split_parts(a, num_cus) > 1 ? a.rows * sizeof(SplitRow) : 0; }
 
-namespace {
-
-template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArgs& a, SplitRow* split, int num_cus, hipStream_t stream) {
-  // a launch has fewer than 2^32 threads, and grids beyond what the card holds gain nothing: the workgroups go round
-  auto grid = [&](uint64_t per_group) {
-    const uint64_t groups = (a.rows + per_group - 1) / per_group, most = (uint64_t)num_cus * 64;
-    return dim3((unsigned)(groups < most ? groups : most));
-  };
-  switch (a.n) {
-#define GX_ROW(N) case N: hipLaunchKernelGGL((row_kernel<T, N, CUT, PACKED>), grid(kBlock), dim3(kBlock), 0, stream, a); return hipGetLastError()
-    GX_ROW(1); GX_ROW(2); GX_ROW(3); GX_ROW(4); GX_ROW(5); GX_ROW(6); GX_ROW(7); GX_ROW(8);
-#undef GX_ROW
-    default: break;
-  }
-#define GX_GROUP(G, E)                                                                                                        \
-  if (a.n <= G * E) {                                                                                                         \
-    hipLaunchKernelGGL((group_kernel<T, G, E, CUT, PACKED>), grid(kBlock / G), dim3(kBlock), 0, stream, a);                   \
-    return hipGetLastError();                                                                                                 \
-  }
-  GX_GROUP(1, 16) GX_GROUP(2, 16) GX_GROUP(4, 16) GX_GROUP(8, 16) GX_GROUP(16, 16) GX_GROUP(32, 16) GX_GROUP(64, 16)
-#undef GX_GROUP
-  if (a.n <= kWideSmall) {
-    hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED, kWhole>), grid(1), dim3(256), 0, stream, a, 1, nullptr);
-    return hipGetLastError();
-  }
-#define GX_WIDE(PART, GRID) \
-  hipLaunchKernelGGL((wide_kernel<T, kWideBlock, kWideBins, kWideSegments, 32, CUT, PACKED, PART>), GRID, dim3(kWideBlock), 0, stream, a, parts, split)
-  const int parts = split_parts(a, num_cus);
-  if (parts < 2) {
-    GX_WIDE(kWhole, grid(1));
-    return hipGetLastError();
-  }
-  const dim3 all((unsigned)(a.rows * (uint64_t)parts));
-  GX_WIDE(kPartMax, all);
-  if constexpr (CUT) {
-    GX_WIDE(kPartList, all);
-    const bool top_p_alone = (a.top_p || a.top_p_all < 1.0f) && (a.top_k || a.top_k_all <= 0 || a.top_k_all >= a.n);
-    if (top_p_alone) GX_WIDE(kPartExact, all);
-  }
-  GX_WIDE(kPartJoin, grid(1));
-#undef GX_WIDE
-  return hipGetLastError();
-}
-
-template <class T> hipError_t launch_typed(const SampleArgs& a, SplitRow* split, int num_cus, hipStream_t stream) {
-  const bool cut = a.temperature || a.top_k || a.top_p || a.min_p || a.greedy_all || (a.top_k_all > 0 && a.top_k_all < a.n) ||
-                   a.top_p_all < 1.0f || a.min_p_all > 0.0f;
-  const bool packed = a.col_stride == 1;
-  if (cut) return packed ? launch_rows<T, true, true>(a, split, num_cus, stream) : launch_rows<T, true, false>(a, split, num_cus, stream);
-  return packed ? launch_rows<T, false, true>(a, split, num_cus, stream) : launch_rows<T, false, false>(a, split, num_cus, stream);
-}
-
-}  // namespace
-
 hipError_t launch_sample_logits(const SampleArgs& a, int dtype, void* workspace, int num_cus, hipStream_t stream) {
-  SplitRow* split = static_cast<SplitRow*>(workspace);
-  if (dtype == GX_F32) return launch_typed<float>(a, split, num_cus, stream);
-  if (dtype == GX_F16) return launch_typed<f16>(a, split, num_cus, stream);
-  return launch_typed<bf16>(a, split, num_cus, stream);
+  if (dtype == GX_F16) return launch_sample_f16(a, workspace, num_cus, stream);
+  if (dtype == GX_BF16) return launch_sample_bf16(a, workspace, num_cus, stream);
+  return launch_sample_typed<float>(a, static_cast<SplitRow*>(workspace), num_cus, stream);
 }
 
 }  // namespace gx

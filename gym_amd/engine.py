@@ -188,14 +188,16 @@ class DeviceBatch:
     def step_logits(self, logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """One step with actions drawn from a policy's logits [num_envs, n_actions] -> (actions int32 [num_envs],
         logprob float32 [num_envs]); the arguments are gym_amd.policy.sample_logits', u = None draws from the batch's
-        generator (gx_vec_step_logits)."""
+        generator (gx_vec_step_logits).  Runs on torch's current stream: steps enqueued on another one (stream = None is
+        the context's) must have been synchronised, and this one must be before calls that run on the context's stream
+        (get_state, get_obs, stats)."""
         from . import policy
 
         return policy.step_logits(self, logits, u, temperature, top_k, top_p, min_p)
 
     def embed_obs(self, weight, scale=1.0, dtype=None, out=None):
         """Rows of an embedding table for the batch's current Discrete observations: gym_amd.policy.embed_lookup with
-        the observation row as ids (gx_vec_embed_obs)."""
+        the observation row as ids (gx_vec_embed_obs).  On torch's current stream, as step_logits."""
         from . import policy
 
         return policy.embed_obs(self, weight, scale, dtype, out)

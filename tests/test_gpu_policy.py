@@ -639,6 +639,35 @@ def test_a_captured_turn_of_a_policy():
     b.close()
 
 
+def test_a_captured_step_of_an_env_that_refuses_actions():
+    """recording leaves nothing behind that a later wait would trip over; a replay's invalid action is reported by the wait
+    after it"""
+    trans = np.zeros((6, 5), dtype=[("next_state", np.int32), ("reward", np.float32), ("done", np.int32)])
+    trans["next_state"] = np.arange(30).reshape(6, 5) % 6
+    b = DeviceBatch(ctx(), L.ENV_TABLE, 64, table=trans)
+    b.reset()
+    logits, u = make_logits(64, 5, F32, 1)
+    b.step_logits(logits, u)
+    torch.cuda.synchronize()
+    b.wait()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a, _ = b.step_logits(logits, u)
+    b.wait()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        b.wait()
+    logits[3] = -INF
+    g.replay()
+    torch.cuda.synchronize()
+    assert int(a[3]) == -1
+    with pytest.raises(L.GymxError, match="outside the action space"):
+        b.wait()
+    b.wait()
+    b.close()
+
+
 def test_the_current_device_is_left_alone_and_the_context_stream_serves():
     """through the C entry without GX_OP_DEFAULT_STREAM: a null stream is the context's, as for the other calls"""
     import ctypes as C

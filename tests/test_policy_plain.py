@@ -134,6 +134,17 @@ def test_struct_sizes():
     assert C.sizeof(L.GxSample) == 136 and C.sizeof(L.GxEmbed) == 112
 
 
+@pytest.mark.parametrize("c_name,cs_name,ct", [("gx_sample", "GxSample", L.GxSample), ("gx_embed", "GxEmbed", L.GxEmbed)])
+def test_struct_fields_agree_in_all_three_languages(c_name, cs_name, ct):
+    import test_csharp_conformance as T
+
+    c, cs = T.header_struct(c_name), T.csharp_struct(cs_name)
+    assert [T._norm(n) for n, _ in c] == [T._norm(n) for n, _ in cs] == [T._norm(f[0]) for f in ct._fields_]
+    assert T._layout(c) == T._layout(cs) == ([getattr(ct, f[0]).offset for f in ct._fields_], C.sizeof(ct))
+    assert T.header_enum("gx_op_flags") == {"GX_OP_DEFAULT_STREAM": L.OP_DEFAULT_STREAM}
+    assert T.csharp_enum("GxOpFlags") == {"None": 0, "DefaultStream": L.OP_DEFAULT_STREAM}
+
+
 def test_python_refuses_host_tensors():
     import torch
 
