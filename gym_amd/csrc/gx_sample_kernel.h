@@ -3,13 +3,19 @@
 // The kept set is a beginning of the order "logit descending, equal logits by index", so it is described by one logit t
 // and a count j: everything above t, and the first j (by index) of those equal to t.  Weights exp((x - m) / T) and their
 // sums are binary64 (or integers of 62 bits) throughout: which action u falls on is a border in a sum of up to 2^24 terms,
-// and a sum in binary32 would move it past one action in a thousand.  The vector units do as many binary64 operations a
-// cycle as binary32 ones, so this costs registers, not time.
+// and a sum in binary32 would move it past one action in a thousand.  A binary64 instruction takes about 6 cycles of a
+// SIMD here (chains of them, measured) and an exponential some 20 of them: what bounds all but the smallest calls is
+// instructions, not memory.
 //
 // Three forms, by the number of actions:
 //   up to 8      a lane a row, every pair of actions compared (row_kernel)
-//   up to 1024   16 or 64 lanes a row, the row sorted in registers where top-k or top-p ask for it (group_kernel)
-//   more         a workgroup a row; the border of the kept set is found by histograms, never by a sort (wide_kernel)
+//   up to 1024   1 to 64 lanes a row, 16 actions a lane, the row sorted in registers where top-k or top-p ask for it
+//                (group_kernel)
+//   more         a workgroup a row, or several where there are few rows; the border of the kept set is found by histograms
+//                and a short list, never by a sort of the row (wide_kernel)
+// The borders, binary32 with top-p 0.9: 1 Mi rows of 8 take 22 us in the first form and 53 in the second, 16 384 rows of
+// 1 000 105 us in the second and 397 in the third, 8 192 rows of 2 048 412 us in the second (32 actions a lane) and 223 in
+// the third.
 #pragma once
 
 #include "gx_launch.h"
@@ -137,8 +143,9 @@ __device__ __forceinline__ void write_result(const SampleArgs& a, uint64_t r, in
 }
 
 // ------------------------------------------------------- up to 8 actions ---
-// A lane a row.  Bound by the arithmetic about as much as by memory: N exponentials, and with a cut every pair of
-// actions: the rank of an action and the mass ahead of it, which are all that the definition asks for.
+// A lane a row.  N exponentials, and with a cut every pair of actions: the rank of an action and the mass ahead of it, which
+// are all that the definition asks for.  16 Mi rows of 4 binary32 logits (470 MB) with temperature and top-p: 132 us,
+// 3.6 TB/s; a copy of as much takes 100 us and the 250 instructions a row about as long, half of them beside the loads.
 template <class T, int N, bool CUT, bool PACKED>
 __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
   for (uint64_t r = (uint64_t)blockIdx.x * kBlock + threadIdx.x; r < a.rows; r += (uint64_t)gridDim.x * kBlock) {
@@ -220,9 +227,12 @@ __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
 }
 
 // ---------------------------------------------------- up to 1024 actions ---
-// G lanes a row (16: four rows a wave), E consecutive actions a lane.  Bound by instructions.  With top-k or top-p the
-// row's values are sorted in registers (a bitonic network: the values alone, not their indices, for t and j are all that
-// is wanted), weighed in that order and summed along it; the draw then goes over the row as it lies.
+// G lanes a row, E consecutive actions a lane.  Bound by instructions.  With top-k or top-p the row's values are sorted in
+// registers (a bitonic network: the values alone, not their indices, for t and j are all that is wanted), weighed in that
+// order and summed along it; the draw then goes over the row as it lies.  Many actions a lane and many rows a wave: most
+// of the network's steps stay within a lane, and what is done once a row (parameters, scans, the logarithm) is done for
+// several at once.  65 536 rows of 255 bfloat16 (33 MB), all cuts, parameters by row: 88 us, against 118 with 4 actions a
+// lane; without a cut 36 and 42.  About 2 000 instructions a wave of four rows at 5.8 cycles are all of that time.
 template <int M> __device__ __forceinline__ float max_with(float v) { return fmaxf(v, __uint_as_float(xor_lane<M>(__float_as_uint(v)))); }
 template <int G> __device__ __forceinline__ float group_max(float v) {
   if constexpr (G > 1) v = max_with<1>(v);
@@ -409,18 +419,22 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 //   4  a short list is sorted: it ends with the border.  Where it is too long, or the estimate was wrong, the border's bin
 //      goes into finer and finer bins with integer masses (whose order of adding changes nothing) until it holds one
 //      value, and a last pass adds up what is kept by segments
-// then the segment u falls into, and in it the action.  The passes are bound by instructions: 20 an exponential in
-// binary64, so step 3 is the only one that takes them of every action.  What runs for few elements is a loop: unrolled,
-// the kernel outgrew the instruction cache and took three times as long.
+// then the segment u falls into, and in it the action.  The passes are bound by instructions, so step 3 is the only one that
+// takes an exponential in binary64 of every action.  256 rows of 131 072 bfloat16 (67 MB, a copy 14 us): 99 us with top-p
+// 0.9 (14 us step 1, 25 step 2, 40 step 3, the rest for the list and the draw), 37 with top-k 50, 41 without a cut.  What
+// runs for few elements is a loop: unrolled, the kernel outgrew the instruction cache and took three times as long.  512
+// threads, not 1 024: those leave a lane 128 registers, and what spilled waited behind the loads on their way (113 and 53 us
+// for the first two).  Rows of up to 4 096 have 256 threads (4 096 rows of as many, top-p: 143 us, 341 with 512).
 //
 // Few rows leave most of the card idle, so each is split among several workgroups (parts), and the steps become launches
 // that hand their results on in the workspace: kPartMax is step 1, kPartList step 2 (and for min-p alone the segments'
 // sums), kPartExact step 3, kPartJoin the rest, by one workgroup a row.  Where a step says that the row needs more than
-// that (a list too long, +inf among the logits, k above kListMost), kPartJoin goes through the row by itself.
+// that (a list too long, +inf or NaN among the logits, k above kListMost), kPartJoin goes through the row by itself.  One
+// row of 131 072: 46 us with top-p against 94 by one workgroup, 27 against 31 with top-k (three launches of 6 to 11 us);
+// 37 rows of 50 001 with min-p 25 against 35.
 constexpr int kWideSmall = 4096;
 constexpr int kAhead = 2;
-// Actions a part has at least.  One row of 131 072, top-p: 46 us with 8 192, 50 with 16 384, 44 with 4 096, whose 32 parts
-// find their lists too long sooner.
+// Actions a part has at least.  One row of 131 072, top-p: 50 us with 16 384, 46 with 8 192, 44 with 4 096.
 constexpr int kPartActions = 8192;
 enum Part { kWhole = 0, kPartMax = 1, kPartList = 2, kPartExact = 3, kPartJoin = 4 };
 constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock;

@@ -372,8 +372,9 @@ typedef enum gx_op_flags { GX_OP_DEFAULT_STREAM = 1u } gx_op_flags;
  *   top_p        of those, the shortest beginning of the order whose weight reaches p times theirs, at least one
  *   min_p        of those, the ones with w >= min_p (the largest has w = 1)
  *   draw         the first action IN INDEX ORDER at which the sum of the weights kept exceeds u times their total
- * Weights and sums are binary64: the action is the one exact arithmetic gives but where u or p lies within a few 1e-12
- * (relative) of a border.  A row of logits that are all -inf (every action masked): action -1, log-probability -inf;
+ * Weights and sums are binary64: the action is the one exact arithmetic gives but where u or p lies within a few
+ * 1e-12 (relative; 1e-10 at 2^24 actions) of a border.  u is read as it is, so binary32's 24 bits are what an action's
+ * share of the probability is resolved to.  A row of logits that are all -inf (every action masked): action -1, log-probability -inf;
  * with +inf among the logits, those share the probability.  T = +inf is uniform over what is not -inf. */
 typedef struct gx_sample {
   uint32_t struct_size;      /* sizeof(gx_sample) */
@@ -398,7 +399,8 @@ typedef struct gx_sample {
   float min_p_all;
   int32_t* actions;          /* out [rows] */
   float* logprob;            /* out [rows], may be NULL: log of the probability the action was drawn with */
-  void* workspace;           /* 256-byte aligned device memory of gx_sample_workspace's size; may be NULL where that is 0 */
+  void* workspace;           /* 256-byte aligned device memory of gx_sample_workspace's size (which follows from rows and
+                                n_actions alone: not 0 for few rows of many actions only); may be NULL where that is 0 */
   uint64_t workspace_bytes;
 } gx_sample;
 int gx_sample_workspace(gx_ctx* ctx, const gx_sample* sample, uint64_t* bytes);
