@@ -834,7 +834,9 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
         }
         // ---- 2: a bound below everything that can be kept (weights below exp(-745) are 0) ...
         double bound = (double)m - 745.0 / s.inv_t;
-        if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * s1 * 0.99 / (double)a.n, 1e-320)) / s.inv_t);
+        // (the estimate is too large where log2(e) / T is too large for binary32; m's own weight, 1, is below any sum)
+        const double least = s.per_t < 3e38 ? s1 * 0.99 : 1.0;
+        if (sums) bound = fmax(bound, (double)m + log(fmax((1.0 - s.p) * least / (double)a.n, 1e-320)) / s.inv_t);
         if (!by_k && s.q > 0.0) bound = fmax(bound, (double)m + log(s.q) / s.inv_t);
         float from = fminf(m, fmaxf((float)(bound - fabs(bound) * 1e-6), -3.402823466e38f));
         if (far_k) from = fminf(m, fmaxf(bottom, from));
@@ -877,7 +879,8 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
         if (PART == kPartMax) continue;
         // ---- ... and the bins
         from = uniform(from);
-        const float per = m > from ? (float)(BINS - 1) / (m - from) : 0.0f;
+        // (finite: m's own bin has to be 0, and 0 * inf is not)
+        const float per = m > from ? fminf((float)(BINS - 1) / (m - from), 3e38f) : 0.0f;
         auto bin_of = [&](float x) { return (int)fminf((m - x) * per, (float)(BINS - 1)); };
         const uint32_t key_from = uniform(key_of(from + 0.0f)), key_m = uniform(key_of(m + 0.0f));
         // the smallest key whose bin is below b (one past the largest where b is 0): bin_of falls as the key rises.  The
@@ -992,7 +995,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
           bool found = true;
           if (sums) want_mass = (unsigned long long)fmax(1.0, ceil(s.p * __builtin_ldexp(s1, scale_bits)));
 #pragma unroll 1
-          for (int level = 0;; level++) {
+          for (int level = 0; level < 5; level++) {  // (keys of 32 bits, 9 or 11 a level)
             const bool listing = first && level == 0;
             if (threadIdx.x == 0 && listing) sh.listed = PART == kPartExact ? sr->listed : 0;
             for (int b = threadIdx.x; b < BINS; b += BLOCK) { sh.count[b] = PART == kPartExact ? sr->bins[b] : 0; sh.mass[b] = 0; }

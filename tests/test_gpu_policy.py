@@ -112,6 +112,19 @@ def test_split_rows(rows):
         check_sample(x[few], u[few], got=(got[0][few], got[1][few]), **cut)
 
 
+@pytest.mark.parametrize("rows", [2, 150])
+def test_temperatures_below_the_smallest_normal_number(rows):
+    """1 / T is no binary32 number there, nor is one over the distance between the largest logit and the smallest kept"""
+    for i, n in enumerate([700, 5000, 20_011]):
+        for t in (1e-38, 1e-40, 5e-42):
+            for dtype in (F32, BF16):
+                x, u = make_logits(rows, n, F32, n + i)
+                x = (-(x * 3).abs().double() * t).to(dtype)
+                x[1::2, ::2] = 0.0
+                for cut in (dict(top_p=0.5), dict(top_p=1e-3), dict(top_k=n // 3), dict(top_k=n // 2, top_p=0.7), dict(min_p=0.5), {}):
+                    check_sample(x[:6], u[:6], got=tuple(v[:6] for v in policy.sample_logits(x, u, temperature=t, **cut)), temperature=t, **cut)
+
+
 def test_many_rows():
     """more rows than any grid has lanes for, small action spaces: a sample of them in binary64, the rest by two runs"""
     for n, cut in [(2, {}), (4, dict(temperature=0.7, top_p=0.95)), (6, dict(top_k=3)), (17, dict(top_p=0.5))]:
