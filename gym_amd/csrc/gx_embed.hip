@@ -348,17 +348,24 @@ __global__ void __launch_bounds__(kBlock) scan_tiles_kernel(uint32_t* counts, ui
   if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
+// The tile is sorted in LDS first, so that its pairs leave in runs of one digit.
 __global__ void __launch_bounds__(kSortThreads) scatter_kernel(EmbedArgs a, const Pair* pairs, uint32_t tiles, int shift, int digit,
                                                                const uint32_t* counts, const uint32_t* totals, Pair* out) {
   constexpr int kWaves = kSortThreads / 64, kEach = kTile / kSortThreads;
-  __shared__ uint32_t place[1 << kMaxDigit];         // where the digit's next token of this tile goes
-  __shared__ uint16_t seen[kWaves][1 << kMaxDigit];  // tokens of the digit in each wave's stretch, then in those before it
+  __shared__ union {
+    struct {
+      uint32_t start[1 << kMaxDigit];         // of the digit's tokens, in this tile
+      uint16_t seen[kWaves][1 << kMaxDigit];  // tokens of the digit in each wave's stretch, then in those before it
+    } s;
+    Pair pairs[kTile];  // by digit
+  } sh;
+  __shared__ uint32_t place[1 << kMaxDigit];  // of the digit's tokens among all, less their place in this tile
   __shared__ uint32_t sums[kWaves];
   const int n_bins = 1 << digit, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int b = threadIdx.x; b < n_bins; b += kSortThreads) {
     place[b] = totals[b];
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) seen[w][b] = 0;
+    for (int w = 0; w < kWaves; w++) sh.s.seen[w][b] = 0;
   }
   __syncthreads();
   scan_lds(place, n_bins, sums);
@@ -375,29 +382,42 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(EmbedArgs a, cons
     const bool live = first + e * 64 < a.tokens;
     const uint32_t d = live ? (p[e].key >> shift) & (n_bins - 1) : 0;
     const unsigned long long same = same_digit(d, digit, __ballot(live)), below = same & ((1ull << lane) - 1);
-    const uint32_t before = live ? seen[wave][d] : 0;
+    const uint32_t before = live ? sh.s.seen[wave][d] : 0;
     wave_order();
     rank[e] = before + __popcll(below);
-    if (live && below == 0) seen[wave][d] = (uint16_t)(before + __popcll(same));
+    if (live && below == 0) sh.s.seen[wave][d] = (uint16_t)(before + __popcll(same));
     wave_order();
   }
   __syncthreads();
   for (int b = threadIdx.x; b < n_bins; b += kSortThreads) {
-    place[b] += counts[(size_t)b * tiles + blockIdx.x];
     uint32_t run = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
-      const uint32_t here = seen[w][b];
-      seen[w][b] = (uint16_t)run;
+      const uint32_t here = sh.s.seen[w][b];
+      sh.s.seen[w][b] = (uint16_t)run;
       run += here;
     }
+    sh.s.start[b] = run;
   }
   __syncthreads();
+  scan_lds(sh.s.start, n_bins, sums);
+  for (int b = threadIdx.x; b < n_bins; b += kSortThreads) place[b] += counts[(size_t)b * tiles + blockIdx.x] - sh.s.start[b];
 #pragma unroll
-  for (int e = 0; e < kEach; e++) {
-    if (first + e * 64 >= a.tokens) continue;
-    const uint32_t d = (p[e].key >> shift) & (n_bins - 1);
-    out[place[d] + seen[wave][d] + rank[e]] = p[e];
+  for (int e = 0; e < kEach; e++)
+    if (first + e * 64 < a.tokens) {
+      const uint32_t d = (p[e].key >> shift) & (n_bins - 1);
+      rank[e] += sh.s.start[d] + sh.s.seen[wave][d];
+    }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; e++)
+    if (first + e * 64 < a.tokens) sh.pairs[rank[e]] = p[e];
+  __syncthreads();
+  const uint64_t left = a.tokens - (uint64_t)blockIdx.x * kTile;
+  const uint32_t here = left < kTile ? (uint32_t)left : kTile;
+  for (uint32_t i = threadIdx.x; i < here; i += kSortThreads) {
+    const Pair q = sh.pairs[i];
+    out[place[(q.key >> shift) & (n_bins - 1)] + i] = q;
   }
 }
 
