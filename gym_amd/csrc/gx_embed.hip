@@ -88,14 +88,18 @@ __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_s
 //   2  the sorted tokens are cut into chunks of equal length whatever the runs of equal ids, so that one state with most
 //      of the tokens is no more work than many.  A group of lanes adds up one chunk: a run that lies inside is written
 //      to the table, what a run has in a chunk it enters or leaves at a border goes to the workspace.
-//   3  runs over several chunks are joined from those parts, in order, in binary64.
+//   3  runs over several chunks are joined from those parts, in order, in binary64; of a run that goes over kFold chunks
+//      that begin at a multiple of kFold, their parts have been added up before, in a launch of its own (5 us; with all
+//      tokens in one state, 4 Mi of 128 columns take 271 us so and 408 without, 8 191 of 1 001 42 and 99).
 // Every addition's place follows from the ids alone: equal calls, equal bits.
-// Bound by the rows it reads: 4 Mi tokens of 128 bfloat16 and 704 states (1.07 GB) take 306 us, 216 of them step 2 at
-// 5.0 TB/s, whatever the order of the ids; 67 the sort (48 its scatter, whose pairs leave in runs of some 20), 26 step 3.
-// 8 191 tokens of 1 001 columns and 50 001 states: 76 us, 32 of them the 200 MB that are cleared while the tokens are sorted.
+// Bound by the rows it reads: 4 Mi tokens of 128 bfloat16 and 704 states (1.07 GB) take 282 us, 216 of them step 2 at
+// 5.0 TB/s, whatever the order of the ids; 56 the sort (37 its scatter: 48 when the pairs left for their places one by one,
+// not in the runs that a sort of the tile in LDS makes of them), 17 step 3.  8 191 tokens of 1 001 columns and 50 001 states:
+// 78 us, 32 of them the 200 MB that are cleared while the tokens are sorted.
 constexpr int kSortOne = 8192, kSortThreads = 1024;  // tokens one workgroup sorts alone
 constexpr int kTile = 16384;                         // tokens of a tile, 16 a thread
 constexpr int kMaxDigit = 10;
+constexpr int kFold = 64;  // chunks whose parts of a long run become one
 
 struct __align__(8) Pair { uint32_t key, token; };
 
@@ -107,7 +111,7 @@ struct GradPlan {
   int lanes_shift;          // lanes of a group: 8 columns each
   int64_t col_tiles;        // groups a row takes
   uint32_t chunk, chunks;   // tokens of a chunk, number of chunks
-  size_t pairs_a, pairs_b, counts, totals, parts, bytes;  // offsets into the workspace
+  size_t pairs_a, pairs_b, counts, totals, parts, folds, bytes;  // offsets into the workspace
 };
 
 // a launch has fewer than 2^32 threads: beyond that the workgroups go round
@@ -154,6 +158,7 @@ GradPlan grad_plan(const EmbedArgs& a, int num_cus) {
     p.totals = take((size_t)4 << p.digit);
   }
   if (p.chunks > 1) p.parts = take((size_t)p.chunks * 2 * (size_t)a.dim * 4);
+  if (p.chunks > 2 * (uint32_t)kFold) p.folds = take((size_t)(p.chunks / kFold) * (size_t)a.dim * 4);
   p.bytes = n ? at : 0;
   return p;
 }
@@ -517,48 +522,102 @@ __global__ void __launch_bounds__(kBlock) sum_kernel(EmbedArgs a, int lanes_shif
   }
 }
 
-// The runs that leave the chunk they begin in: a wave looks at one chunk's end and, if such a run begins there, adds up its
-// parts, 256 columns, four a lane.  Runs of more than kJoinAlone parts are added by the whole workgroup.
 constexpr int kJoinWaves = 8, kJoinAlone = 32;
 
+// Parts first, first + step, .. below count added up in binary64, four columns from c on; at(k) is where a part's columns
+// begin.  The wave's groups of lanes take different parts; every lane of a column ends with the wave's sum.
+template <class F>
+__device__ __forceinline__ void add_parts(uint32_t first, uint32_t count, uint32_t step, int64_t c, int64_t dim, int lanes_shift, F at, double* sum) {
+  const int cols = dim - c < 4 ? (int)(dim - c) : 4;  // may be <= 0
+  if (cols == 4) {
+    for (uint32_t k = first; k < count; k += 8 * step) {
+      Pack<float, 4> x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = load_pack<float, 4>(at(k + e * step < count ? k + e * step : count - 1) + c);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (k + e * step < count)
+#pragma unroll
+          for (int j = 0; j < 4; j++) sum[j] += (double)x[e].v[j];
+    }
+  } else {
+    for (uint32_t k = first; k < count; k += step)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (j < cols) sum[j] += (double)at(k)[c + j];
+  }
+  for (int d = 1 << lanes_shift; d < 64; d <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; j++) sum[j] += shfl_xor_f64(sum[j], d);
+}
+
+// A workgroup looks at kFold chunks and, if one run goes through all of them, adds up their parts, 256 columns.
+__global__ void __launch_bounds__(64 * kJoinWaves) fold_kernel(EmbedArgs a, int lanes_shift, uint32_t chunk, uint32_t chunks, const Pair* pairs,
+                                                               const float* parts, float* folds) {
+  __shared__ double sums[kJoinWaves][256];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int group = lane >> lanes_shift, n_groups = 64 >> lanes_shift;
+  const uint64_t col_tiles = (uint64_t)(a.dim + 255) / 256, units = (uint64_t)(chunks / kFold) * col_tiles;
+  for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const uint32_t c0 = (uint32_t)(u / col_tiles) * kFold;
+    if (c0 == 0 || c0 + kFold >= chunks) continue;
+    const uint32_t key = pairs[c0 * chunk - 1].key;
+    if (key >= (uint32_t)a.n_states || pairs[(c0 + kFold) * chunk].key != key) continue;
+    const int64_t base = (int64_t)(u % col_tiles) * 256, c = base + (int64_t)(lane & ((1 << lanes_shift) - 1)) * 4;
+    double sum[4] = {};
+    add_parts(wave * n_groups + group, kFold, kJoinWaves * n_groups, c, a.dim, lanes_shift,
+              [&](uint32_t k) { return parts + (size_t)(c0 + k) * 2 * (size_t)a.dim; }, sum);
+    if (group == 0)
+#pragma unroll
+      for (int j = 0; j < 4; j++) sums[wave][lane * 4 + j] = sum[j];
+    __syncthreads();
+    if (threadIdx.x < (4u << lanes_shift) && base + threadIdx.x < a.dim) {
+      double all = 0.0;
+#pragma unroll
+      for (int q = 0; q < kJoinWaves; q++) all += sums[q][threadIdx.x];
+      folds[(size_t)(c0 / kFold) * (size_t)a.dim + base + threadIdx.x] = (float)all;
+    }
+    __syncthreads();
+  }
+}
+
+// The runs that leave the chunk they begin in: a wave looks at one chunk's end and, if such a run begins there, adds up its
+// parts, 256 columns, four a lane.  Runs of more than kJoinAlone parts are added by the whole workgroup.
 template <class T>
 __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(EmbedArgs a, int lanes_shift, uint32_t chunk, uint32_t chunks, const Pair* pairs,
-                                                               const float* parts) {
+                                                               const float* parts, const float* folds) {
   __shared__ double sums[kJoinWaves][256];
   __shared__ uint32_t long_last[kJoinWaves];  // the run's last chunk, 0: none for the workgroup
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int group = lane >> lanes_shift, n_groups = 64 >> lanes_shift;
-  const uint64_t col_tiles = (uint64_t)(a.dim + 255) / 256, units = (uint64_t)(chunks - 1) * col_tiles;  // the last chunk has nothing to join
-  // parts first, first + step, .. last of the run that begins in c0, in four columns from c on
-  auto add_parts = [&](uint32_t c0, uint32_t first, uint32_t last, uint32_t step, int64_t c, double* sum) {
-    const int cols = a.dim - c < 4 ? (int)(a.dim - c) : 4;  // may be <= 0
-    auto part = [&](uint32_t k) { return parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * (size_t)a.dim + c; };
-    uint32_t k = first;
-    if (cols == 4) {
-      for (; k <= last; k += 8 * step) {
-        Pack<float, 4> x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = load_pack<float, 4>(part(k + e * step <= last ? k + e * step : last));
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (k + e * step <= last)
-#pragma unroll
-            for (int j = 0; j < 4; j++) sum[j] += (double)x[e].v[j];
-      }
-    } else {
-      for (; k <= last; k += step)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (j < cols) sum[j] += (double)part(k)[j];
-    }
-    for (int d = 1 << lanes_shift; d < 64; d <<= 1)
-#pragma unroll
-      for (int j = 0; j < 4; j++) sum[j] += shfl_xor_f64(sum[j], d);
+  // (the last chunk has nothing to join; all chunks' first columns, then their next: a run's are several workgroups' work)
+  const uint64_t ends = chunks - 1, units = ends * ((uint64_t)(a.dim + 255) / 256);
+  // The parts of the run from chunk c0 to chunk `last`: those before the first multiple of kFold, the folded ones, and those
+  // behind them.
+  struct Parts { uint32_t c0, head, folded, fold0, tail0, count; };
+  auto parts_of = [&](uint32_t c0, uint32_t last) {
+    Parts p;
+    const uint32_t f0 = c0 / kFold + 1, f1 = last / kFold;  // folds f0 .. f1 - 1
+    p.c0 = c0;
+    p.folded = folds && f1 > f0 ? f1 - f0 : 0;
+    p.head = p.folded ? f0 * kFold - c0 : last - c0 + 1;
+    p.fold0 = f0;
+    p.tail0 = f1 * kFold;
+    p.count = p.folded ? p.head + p.folded + (last - p.tail0 + 1) : p.head;
+    return p;
+  };
+  auto add = [&](const Parts& p, uint32_t first, uint32_t step, int64_t c, double* sum) {
+    add_parts(first, p.count, step, c, a.dim, lanes_shift, [&](uint32_t k) {
+      const uint32_t in_tail = k - p.head - p.folded;  // (of those)
+      const uint32_t at = k < p.head ? p.c0 + k : p.tail0 + in_tail;
+      const float* single = parts + ((size_t)at * 2 + (k == 0 ? 1 : 0)) * (size_t)a.dim;
+      return k < p.head || k >= p.head + p.folded ? single : folds + (size_t)(p.fold0 + (k - p.head)) * (size_t)a.dim;
+    }, sum);
   };
   for (uint64_t u0 = (uint64_t)blockIdx.x * kJoinWaves; u0 < units; u0 += (uint64_t)gridDim.x * kJoinWaves) {
     const uint64_t u = u0 + wave;
-    const uint32_t c0 = (uint32_t)(u / col_tiles);
-    const int64_t col0 = (int64_t)(u % col_tiles) * 256;
+    const uint32_t c0 = (uint32_t)(u % ends);
+    const int64_t col0 = (int64_t)(u / ends) * 256;
     uint32_t last = 0, key = 0;
     if (u < units) {
       // the last token of the chunk, the one after it, the last of the chunk before
@@ -583,12 +642,13 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(EmbedArgs a, int 
         }
       }
     }
-    const bool alone = last - c0 < (uint32_t)kJoinAlone;
+    const Parts mine = parts_of(c0, last);
+    const bool alone = mine.count <= (uint32_t)kJoinAlone;
     if (lane == 0) long_last[wave] = last && !alone ? last : 0;
     if (last && alone) {
       const int64_t c = col0 + (int64_t)(lane & ((1 << lanes_shift) - 1)) * 4;
       double sum[4] = {};
-      add_parts(c0, c0 + group, last, n_groups, c, sum);
+      add(mine, group, n_groups, c, sum);
       if (group == 0)
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -598,10 +658,10 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(EmbedArgs a, int 
     for (int w = 0; w < kJoinWaves; w++) {
       const uint32_t long_end = long_last[w];
       if (!long_end) continue;
-      const uint32_t l0 = (uint32_t)((u0 + w) / col_tiles);
-      const int64_t base = (int64_t)((u0 + w) % col_tiles) * 256, c = base + (int64_t)(lane & ((1 << lanes_shift) - 1)) * 4;
+      const uint32_t l0 = (uint32_t)((u0 + w) % ends);
+      const int64_t base = (int64_t)((u0 + w) / ends) * 256, c = base + (int64_t)(lane & ((1 << lanes_shift) - 1)) * 4;
       double sum[4] = {};
-      add_parts(l0, l0 + wave * n_groups + group, long_end, kJoinWaves * n_groups, c, sum);
+      add(parts_of(l0, long_end), wave * n_groups + group, kJoinWaves * n_groups, c, sum);
       if (group == 0)
 #pragma unroll
         for (int j = 0; j < 4; j++) sums[wave][lane * 4 + j] = sum[j];
@@ -749,9 +809,13 @@ hipError_t launch_embed_grad(const EmbedArgs& a, int table, int rows, void* work
     if (e != hipSuccess || p.chunks < 2) return e;
     int join_shift = 0;  // lanes a row at four columns each
     while (join_shift < 6 && ((int64_t)4 << join_shift) < a.dim) join_shift++;
-    const uint64_t units = (uint64_t)(p.chunks - 1) * ((uint64_t)(a.dim + 255) / 256);
+    const uint64_t join_tiles = (uint64_t)(a.dim + 255) / 256, units = (uint64_t)(p.chunks - 1) * join_tiles;
+    float* folds = p.folds ? reinterpret_cast<float*>(ws + p.folds) : nullptr;
+    if (folds)
+      hipLaunchKernelGGL(fold_kernel, dim3(capped((uint64_t)(p.chunks / kFold) * join_tiles)), dim3(64 * kJoinWaves), 0, stream, a, join_shift, p.chunk,
+                         p.chunks, pairs, parts, folds);
     hipLaunchKernelGGL(join_kernel<T>, dim3(capped((units + kJoinWaves - 1) / kJoinWaves)), dim3(64 * kJoinWaves), 0, stream, a, join_shift,
-                       p.chunk, p.chunks, pairs, parts);
+                       p.chunk, p.chunks, pairs, parts, folds);
     return hipGetLastError();
   });
 }

@@ -350,6 +350,22 @@ def test_grad_few_states_many_tokens():
         assert torch.equal(a, policy.embed_grad(grad, ids, states, scale=2.0))
 
 
+@pytest.mark.parametrize("dim", [1, 4, 30, 257, 300])
+def test_grad_runs_that_begin_and_end_anywhere(dim):
+    """runs of a few chunks, of many and of whole multiples of them, one token more or less (a chunk has 8 tokens here)"""
+    tokens = 40_000 if dim < 100 else 9000
+    for shift in (0, 1, 5, 511, 512, 513):
+        lengths = [shift, 512, 1, 1023, 1025, 511, 7, 520, 4096, 1537, 2048, 3]
+        ids = torch.cat([torch.full((n,), 3 * i, dtype=torch.int32) for i, n in enumerate(lengths)])[:tokens]
+        ids = torch.cat([ids, torch.full((tokens - len(ids),), 40, dtype=torch.int32)]).cuda()
+        g = gen(dim + shift)
+        grad = torch.randn(tokens, dim, generator=g, device="cuda")
+        mixed = torch.randperm(tokens, generator=g, device="cuda")
+        check_grad(grad, ids, 50, -1.5)
+        check_grad(grad, ids[mixed], 50)
+        check_grad(grad, torch.where(ids == 40, 50, ids), 50)  # the longest run outside the table
+
+
 @pytest.mark.parametrize("tokens", [8191, 8192, 8193, 12_289, 70_000])
 def test_grad_sizes_of_the_sort(tokens):
     """one workgroup's sort and the tiles', one to three digits"""
