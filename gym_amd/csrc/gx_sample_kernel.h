@@ -1016,6 +1016,21 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
                   if (x[j] >= x_lo) atomicAdd(&sh.count[bin_of(x[j])], (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - m, per_t, guess_bits)) + 0.5f));
                 if (!append) return;
               }
+              if (exact && !append) {
+                // a stretch of one value, all of the wave's: at once (a row of equal logits has nothing else)
+                const float v = uniform(x[0]);
+                bool same = in == (1u << kRun) - 1;
+#pragma unroll
+                for (int j = 0; j < kRun; j++) same = same && x[j] == v;
+                if (__all(same)) {
+                  if (lane == 0) {
+                    const int b = level ? (int)((key_hi - key_of(v + 0.0f)) >> shift) : bin_of(v);
+                    atomicAdd(&sh.count[b], 64u * kRun);
+                    atomicAdd(&sh.mass[b], 64ull * kRun * (unsigned long long)__builtin_ldexp(weight(v, m, s.per_t), scale_bits));
+                  }
+                  return;
+                }
+              }
 #pragma unroll 1
               while (in) {
                 const int j = __ffs(in) - 1;
@@ -1080,13 +1095,13 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
               float x_lo = kInf, x_hi = kInf;  // nothing
               int beside = 0;
               if (found) {
-                // as many bins on either side as the list should hold, at least one (logits of 16 bits may leave some empty)
+                // as many bins on either side as the list should hold; one, if it can
                 const float one = __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits);  // a logit's weight there
                 auto in_bin = [&](int at) { return at >= 0 && at < BINS ? (float)sh.count[at] : 0.0f; };
                 float in_list = in_bin(b);
                 for (; beside < 8; beside++) {
                   const float more = in_bin(b - beside - 1) + in_bin(b + beside + 1);
-                  if (beside > 0 && in_list + more > one * (float)(BLOCK * 5 / 8)) break;
+                  if (in_list + more > one * (float)(beside > 0 ? BLOCK * 5 / 8 : BLOCK * 7 / 8)) break;
                   in_list += more;
                 }
                 x_lo = uniform(low_value(first_key_below(b + uniform(beside) + 1)));
