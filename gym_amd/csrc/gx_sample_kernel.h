@@ -437,7 +437,7 @@ constexpr int kAhead = 2;
 // Actions a part has at least.  One row of 131 072, top-p: 50 us with 16 384, 46 with 8 192, 44 with 4 096.
 constexpr int kPartActions = 8192;
 enum Part { kWhole = 0, kPartMax = 1, kPartList = 2, kPartExact = 3, kPartJoin = 4 };
-constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock;
+constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock, kZoom = 64;
 
 struct SplitRow {
   double sum[kMostParts];       // of each part: exact, and estimated relative to its largest logit
@@ -965,6 +965,16 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
           __syncthreads();
           return uniform(all);
         };
+        // a stretch of one value, all of the wave's (a row of equal logits has nothing else)?  It is counted at once.
+        auto one_value = [&](const float* x) {
+          const float v = uniform(x[0]);
+          bool same = x[0] == v && x[kRun - 1] == v;
+          if (!__all(same)) return false;
+#pragma unroll
+          for (int j = 1; j < kRun - 1; j++) same = same && x[j] == v;
+          return (bool)__all(same);
+        };
+        auto guess_of = [&](float x) { return (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(x - m, per_t, guess_bits)) + 0.5f); };
         // those of a list of this workgroup's that is not too long, into the row's
         auto hand_on = [&](uint32_t* count, float* to_x, int* to_i) {
           const uint32_t n = uniform(sh.listed);
@@ -1011,22 +1021,21 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
               const bool append = listing && sh.listed <= (uint32_t)BLOCK;
               if (!exact) {
                 // estimates: 24 bits are enough to find the bin, or the one beside it
+                if (one_value(x)) {
+                  if (lane == 0 && x[0] >= x_lo) atomicAdd(&sh.count[bin_of(x[0])], 64u * kRun * guess_of(x[0]));
+                } else {
 #pragma unroll
-                for (int j = 0; j < kRun; j++)
-                  if (x[j] >= x_lo) atomicAdd(&sh.count[bin_of(x[j])], (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - m, per_t, guess_bits)) + 0.5f));
+                  for (int j = 0; j < kRun; j++)
+                    if (x[j] >= x_lo) atomicAdd(&sh.count[bin_of(x[j])], guess_of(x[j]));
+                }
                 if (!append) return;
               }
               if (exact && !append) {
-                // a stretch of one value, all of the wave's: at once (a row of equal logits has nothing else)
-                const float v = uniform(x[0]);
-                bool same = in == (1u << kRun) - 1;
-#pragma unroll
-                for (int j = 0; j < kRun; j++) same = same && x[j] == v;
-                if (__all(same)) {
+                if (one_value(x) && __all(in & 1)) {
                   if (lane == 0) {
-                    const int b = level ? (int)((key_hi - key_of(v + 0.0f)) >> shift) : bin_of(v);
+                    const int b = level ? (int)((key_hi - key_of(x[0] + 0.0f)) >> shift) : bin_of(x[0]);
                     atomicAdd(&sh.count[b], 64u * kRun);
-                    atomicAdd(&sh.mass[b], 64ull * kRun * (unsigned long long)__builtin_ldexp(weight(v, m, s.per_t), scale_bits));
+                    atomicAdd(&sh.mass[b], 64ull * kRun * (unsigned long long)__builtin_ldexp(weight(x[0], m, s.per_t), scale_bits));
                   }
                   return;
                 }
@@ -1090,22 +1099,60 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
           if (!exact) {
             // ---- 3: the exact sum; above the border's bin and its neighbours by segments, and those listed
             int b = uniform(sh.bin);
+            // Where the border's bin holds more than the list (a flat row), that bin and those beside it again, in kZoom bins:
+            // 256 rows of 131 072, spread 0.05, 137 us, 300 by the finer and finer bins of step 4
+            float z_hi = 0.0f, z_per = 0.0f;
+            if (!kOnePart && found) {
+              const float one = __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits);
+              const float z_lo = uniform(low_value(first_key_below(min(b + 2, BINS))));
+              const unsigned long long z_above = uniform(sh.above_mass) - ((unsigned long long)(b > 0 ? sh.count[b - 1] : 0) << guess_shift);
+              z_hi = uniform(high_value(first_key_below(b - 1) - 1));
+              if ((float)sh.count[b] > one * (float)(BLOCK * 7 / 8) && z_hi > z_lo) {
+                z_per = fminf((float)kZoom / (z_hi - z_lo), 3e38f);
+                __syncthreads();
+                for (int q = threadIdx.x; q < BINS; q += BLOCK) sh.count[q] = 0;
+                __syncthreads();
+                each([&](int, bool, int i, const Run& e) {
+                  if (!__any(largest(e, i) >= z_lo)) return;
+                  float x[kRun];
+                  values(e, i, x);
+                  auto zoom_bin = [&](float v) { return (int)fminf((z_hi - v) * z_per, (float)(kZoom - 1)); };
+                  if (one_value(x)) {
+                    if (lane == 0 && x[0] >= z_lo && x[0] <= z_hi) atomicAdd(&sh.count[zoom_bin(x[0])], 64u * kRun * guess_of(x[0]));
+                    return;
+                  }
+#pragma unroll
+                  for (int j = 0; j < kRun; j++)
+                    if (x[j] >= z_lo && x[j] <= z_hi) atomicAdd(&sh.count[zoom_bin(x[j])], guess_of(x[j]));
+                });
+                __syncthreads();
+                const int z = find_bin(true, 0, want_mass - z_above);
+                b = z < 0 ? kZoom - 1 : z;
+              }
+            }
 #pragma unroll 1
             for (int attempt = 0;; attempt++) {
               float x_lo = kInf, x_hi = kInf;  // nothing
               int beside = 0;
               if (found) {
                 // as many bins on either side as the list should hold; one, if it can
-                const float one = __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits);  // a logit's weight there
+                const float down = z_per > 0.0f ? (m - z_hi) + (float)b / z_per : (per > 0.0f ? (float)b / per : 0.0f);
+                const float one = __builtin_amdgcn_exp2f(guess_bits - down * per_t);  // a logit's weight there
                 auto in_bin = [&](int at) { return at >= 0 && at < BINS ? (float)sh.count[at] : 0.0f; };
                 float in_list = in_bin(b);
-                for (; beside < 8; beside++) {
+                for (; beside < (z_per > 0.0f ? kZoom : 8); beside++) {
                   const float more = in_bin(b - beside - 1) + in_bin(b + beside + 1);
                   if (in_list + more > one * (float)(beside > 0 ? BLOCK * 5 / 8 : BLOCK * 7 / 8)) break;
                   in_list += more;
                 }
-                x_lo = uniform(low_value(first_key_below(b + uniform(beside) + 1)));
-                x_hi = uniform(high_value(first_key_below(b - uniform(beside)) - 1));
+                beside = uniform(beside);
+                if (z_per > 0.0f) {
+                  x_lo = uniform(z_hi - (float)(b + beside + 1) / z_per);
+                  x_hi = uniform(fminf(m, z_hi - (float)(b - beside) / z_per));
+                } else {
+                  x_lo = uniform(low_value(first_key_below(b + beside + 1)));
+                  x_hi = uniform(high_value(first_key_below(b - beside) - 1));
+                }
               }
               __syncthreads();
               if (threadIdx.x == 0 && !whole_list) sh.listed = 0;
@@ -1165,7 +1212,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
                   // next to it then: the nearest bin with anything in it, once
                   const int way = target <= above ? -1 : 1;
                   above = 0.0;
-                  b = uniform(b + way * (beside + 1));
+                  b = b + way * (beside + 1);
                   while (b >= 0 && b < BINS && !sh.count[b]) b += way;
                   if (attempt == 0 && b >= 0 && b < BINS) continue;
                 }

@@ -112,6 +112,18 @@ def test_split_rows(rows):
         check_sample(x[few], u[few], got=(got[0][few], got[1][few]), **cut)
 
 
+@pytest.mark.parametrize("rows", [1, 130])
+@pytest.mark.parametrize("spread", [0.0, 0.002, 0.02, 0.2])
+def test_flat_rows(rows, spread):
+    """many actions of nearly the same weight, split rows and whole ones: the border lies among thousands of them"""
+    for i, (n, dtype) in enumerate([(60_000, F32), (60_001, F16), (50_007, BF16), (33_333, F32)]):
+        x, u = make_logits(rows, n, dtype, n + rows, spread=spread)
+        if i == 3:
+            x[:, ::3] = 0.25
+        for cut in (dict(top_p=0.9), dict(top_p=0.01), dict(top_p=0.5, min_p=0.5), dict(top_p=0.999)):
+            check_sample(x[:5], u[:5], got=tuple(v[:5] for v in policy.sample_logits(x, u, **cut)), **cut)
+
+
 @pytest.mark.parametrize("rows", [2, 150])
 def test_temperatures_below_the_smallest_normal_number(rows):
     """1 / T is no binary32 number there, nor is one over the distance between the largest logit and the smallest kept"""
