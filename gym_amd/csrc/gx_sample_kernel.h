@@ -1102,12 +1102,11 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
             // Where the border's bin holds more than the list (a flat row), that bin and those beside it again, in kZoom bins:
             // 256 rows of 131 072, spread 0.05, 137 us, 300 by the finer and finer bins of step 4
             float z_hi = 0.0f, z_per = 0.0f;
-            if (!kOnePart && found) {
-              const float one = __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits);
+            if (!kOnePart && found && (float)sh.count[b] > __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits) * (float)(BLOCK * 7 / 8)) {
               const float z_lo = uniform(low_value(first_key_below(min(b + 2, BINS))));
               const unsigned long long z_above = uniform(sh.above_mass) - ((unsigned long long)(b > 0 ? sh.count[b - 1] : 0) << guess_shift);
               z_hi = uniform(high_value(first_key_below(b - 1) - 1));
-              if ((float)sh.count[b] > one * (float)(BLOCK * 7 / 8) && z_hi > z_lo) {
+              if (z_hi > z_lo) {
                 z_per = fminf((float)kZoom / (z_hi - z_lo), 3e38f);
                 __syncthreads();
                 for (int q = threadIdx.x; q < BINS; q += BLOCK) sh.count[q] = 0;
