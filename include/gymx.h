@@ -400,7 +400,7 @@ typedef struct gx_sample {
   int32_t* actions;          /* out [rows] */
   float* logprob;            /* out [rows], may be NULL: log of the probability the action was drawn with */
   void* workspace;           /* 256-byte aligned device memory of gx_sample_workspace's size (which follows from rows and
-                                n_actions alone: not 0 for few rows of many actions only); may be NULL where that is 0 */
+                                n_actions alone, 0 but for few rows of many actions); may be NULL where that is 0 */
   uint64_t workspace_bytes;
 } gx_sample;
 int gx_sample_workspace(gx_ctx* ctx, const gx_sample* sample, uint64_t* bytes);
