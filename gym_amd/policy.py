@@ -11,12 +11,21 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .envs import default_context
+from .envs import _contexts, default_context
 
 _dtypes = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16, torch.int32: L.I32, torch.int64: L.I64}
 _float_types = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 # the current stream's handle without building a Stream object: 0.1 instead of 1.9 us of a call's 9
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+# bytes of workspace by (query, GPU, sizes), which they follow from alone
+_needs = {}
+_sample_size, _embed_size = C.sizeof(L.GxSample), C.sizeof(L.GxEmbed)
+
+
+def _context(index):
+    return _contexts.get(index) or default_context(index)
 
 
 def _float_type(name, dtype):
@@ -37,7 +46,7 @@ def _on_gpu(name, t, device=None):
 
 def _vector(name, t, dtype, n, device):
     _on_gpu(name, t, device)
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
         raise ValueError("%s must be a contiguous %s tensor of shape (%d,)" % (name, dtype, n))
     return t.data_ptr()
 
@@ -48,23 +57,26 @@ def _call(fn, handle, desc, device):
         L.check(code)
 
 
-def _workspace(fn, ctx, desc, device):
-    need = C.c_uint64()
-    code = fn(ctx._h, C.byref(desc), C.byref(need))
-    if code:
-        L.check(code)
-    if not need.value:
+def _workspace(query, ctx, desc, device, *sizes):
+    key = (query, device.index) + sizes
+    need = _needs.get(key)
+    if need is None:
+        out = C.c_uint64()
+        L.check(getattr(L.load(), query)(ctx._h, C.byref(desc), C.byref(out)))
+        if len(_needs) >= 4096:
+            _needs.clear()
+        need = _needs[key] = out.value
+    if not need:
         return None
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device)  # torch's blocks are 512-byte aligned
-    desc.workspace, desc.workspace_bytes = ws.data_ptr(), need.value
+    ws = torch.empty(need, dtype=torch.uint8, device=device)  # torch's blocks are 512-byte aligned
+    desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
     return ws
 
 
 def _sample_desc(logits, u, temperature, top_k, top_p, min_p, actions, logprob):
     rows, n = logits.shape
     dev = logits.device
-    d = L.GxSample(C.sizeof(L.GxSample), L.OP_DEFAULT_STREAM, _float_type("logits", logits.dtype), n, rows,
-                   logits.stride(0), logits.stride(1), logits.data_ptr())
+    d = L.GxSample(_sample_size, L.OP_DEFAULT_STREAM, _float_type("logits", logits.dtype), n, rows, *logits.stride(), logits.data_ptr())
     if u is not None:
         d.u = _vector("u", u, torch.float32, rows, dev)
     if isinstance(temperature, torch.Tensor):
@@ -114,11 +126,12 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out
     if u is None:
         raise TypeError("u must be a torch tensor of random numbers (DeviceBatch.step_logits can draw its own)")
     dev = logits.device
-    out = _result("out", out, torch.int32, logits.shape[0], dev)
-    logprob = _result("logprob", logprob, torch.float32, logits.shape[0], dev)
-    ctx = default_context(dev.index)
+    rows, n = logits.shape
+    out = _result("out", out, torch.int32, rows, dev)
+    logprob = _result("logprob", logprob, torch.float32, rows, dev)
+    ctx = _context(dev.index)
     d = _sample_desc(logits, u, temperature, top_k, top_p, min_p, out, logprob)
-    ws = _workspace(L.load().gx_sample_workspace, ctx, d, dev)  # noqa: F841  (alive until the launch)
+    ws = _workspace("gx_sample_workspace", ctx, d, dev, rows, n)  # noqa: F841  (alive until the launch)
     _call(L.load().gx_sample_logits, ctx._h, d, dev)
     return out, logprob
 
@@ -133,18 +146,23 @@ def step_logits(batch, logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_
     actions = torch.empty(int(batch.view().stride), dtype=torch.int32, device=dev)
     logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=dev)
     d = _sample_desc(logits, u, temperature, top_k, top_p, min_p, actions, logprob)
-    ws = _workspace(L.load().gx_sample_workspace, batch.ctx, d, dev)  # noqa: F841
+    ws = _workspace("gx_sample_workspace", batch.ctx, d, dev, *logits.shape)  # noqa: F841
     _call(L.load().gx_vec_step_logits, batch._h, d, dev)
     return actions[:batch.n], logprob
 
 
 def _matrix(name, t, device=None):
+    """-> rows, columns, elements between rows"""
     _on_gpu(name, t, device)
-    if t.dim() != 2 or t.shape[1] < 1:
+    if t.dim() != 2:
         raise ValueError("%s must have shape (rows, dim), not %s" % (name, tuple(t.shape)))
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    rows, dim = t.shape
+    row_stride, col_stride = t.stride()
+    if dim < 1:
+        raise ValueError("%s must have shape (rows, dim), not %s" % (name, tuple(t.shape)))
+    if dim > 1 and col_stride != 1 or rows > 1 and row_stride < dim:
         raise ValueError("%s must have contiguous rows that do not overlap, strides are %s" % (name, t.stride()))
-    return max(t.stride(0), t.shape[1])
+    return rows, dim, row_stride if row_stride > dim else dim
 
 
 def _ids(ids, device):
@@ -153,20 +171,26 @@ def _ids(ids, device):
         raise ValueError("ids must be a contiguous int32 or int64 tensor of shape (tokens,)")
 
 
+def _rows(name, t, rows, dim, new, dtype, device):
+    """a matrix to write into, the caller's, checked, or a new one of type `new` -> it, elements between its rows"""
+    if t is None:
+        return torch.empty(rows, dim, dtype=new, device=device), dim
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError("%s is %s, dtype says %s" % (name, t.dtype, dtype))
+    stride = _matrix(name, t, device)[2]
+    if t.shape != (rows, dim):
+        raise ValueError("%s must have shape (%d, %d), not %s" % (name, rows, dim, tuple(t.shape)))
+    return t, stride
+
+
 def _lookup(fn, handle, weight, ids, tokens, scale, dtype, out):
-    stride = _matrix("weight", weight)
+    states, dim, stride = _matrix("weight", weight)
     dev = weight.device
-    if weight.shape[0] < 1:
+    if states < 1:
         raise ValueError("weight has no rows")
-    if out is None:
-        out = torch.empty(tokens, weight.shape[1], dtype=dtype or weight.dtype, device=dev)
-    elif dtype is not None and out.dtype != dtype:
-        raise ValueError("out is %s, dtype says %s" % (out.dtype, dtype))
-    out_stride = _matrix("out", out, dev)
-    if tuple(out.shape) != (tokens, weight.shape[1]):
-        raise ValueError("out must have shape (%d, %d), not %s" % (tokens, weight.shape[1], tuple(out.shape)))
-    d = L.GxEmbed(C.sizeof(L.GxEmbed), L.OP_DEFAULT_STREAM, _float_type("weight", weight.dtype), _float_type("out", out.dtype),
-                  L.I32 if ids is None else _dtypes[ids.dtype], 0, tokens, weight.shape[0], weight.shape[1], stride, out_stride,
+    out, out_stride = _rows("out", out, tokens, dim, dtype or weight.dtype, dtype, dev)
+    d = L.GxEmbed(_embed_size, L.OP_DEFAULT_STREAM, _float_type("weight", weight.dtype), _float_type("out", out.dtype),
+                  L.I32 if ids is None else _dtypes[ids.dtype], 0, tokens, states, dim, stride, out_stride,
                   None if ids is None else ids.data_ptr(), weight.data_ptr(), out.data_ptr(), None, 0, scale, 0)
     _call(fn, handle, d, dev)
     return out
@@ -179,7 +203,7 @@ def embed_lookup(weight, ids, scale=1.0, dtype=None, out=None):
     at least dim.  ids [tokens], int32 (an observation row of a batch) or int64; an id outside the table gives zeros."""
     _on_gpu("weight", weight)
     _ids(ids, weight.device)
-    return _lookup(L.load().gx_embed_lookup, default_context(weight.device.index)._h, weight, ids, ids.shape[0], scale, dtype, out)
+    return _lookup(L.load().gx_embed_lookup, _context(weight.device.index)._h, weight, ids, ids.shape[0], scale, dtype, out)
 
 
 def embed_obs(batch, weight, scale=1.0, dtype=None, out=None):
@@ -196,26 +220,21 @@ def embed_grad(grad, ids, n_states, scale=1.0, dtype=None, out=None, accumulate=
     grad [tokens, dim] and the result [n_states, dim]: float32 / float16 / bfloat16 each (`dtype`: float32 by default),
     contiguous rows.  out: a tensor to write into, accumulate adds to what it holds.  Ids outside the table are left
     out.  Equal calls give equal bits: the order of the additions depends on the ids alone."""
-    grad_stride = _matrix("grad", grad)
+    tokens, dim, grad_stride = _matrix("grad", grad)
     dev = grad.device
     _ids(ids, dev)
-    if ids.shape[0] != grad.shape[0]:
-        raise ValueError("%d ids for %d rows of grad" % (ids.shape[0], grad.shape[0]))
+    if ids.shape[0] != tokens:
+        raise ValueError("%d ids for %d rows of grad" % (ids.shape[0], tokens))
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
         if n_states < 1:
             raise ValueError("n_states must be positive")
-        out = torch.empty(n_states, grad.shape[1], dtype=dtype or torch.float32, device=dev)
-    elif dtype is not None and out.dtype != dtype:
-        raise ValueError("out is %s, dtype says %s" % (out.dtype, dtype))
-    out_stride = _matrix("out", out, dev)
-    if tuple(out.shape) != (n_states, grad.shape[1]):
-        raise ValueError("out must have shape (%d, %d), not %s" % (n_states, grad.shape[1], tuple(out.shape)))
-    ctx = default_context(dev.index)
-    d = L.GxEmbed(C.sizeof(L.GxEmbed), L.OP_DEFAULT_STREAM, _float_type("out", out.dtype), _float_type("grad", grad.dtype),
-                  _dtypes[ids.dtype], 1 if accumulate else 0, ids.shape[0], n_states, grad.shape[1], out_stride, grad_stride,
+    out, out_stride = _rows("out", out, n_states, dim, dtype or torch.float32, dtype, dev)
+    ctx = _context(dev.index)
+    d = L.GxEmbed(_embed_size, L.OP_DEFAULT_STREAM, _float_type("out", out.dtype), _float_type("grad", grad.dtype),
+                  _dtypes[ids.dtype], 1 if accumulate else 0, tokens, n_states, dim, out_stride, grad_stride,
                   ids.data_ptr(), out.data_ptr(), grad.data_ptr(), None, 0, scale, 0)
-    ws = _workspace(L.load().gx_embed_grad_workspace, ctx, d, dev)  # noqa: F841
+    ws = _workspace("gx_embed_grad_workspace", ctx, d, dev, tokens, n_states, dim)  # noqa: F841
     _call(L.load().gx_embed_grad, ctx._h, d, dev)
     return out
