@@ -73,30 +73,33 @@ def _workspace(query, ctx, desc, device, *sizes):
     return ws
 
 
+def _parameter(name, v, dtype, rows, device, otherwise):
+    """-> address of a parameter by row and its common value, or no address and the number"""
+    if isinstance(v, torch.Tensor):
+        return _vector(name, v, dtype, rows, device), otherwise
+    return None, v
+
+
+_numbers = (float, int)  # what _parameter need not be asked about
+
+
 def _sample_desc(logits, u, temperature, top_k, top_p, min_p, actions, logprob):
     rows, n = logits.shape
     dev = logits.device
-    d = L.GxSample(_sample_size, L.OP_DEFAULT_STREAM, _float_type("logits", logits.dtype), n, rows, *logits.stride(), logits.data_ptr())
-    if u is not None:
-        d.u = _vector("u", u, torch.float32, rows, dev)
-    if isinstance(temperature, torch.Tensor):
-        d.temperature = _vector("temperature", temperature, torch.float32, rows, dev)
-    else:
-        d.temperature_all = temperature
-    if isinstance(top_k, torch.Tensor):
-        d.top_k = _vector("top_k", top_k, torch.int32, rows, dev)
-    else:
-        d.top_k_all = max(-1, min(top_k, 2**31 - 1))  # (the field would cut a larger number short)
-    if isinstance(top_p, torch.Tensor):
-        d.top_p = _vector("top_p", top_p, torch.float32, rows, dev)
-    else:
-        d.top_p_all = top_p
-    if isinstance(min_p, torch.Tensor):
-        d.min_p = _vector("min_p", min_p, torch.float32, rows, dev)
-    else:
-        d.min_p_all = min_p
-    d.actions, d.logprob = actions.data_ptr(), logprob.data_ptr()
-    return d
+    t = k = p = q = None
+    if type(temperature) not in _numbers:
+        t, temperature = _parameter("temperature", temperature, torch.float32, rows, dev, 1.0)
+    if type(top_k) is not int:
+        k, top_k = _parameter("top_k", top_k, torch.int32, rows, dev, 0)
+    if type(top_p) not in _numbers:
+        p, top_p = _parameter("top_p", top_p, torch.float32, rows, dev, 1.0)
+    if type(min_p) not in _numbers:
+        q, min_p = _parameter("min_p", min_p, torch.float32, rows, dev, 0.0)
+    if top_k > 2**31 - 1 or top_k < -1:  # (the field would cut them short)
+        top_k = max(-1, min(top_k, 2**31 - 1))
+    return L.GxSample(_sample_size, L.OP_DEFAULT_STREAM, _float_type("logits", logits.dtype), n, rows, *logits.stride(), logits.data_ptr(),
+                      None if u is None else _vector("u", u, torch.float32, rows, dev), t, k, p, q, temperature, top_k, top_p, min_p,
+                      actions.data_ptr(), logprob.data_ptr())
 
 
 def _logits(logits):
