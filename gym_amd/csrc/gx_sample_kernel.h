@@ -438,6 +438,7 @@ constexpr int kAhead = 2;
 constexpr int kPartActions = 8192;
 enum Part { kWhole = 0, kPartMax = 1, kPartList = 2, kPartExact = 3, kPartJoin = 4 };
 constexpr int kMostParts = 64, kWideBlock = 512, kWideBins = 2048, kWideSegments = 1024, kListMost = kWideBlock, kZoom = 64;
+constexpr int kTopsMost = 8192;  // places in the lists of a row's parts together
 
 struct SplitRow {
   double sum[kMostParts];       // of each part: exact, and estimated relative to its largest logit
@@ -445,6 +446,7 @@ struct SplitRow {
   float top[kMostParts];        // its largest logit
   float bound[kMostParts];      // what k of its lanes' largest reach, or -inf
   float share[kMostParts];      // what 2 k / parts of them reach: half the parts together have k that reach their median
+  uint32_t tops[kMostParts];    // lengths of the parts' own lists (see cap)
   uint32_t listed, around;      // lengths of the lists; more than kListMost: not kept
   float list_x[kListMost];      // what may be kept
   int list_i[kListMost];
@@ -453,6 +455,8 @@ struct SplitRow {
   uint32_t bins[kWideBins];     // estimates
   double seg_sum[kWideSegments];
   float seg_max[kWideSegments];
+  float tops_x[kTopsMost];      // cap places a part
+  int tops_i[kTopsMost];
 };
 
 // low bits of the ordered key that are the same for every value of the type (all clear, or all set below zero)
@@ -554,7 +558,7 @@ template <class T, int W> __device__ __forceinline__ float run_largest(const uin
 __host__ __device__ __forceinline__ int share_of(int k, int parts) { return (2 * k + parts - 1) / parts; }
 
 template <class T, int BLOCK, int BINS, int SEGMENTS, int RUN_BYTES, bool CUT, bool PACKED, Part PART>
-__global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, SplitRow* split) {
+__global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, int cap, SplitRow* split) {
   constexpr bool kOnePart = PART == kPartMax || PART == kPartList || PART == kPartExact;  // of a row, not all of it
   constexpr int kWaves = BLOCK / 64, kRun = PACKED ? RUN_BYTES / (int)sizeof(T) : 8, kTurn = 64 * kRun;
   __shared__ WideShared<BLOCK, BINS, SEGMENTS> sh;
@@ -736,25 +740,67 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
       double above = 0.0;   // what lies above the list
       double s1 = 0.0;      // the sum (of all; for top-p alone)
       float split_bound = -kInf;
+      // what the parts left, asked for at once (64 of them at most: every wave has them all)
+      float part_top = -kInf, part_bound = -kInf, part_share = -kInf, early_x[2] = {};
+      uint32_t part_tops = 0;
+      int early_i[2] = {};
+      if (PART >= kPartList) {
+        if (lane < parts) {
+          part_top = sr->top[lane];
+          part_bound = sr->bound[lane];
+          part_share = sr->share[lane];
+          part_tops = sr->tops[lane];
+        }
+        if (PART == kPartJoin && cap)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {  // (cap is 128 at least)
+            const int at = min(wave + e * kWaves, parts - 1) * cap + lane;
+            early_x[e] = sr->tops_x[at];
+            early_i[e] = sr->tops_i[at];
+          }
+      }
+      // what one part's lanes reach alone; or what enough parts reach with their share (see kPartMax)
+      auto bound_of_parts = [&]() {
+        const float bound = group_max<64>(part_bound), b = part_share;
+        const int share = min(share_of(s.k, parts), s.k), need = (s.k + share - 1) / share;
+        int rank = 0;
+        for (int j = 0; j < parts; j++) {
+          const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(b), j));
+          rank += o > b || (o == b && j < lane) ? 1 : 0;
+        }
+        const unsigned long long who = __ballot(lane < parts && rank == need - 1);
+        return fmaxf(bound, __shfl(b, __ffsll(who) - 1, 64));
+      };
       if (PART >= kPartList) {
         const bool mine = (int)threadIdx.x < parts;
-        m = block_max(mine ? sr->top[threadIdx.x] : -kInf);
+        m = uniform(group_max<64>(part_top));
         if (kOnePart && (far_k || m == kInf || m == -kInf || (PART == kPartExact && !sums))) continue;
         if (m < kInf && m > -kInf) {
           if (PART != kPartJoin) {
             if (sums) s1 = block_sum(mine ? sr->estimate[threadIdx.x] * weight(sr->top[threadIdx.x], m, s.per_t) : 0.0);
-            if (by_k) {
-              // what one part's lanes reach alone; or what enough parts reach with their share (see kPartMax)
-              split_bound = block_max(mine ? sr->bound[threadIdx.x] : -kInf);
-              const int share = min(share_of(s.k, parts), s.k), need = (s.k + share - 1) / share;
-              const float b = lane < parts ? sr->share[lane] : -kInf;
-              int rank = 0;
-              for (int j = 0; j < parts; j++) {
-                const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(b), j));
-                rank += o > b || (o == b && j < lane) ? 1 : 0;
+            if (by_k) split_bound = bound_of_parts();
+          } else if (cap) {
+            if (__all(part_tops <= (uint32_t)cap)) {
+              const float b = uniform(bound_of_parts());
+              if (threadIdx.x == 0) sh.listed = 0;
+              __syncthreads();
+              for (int q = wave, e = 0; q < parts; q += kWaves, e++) {
+                const int n = __builtin_amdgcn_readlane((int)part_tops, q);
+                for (int at = lane; at < n; at += 64) {
+                  const bool early = at == lane && e < 2;
+                  const float v = early ? (e ? early_x[1] : early_x[0]) : sr->tops_x[q * cap + at];
+                  if (v >= b) {
+                    const int i = early ? (e ? early_i[1] : early_i[0]) : sr->tops_i[q * cap + at];
+                    const uint32_t to = atomicAdd(&sh.listed, 1u);
+                    if (to < (uint32_t)BLOCK) {
+                      sh.list_x[to] = v;
+                      sh.list_i[to] = i;
+                    }
+                  }
+                }
               }
-              const unsigned long long who = __ballot(lane < parts && rank == need - 1);
-              split_bound = fmaxf(split_bound, __shfl(b, __ffsll(who) - 1, 64));
+              __syncthreads();
+              list = taken = uniform(sh.listed) <= (uint32_t)BLOCK;
             }
           } else if (!far_k) {
             const uint32_t listed = uniform(sr->listed), around = uniform(sr->around);
@@ -823,6 +869,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
           sr->top[part] = m;
           sr->estimate[part] = s1;
           sr->bound[part] = sr->share[part] = -kInf;
+          sr->tops[part] = m > -kInf ? kListMost + 1 : 0;
           if (part == 0) sr->listed = sr->around = 0;
         }
         if (!by_k || far_k || !(m > -kInf && m < kInf)) continue;
@@ -870,13 +917,50 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, Sp
             const float b = reached_by(wave == 0 ? s.k : min(share_of(s.k, parts), s.k), from);
             if (lane == 0) {
               if (PART == kPartMax) (wave == 0 ? sr->bound : sr->share)[part] = b;
-              else sh.bound = fmaxf(from, b);
+              if (wave == 0) sh.bound = fmaxf(from, b);
             }
           }
           __syncthreads();
-          if (PART != kPartMax) from = uniform(sh.bound);
+          from = uniform(sh.bound);
         }
-        if (PART == kPartMax) continue;
+        if (PART == kPartMax) {
+          if (cap) {  // this part's own list, of what k of its lanes reach: kPartJoin takes what all parts' bound leaves of them
+            __syncthreads();
+            if (threadIdx.x == 0) sh.listed = 0;
+            __syncthreads();
+            each([&](int, bool, int i, const Run& e) {
+              if (!__any(largest(e, i) >= from)) return;
+              float x[kRun];
+              values(e, i, x);
+              uint32_t in = 0;
+#pragma unroll
+              for (int j = 0; j < kRun; j++) in |= x[j] >= from ? 1u << j : 0u;
+#pragma unroll 1
+              while (in) {
+                const int j = __ffs(in) - 1;
+                in &= in - 1;
+                float v = x[0];
+#pragma unroll
+                for (int k = 1; k < kRun; k++) v = j == k ? x[k] : v;
+                if (sh.listed <= (uint32_t)BLOCK) {
+                  const uint32_t at = atomicAdd(&sh.listed, 1u);
+                  if (at < (uint32_t)BLOCK) {
+                    sh.list_x[at] = v;
+                    sh.list_i[at] = start(i) + j;
+                  }
+                }
+              }
+            });
+            __syncthreads();
+            const uint32_t n = uniform(sh.listed);
+            if (threadIdx.x == 0) sr->tops[part] = n;
+            if (threadIdx.x < n && threadIdx.x < (uint32_t)cap) {
+              sr->tops_x[part * cap + threadIdx.x] = sh.list_x[threadIdx.x];
+              sr->tops_i[part * cap + threadIdx.x] = sh.list_i[threadIdx.x];
+            }
+          }
+          continue;
+        }
         // ---- ... and the bins
         from = uniform(from);
         // (finite: m's own bin has to be 0, and 0 * inf is not)
@@ -1508,22 +1592,29 @@ template <class T, bool CUT, bool PACKED> hipError_t launch_rows(const SampleArg
   GX_GROUP(1, 16) GX_GROUP(2, 16) GX_GROUP(4, 16) GX_GROUP(8, 16) GX_GROUP(16, 16) GX_GROUP(32, 16) GX_GROUP(64, 16)
 #undef GX_GROUP
   if (a.n <= kWideSmall) {
-    hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED, kWhole>), grid(1), dim3(256), 0, stream, a, 1, nullptr);
+    hipLaunchKernelGGL((wide_kernel<T, 256, 512, 16, 16, CUT, PACKED, kWhole>), grid(1), dim3(256), 0, stream, a, 1, 0, nullptr);
     return hipGetLastError();
   }
 #define GX_WIDE(PART, GRID) \
-  hipLaunchKernelGGL((wide_kernel<T, kWideBlock, kWideBins, kWideSegments, 32, CUT, PACKED, PART>), GRID, dim3(kWideBlock), 0, stream, a, parts, split)
+  hipLaunchKernelGGL((wide_kernel<T, kWideBlock, kWideBins, kWideSegments, 32, CUT, PACKED, PART>), GRID, dim3(kWideBlock), 0, stream, a, parts, cap, split)
+  int cap = 0;
   const int parts = split_parts(a, num_cus);
   if (parts < 2) {
     GX_WIDE(kWhole, grid(1));
     return hipGetLastError();
   }
   const dim3 all((unsigned)(a.rows * (uint64_t)parts));
+  // A top-k known here leaves so little of a part that its list is made at once
+  const int k = a.greedy_all ? 1 : a.top_k ? 0 : a.top_k_all;
+  const int places = kTopsMost / parts < kListMost ? kTopsMost / parts : kListMost;
+  if (k > 0 && k < a.n && 2 * k <= places) cap = places;
   GX_WIDE(kPartMax, all);
   if constexpr (CUT) {
-    GX_WIDE(kPartList, all);
-    const bool top_p_alone = (a.top_p || a.top_p_all < 1.0f) && (a.top_k || a.top_k_all <= 0 || a.top_k_all >= a.n);
-    if (top_p_alone) GX_WIDE(kPartExact, all);
+    if (!cap) {
+      GX_WIDE(kPartList, all);
+      const bool top_p_alone = (a.top_p || a.top_p_all < 1.0f) && (a.top_k || a.top_k_all <= 0 || a.top_k_all >= a.n);
+      if (top_p_alone) GX_WIDE(kPartExact, all);
+    }
   }
   GX_WIDE(kPartJoin, grid(1));
 #undef GX_WIDE

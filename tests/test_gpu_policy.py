@@ -112,6 +112,27 @@ def test_split_rows(rows):
         check_sample(x[few], u[few], got=(got[0][few], got[1][few]), **cut)
 
 
+@pytest.mark.parametrize("n", [16_384, 50_001, 300_000, 600_001])
+def test_split_rows_top_k(n):
+    """the parts' own lists: all of the largest in one part, parts with nothing or too little, more than the places hold"""
+    for i, (dtype, k) in enumerate([(F32, 1), (BF16, 7), (F16, 50), (F32, 64), (F32, 128), (BF16, 256), (F16, 257), (F32, 512), (F32, 513)]):
+        x, u = make_logits(5, n, dtype, n + k, spread=1.0)
+        x[1, : n // 3] += 9
+        x[2, n // 40:] = -INF
+        x[3] = -INF
+        x[3, :: max(1, n // (k // 2 + 2))] = 1.0
+        x[4, 100:-100] = -INF
+        check_sample(x, u, top_k=k)
+        check_sample(x, u, top_k=k, top_p=0.6, temperature=2.0, min_p=0.001)
+        x[0] = 0.5
+        x[1, n // 2] = INF
+        x[2, 5] = math.nan
+        check_sample(x, u, top_k=k, top_p=0.9)
+    t = torch.tensor([1.0, 0.0, 0.5, 2.0, math.nan], device="cuda")
+    check_sample(x, u, got=policy.sample_logits(x, u, temperature=t, top_k=40), temperature=torch.nan_to_num(t), top_k=40)
+    check_sample(x, u, temperature=0.0, top_p=0.5)
+
+
 @pytest.mark.parametrize("rows", [1, 130])
 @pytest.mark.parametrize("spread", [0.0, 0.002, 0.02, 0.2])
 def test_flat_rows(rows, spread):
