@@ -429,9 +429,10 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 // Few rows leave most of the card idle, so each is split among several workgroups (parts), and the steps become launches
 // that hand their results on in the workspace: kPartMax is step 1, kPartList step 2 (and for min-p alone the segments'
 // sums), kPartExact step 3, kPartJoin the rest, by one workgroup a row.  Where a step says that the row needs more than
-// that (a list too long, +inf or NaN among the logits, k above kListMost), kPartJoin goes through the row by itself.  One
-// row of 131 072: 46 us with top-p against 94 by one workgroup, 27 against 31 with top-k (three launches of 6 to 11 us);
-// 37 rows of 50 001 with min-p 25 against 35.
+// that (a list too long, +inf or NaN among the logits, k above kListMost), kPartJoin goes through the row by itself.  With
+// a small top-k for all rows step 2 needs no launch: kPartMax lists what the part's own bound leaves (`cap` places a part),
+// and kPartJoin takes what all parts' bound leaves of that.  One row of 131 072: 46 us with top-p against 94 by one
+// workgroup; 21 with top-k 50, 26 with a launch for step 2, 31 by one workgroup; 37 rows of 50 001 with min-p 25 and 35.
 constexpr int kWideSmall = 4096;
 constexpr int kAhead = 2;
 // Actions a part has at least.  One row of 131 072, top-p: 50 us with 16 384, 46 with 8 192, 44 with 4 096.
