@@ -1059,7 +1059,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
           for (int j = 1; j < kRun - 1; j++) same = same && x[j] == v;
           return (bool)__all(same);
         };
-        auto guess_of = [&](float x) { return (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(x - m, per_t, guess_bits)) + 0.5f); };
+        auto guess_of = [&](float x) { return (uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(m - x, -per_t, guess_bits)) + 0.5f); };
         // those of a list of this workgroup's that is not too long, into the row's
         auto hand_on = [&](uint32_t* count, float* to_x, int* to_i) {
           const uint32_t n = uniform(sh.listed);
@@ -1100,9 +1100,6 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
               if (!__any(largest(e, i) >= x_lo)) return;
               float x[kRun];
               values(e, i, x);
-              uint32_t in = 0;  // which of the run
-#pragma unroll
-              for (int j = 0; j < kRun; j++) in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
               const bool append = listing && sh.listed <= (uint32_t)BLOCK;
               if (!exact) {
                 // estimates: 24 bits are enough to find the bin, or the one beside it
@@ -1115,6 +1112,9 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
                 }
                 if (!append) return;
               }
+              uint32_t in = 0;  // which of the run
+#pragma unroll
+              for (int j = 0; j < kRun; j++) in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
               if (exact && !append) {
                 if (one_value(x) && __all(in & 1)) {
                   if (lane == 0) {
@@ -1250,8 +1250,9 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
                 for (int j = 0; j < kRun; j++) {
                   const double w = weight(x[j], m, s.per_t);
                   sum += w;
-                  here += x[j] > x_hi ? w : 0.0;  // above min-p's bound too, which no bin lies below
-                  in |= x[j] >= x_lo && x[j] <= x_hi ? 1u << j : 0u;
+                  const bool over = x[j] > x_hi;  // above min-p's bound too, which no bin lies below
+                  here = __builtin_fma(w, __hiloint2double(over ? 0x3FF00000 : 0, 0), here);  // w times 1 or 0: one choice, not two
+                  in |= x[j] >= x_lo && !over ? 1u << j : 0u;
                 }
 #pragma unroll 1
                 while (in) {
