@@ -19,6 +19,7 @@
 #pragma once
 
 #include "gx_launch.h"
+#include "gx_math.h"
 #include "gx_policy.h"
 
 namespace gx {
@@ -88,19 +89,21 @@ template <bool CUT> __device__ __forceinline__ RowParams row_params(const Sample
 }
 
 // 2^t, t <= 0: t = k + f, |f| <= 1/2, and a polynomial for 2^f with a relative error below 1.5e-13 (an equal-ripple fit
-// of degree 9, exact at f = 0)
-__device__ __forceinline__ double exp2_neg(double t) {
+// of degree 9, exact at f = 0).  SCALAR: the coefficients in scalar registers, where the compiler, short of them, would
+// move each into vector registers first (group_kernel: 92 -> 89 us of 65 536 rows of 255; the large form spills with it).
+template <bool SCALAR> __device__ __forceinline__ double exp2_neg(double t) {
+  auto term = [](double e, double f, double c) { return SCALAR ? math::fma_k(e, f, c) : __builtin_fma(e, f, c); };
   t = fmax(t, -1100.0);  // 2^t is 0 there, and for a NaN
   const double k = rint(t), f = t - k;
   double e = 0x1.89efabdef686ep-24;
-  e = __builtin_fma(e, f, 0x1.63c688cf3cab8p-20);
-  e = __builtin_fma(e, f, 0x1.fffb62b51cef6p-17);
-  e = __builtin_fma(e, f, 0x1.4308b503274e4p-13);
-  e = __builtin_fma(e, f, 0x1.5d87ed72fbd66p-10);
-  e = __builtin_fma(e, f, 0x1.3b2ab71455231p-7);
-  e = __builtin_fma(e, f, 0x1.c6b08d793b970p-5);
-  e = __builtin_fma(e, f, 0x1.ebfbdff8256ebp-3);
-  e = __builtin_fma(e, f, 0x1.62e42fefa11f3p-1);
+  e = term(e, f, 0x1.63c688cf3cab8p-20);
+  e = term(e, f, 0x1.fffb62b51cef6p-17);
+  e = term(e, f, 0x1.4308b503274e4p-13);
+  e = term(e, f, 0x1.5d87ed72fbd66p-10);
+  e = term(e, f, 0x1.3b2ab71455231p-7);
+  e = term(e, f, 0x1.c6b08d793b970p-5);
+  e = term(e, f, 0x1.ebfbdff8256ebp-3);
+  e = term(e, f, 0x1.62e42fefa11f3p-1);
   e = __builtin_fma(e, f, 1.0);
   return __builtin_ldexp(e, (int)k);
 }
@@ -132,7 +135,9 @@ __device__ __forceinline__ double log_from_one(double c) {
 
 // The weight of a logit beside the largest, which is finite (see without_inf): 1 for that, 0 for -inf.  `per_t` is
 // log2(e) / T.  (-inf / inf is a NaN on the way and 0 in the end.)
-__device__ __forceinline__ double weight(float x, float m, double per_t) { return exp2_neg(((double)x - (double)m) * per_t); }
+template <bool SCALAR = false> __device__ __forceinline__ double weight(float x, float m, double per_t) {
+  return exp2_neg<SCALAR>(((double)x - (double)m) * per_t);
+}
 
 // Beside +inf every finite logit weighs nothing, and those that are +inf weigh the same: 0 and -inf say that in finite terms.
 __device__ __forceinline__ float without_inf(float x) { return x == kInf ? 0.0f : -kInf; }
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       double sw[E], sum = 0.0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        sw[e] = first + e < s.k ? weight(value_of(v[e]), m, s.per_t) : 0.0;
+        sw[e] = first + e < s.k ? weight<true>(value_of(v[e]), m, s.per_t) : 0.0;
         sum += sw[e];
       }
       double s1, ahead = group_before<G>(sum, &s1);
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
     double w[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      w[e] = weight(x[e], m, s.per_t);
+      w[e] = weight<true>(x[e], m, s.per_t);
       if (CUT) {
         const bool tie = x[e] == t;
         w[e] = (x[e] > t || (tie && before < ties)) && w[e] >= s.q ? w[e] : 0.0;
