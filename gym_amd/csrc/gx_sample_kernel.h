@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 #pragma unroll
     for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
     m = group_max<G>(m);
-    if (__any(m == kInf) && m == kInf) {
+    const bool infinite = m == kInf;
+    if (__any(infinite) && infinite) {
 #pragma unroll
       for (int e = 0; e < E; e++) x[e] = without_inf(x[e]);
       m = 0.0f;
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       double sw[E], sum = 0.0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        sw[e] = first + e < s.k ? weight<true>(value_of(v[e]), m, s.per_t) : 0.0;
+        sw[e] = weight<true>(first + e < s.k ? value_of(v[e]) : -kInf, m, s.per_t);
         sum += sw[e];
       }
       double s1, ahead = group_before<G>(sum, &s1);
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       int kept = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const bool in = first + e == 0 || (first + e < s.k && ahead < target && sw[e] > 0.0);
+        const bool in = (e == 0 && first == 0) || (ahead < target && sw[e] > 0.0);
         ahead += sw[e];
         mine = in ? v[e] : mine;
         kept += in ? 1 : 0;
@@ -365,11 +366,11 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       int above = 0, equal = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        above += __popcll(group_ballot<G>(x[e] > t));
+        above += x[e] > t ? 1 : 0;
         equal += x[e] == t ? 1 : 0;
       }
       before = running_sum<G>(equal) - equal;
-      ties = count - above;
+      ties = count - group_lane<G>(running_sum<G>(above), G - 1);
     }
     double w[E];
 #pragma unroll
@@ -377,35 +378,41 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
       w[e] = weight<true>(x[e], m, s.per_t);
       if (CUT) {
         const bool tie = x[e] == t;
-        w[e] = (x[e] > t || (tie && before < ties)) && w[e] >= s.q ? w[e] : 0.0;
+        w[e] = x[e] > t || (tie && before < ties) ? w[e] : 0.0;
         before += tie ? 1 : 0;
       }
     }
+    if (CUT && __any(s.q > 0.0))
+#pragma unroll
+      for (int e = 0; e < E; e++) w[e] = w[e] >= s.q ? w[e] : 0.0;
     double sum = 0.0, total;
 #pragma unroll
     for (int e = 0; e < E; e++) sum += w[e];
-    double c = group_before<G>(sum, &total);
-    const double stop = s.u * total;
-    int past = -1, last = -1;  // this lane's first action past the border, its last one kept
-    float x_past = 0.0f, x_last = 0.0f;
+    const double start = group_before<G>(sum, &total), stop = s.u * total;
+    double c = start;
+    int at = first;  // the lane's first action past the border: as many as are not
 #pragma unroll
     for (int e = 0; e < E; e++) {
       c += w[e];
-      if (w[e] > 0.0) {
-        last = first + e;
-        x_last = x[e];
-        if (past < 0 && c > stop) {
-          past = last;
-          x_past = x_last;
-        }
-      }
+      at += c > stop ? 0 : 1;
     }
-    const unsigned long long over = group_ballot<G>(past >= 0), kept = group_ballot<G>(last >= 0);
-    // rounding may have put the border at the total: the last one kept then
-    const int chosen_lane = over ? __ffsll(over) - 1 : (kept ? 63 - __clzll(kept) : 0);
+    const unsigned long long over = group_ballot<G>(c > stop && sum > 0.0);
+    int chosen_lane = __ffsll(over) - 1;
+    if (__any(lane == chosen_lane && start > stop) && start > stop) {  // rounding put the border between two lanes: the first kept
+      at = first + E;
+#pragma unroll
+      for (int e = E - 1; e >= 0; e--) at = w[e] > 0.0 ? first + e : at;
+    }
+    if (__any(!over) && !over) {  // rounding put the border at the total, or nothing is kept: the last one kept
+      at = -1;
+#pragma unroll
+      for (int e = 0; e < E; e++) at = w[e] > 0.0 ? first + e : at;
+      const unsigned long long kept = group_ballot<G>(at >= 0);
+      chosen_lane = kept ? 63 - __clzll(kept) : 0;
+    }
     if (live && lane == chosen_lane) {
       const bool none = m == -kInf;
-      write_result(a, r, none ? -1 : (over ? past : last), over ? x_past : x_last, m, s.inv_t, total);
+      write_result(a, r, none ? -1 : at, infinite || none ? 0.0f : clean(to_f32(row[(int64_t)at * a.col_stride])), m, s.inv_t, total);
     }
   }
 }
