@@ -29,7 +29,7 @@ namespace {
 constexpr float kInf = __builtin_inff();
 
 // ordered bits: a < b as numbers <=> key(a) < key(b); -0 and +0 are one, NaN is -inf
-__device__ __forceinline__ float clean(float x) { return x != x ? -kInf : x + 0.0f; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.0f, -kInf); }
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
