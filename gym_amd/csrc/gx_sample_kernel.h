@@ -3,9 +3,9 @@
 // The kept set is a beginning of the order "logit descending, equal logits by index", so it is described by one logit t
 // and a count j: everything above t, and the first j (by index) of those equal to t.  Weights exp((x - m) / T) and their
 // sums are binary64 (or integers of 62 bits) throughout: which action u falls on is a border in a sum of up to 2^24 terms,
-// and a sum in binary32 would move it past one action in a thousand.  A binary64 instruction takes about 6 cycles of a
-// SIMD here (chains of them, measured) and an exponential some 20 of them: what bounds all but the smallest calls is
-// instructions, not memory.
+// and a sum in binary32 would move it past one action in a thousand.  A binary64 instruction takes a SIMD 2.1 ns here, a
+// binary32 one 1.8, whether it waits for the one before or not (chains of them, 8 waves a SIMD), and an exponential is 18
+// of them: what bounds all but the smallest calls is the number of instructions, not memory.
 //
 // Three forms, by the number of actions:
 //   up to 8      a lane a row, every pair of actions compared (row_kernel)
@@ -13,8 +13,8 @@
 //                (group_kernel)
 //   more         a workgroup a row, or several where there are few rows; the border of the kept set is found by histograms
 //                and a short list, never by a sort of the row (wide_kernel)
-// The borders, binary32 with top-p 0.9: 1 Mi rows of 8 take 22 us in the first form and 53 in the second, 16 384 rows of
-// 1 000 105 us in the second and 397 in the third, 8 192 rows of 2 048 412 us in the second (32 actions a lane) and 223 in
+// The borders, binary32 with top-p 0.9: 1 Mi rows of 8 take 21 us in the first form and 53 in the second, 16 384 rows of
+// 1 000 95 us in the second and 397 in the third, 8 192 rows of 2 048 412 us in the second (32 actions a lane) and 225 in
 // the third.
 #pragma once
 
@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(kBlock) row_kernel(SampleArgs a) {
 // registers (a bitonic network: the values alone, not their indices, for t and j are all that is wanted), weighed in that
 // order and summed along it; the draw then goes over the row as it lies.  Many actions a lane and many rows a wave: most
 // of the network's steps stay within a lane, and what is done once a row (parameters, scans, the logarithm) is done for
-// several at once.  65 536 rows of 255 bfloat16 (33 MB), all cuts, parameters by row: 88 us, against 118 with 4 actions a
-// lane; without a cut 36 and 42.  About 2 000 instructions a wave of four rows at 5.8 cycles are all of that time.
+// several at once.  65 536 rows of 255 bfloat16 (33 MB), all cuts, parameters by row: 78 us (when 4 actions a lane were
+// tried, 118 with them and 92 with 16); without a cut 30.  Some 1 900 instructions a wave of four rows are all of that time.
 template <int M> __device__ __forceinline__ float max_with(float v) { return fmaxf(v, __uint_as_float(xor_lane<M>(__float_as_uint(v)))); }
 template <int G> __device__ __forceinline__ float group_max(float v) {
   if constexpr (G > 1) v = max_with<1>(v);
@@ -432,8 +432,8 @@ __global__ void __launch_bounds__(kBlock) group_kernel(SampleArgs a) {
 //      goes into finer and finer bins with integer masses (whose order of adding changes nothing) until it holds one
 //      value, and a last pass adds up what is kept by segments
 // then the segment u falls into, and in it the action.  The passes are bound by instructions, so step 3 is the only one that
-// takes an exponential in binary64 of every action.  256 rows of 131 072 bfloat16 (67 MB, a copy 14 us): 99 us with top-p
-// 0.9 (14 us step 1, 25 step 2, 40 step 3, the rest for the list and the draw), 37 with top-k 50, 41 without a cut.  What
+// takes an exponential in binary64 of every action.  256 rows of 131 072 bfloat16 (67 MB, a copy 14 us): 95 us with top-p
+// 0.9 (14 us step 1, 22 step 2, 37 step 3, the rest for the list and the draw), 37 with top-k 50, 38 without a cut.  What
 // runs for few elements is a loop: unrolled, the kernel outgrew the instruction cache and took three times as long.  512
 // threads, not 1 024: those leave a lane 128 registers, and what spilled waited behind the loads on their way (113 and 53 us
 // for the first two).  Rows of up to 4 096 have 256 threads (4 096 rows of as many, top-p: 143 us, 341 with 512).
@@ -1197,7 +1197,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
             // ---- 3: the exact sum; above the border's bin and its neighbours by segments, and those listed
             int b = uniform(sh.bin);
             // Where the border's bin holds more than the list (a flat row), that bin and those beside it again, in kZoom bins:
-            // 256 rows of 131 072, spread 0.05, 137 us, 300 by the finer and finer bins of step 4
+            // 256 rows of 131 072, spread 0.05, 132 us, 300 by the finer and finer bins of step 4
             float z_hi = 0.0f, z_per = 0.0f;
             if (!kOnePart && found && (float)sh.count[b] > __builtin_amdgcn_exp2f(per > 0.0f ? guess_bits - (float)b / per * per_t : guess_bits) * (float)(BLOCK * 7 / 8)) {
               const float z_lo = uniform(low_value(first_key_below(min(b + 2, BINS))));
