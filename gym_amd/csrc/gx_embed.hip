@@ -95,10 +95,10 @@ __global__ void __launch_bounds__(kBlock) lookup_kernel(EmbedArgs a, int lanes_s
 // Bound by the rows it reads: 4 Mi tokens of 128 bfloat16 and 704 states (1.07 GB) take 282 us, 216 of them step 2 at
 // 5.0 TB/s, whatever the order of the ids; 56 the sort (37 its scatter: 48 when the pairs left for their places one by one,
 // not in the runs that a sort of the tile in LDS makes of them), 17 step 3.  8 191 tokens of 1 001 columns and 50 001 states:
-// 78 us, 32 of them the 200 MB that are cleared while the tokens are sorted.
+// 75 us, 28 of them the 200 MB that are cleared while the tokens are sorted.
 constexpr int kSortOne = 8192, kSortThreads = 1024;  // tokens one workgroup sorts alone
 constexpr int kTile = 16384;                         // tokens of a tile, 16 a thread
-constexpr int kMaxDigit = 10;
+constexpr int kMaxDigit = 10, kOneBits = 8;          // bits of a digit, of tiles and of one workgroup's sort
 constexpr int kFold = 64;  // chunks whose parts of a long run become one
 
 struct __align__(8) Pair { uint32_t key, token; };
@@ -136,9 +136,10 @@ GradPlan grad_plan(const EmbedArgs& a, int num_cus) {
   p.direct = n > 0 && n <= 2048 && groups <= 24576 && groups * ((n + 63) / 64) <= (1u << 17);
   if (p.direct) return p;
   p.bits = 64 - __builtin_clzll((unsigned long long)a.n_states);  // 0 .. n_states
-  p.passes = (p.bits + kMaxDigit - 1) / kMaxDigit;
-  p.digit = (p.bits + p.passes - 1) / p.passes;
   p.one = n <= (uint64_t)kSortOne;
+  const int most = p.one ? kOneBits : kMaxDigit;
+  p.passes = (p.bits + most - 1) / most;
+  p.digit = (p.bits + p.passes - 1) / p.passes;
   p.tiles = (uint32_t)((n + kTile - 1) / kTile);
   const int64_t pieces = a.dim >= kPiece ? (a.dim + kPiece - 1) / kPiece : a.dim;
   p.lanes_shift = shift_for(a.dim, 6);
@@ -238,20 +239,20 @@ __device__ __forceinline__ void scan_lds(uint32_t* values, int n, uint32_t* sums
   __syncthreads();
 }
 
-// Up to kSortOne tokens by one workgroup: digits of 5 bits (the counters of 16 waves fit beside the pairs in LDS), each
+// Up to kSortOne tokens by one workgroup: digits of up to 8 bits (the counters of 16 waves fit beside the pairs in LDS), each
 // wave owning a contiguous stretch, so that (digit, wave) order keeps equal ids in the order of their tokens.
-constexpr int kOneBits = 5;
 template <class T>
-__global__ void __launch_bounds__(kSortThreads) sort_one_kernel(EmbedArgs a, int bits, Pair* out) {
+__global__ void __launch_bounds__(kSortThreads) sort_one_kernel(EmbedArgs a, int bits, int digit, Pair* out) {
   if (blockIdx.x) {
     clear_table<T>(a, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
-  constexpr int kWaves = kSortThreads / 64, kMost = kSortOne / kSortThreads, kBins = 1 << kOneBits;
+  constexpr int kWaves = kSortThreads / 64, kMost = kSortOne / kSortThreads;
   __shared__ Pair pairs[kSortOne];
-  __shared__ uint32_t counts[kBins * kWaves];  // [digit][wave]
+  __shared__ uint32_t counts[kWaves << kOneBits];  // [digit][wave]
   __shared__ uint32_t sums[kWaves];
-  static_assert(kBins * kWaves <= kSortThreads, "one counter a thread");
+  static_assert((kWaves << kOneBits) <= 4 * kSortThreads, "scan_lds takes four a thread");
+  const int n_bins = 1 << digit;
   const int n = (int)a.tokens, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // element e of this lane is token (wave * each + e) * 64 + lane
   const int each = (n + kSortThreads - 1) / kSortThreads, base = wave * each * 64 + lane;
@@ -261,16 +262,16 @@ __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(EmbedArgs a, int
     const int i = base + e * 64;
     if (e < each && i < n) p[e] = Pair{sort_key(a, i), (uint32_t)i};
   }
-  for (int shift = 0; shift < bits; shift += kOneBits) {
-    if (threadIdx.x < kBins * kWaves) counts[threadIdx.x] = 0;
+  for (int shift = 0; shift < bits; shift += digit) {
+    for (int b = threadIdx.x; b < n_bins * kWaves; b += kSortThreads) counts[b] = 0;
     __syncthreads();
     uint32_t rank[kMost];
 #pragma unroll
     for (int e = 0; e < kMost; e++) {
       if (e >= each) break;
       const bool live = base + e * 64 < n;
-      const uint32_t d = live ? (p[e].key >> shift) & (kBins - 1) : 0;
-      const unsigned long long same = same_digit(d, kOneBits, __ballot(live)), below = same & ((1ull << lane) - 1);
+      const uint32_t d = live ? (p[e].key >> shift) & (n_bins - 1) : 0;
+      const unsigned long long same = same_digit(d, digit, __ballot(live)), below = same & ((1ull << lane) - 1);
       const uint32_t before = live ? counts[d * kWaves + wave] : 0;
       wave_order();
       rank[e] = before + __popcll(below);
@@ -278,10 +279,10 @@ __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(EmbedArgs a, int
       wave_order();
     }
     __syncthreads();
-    scan_lds(counts, kBins * kWaves, sums);
+    scan_lds(counts, n_bins * kWaves, sums);
 #pragma unroll
     for (int e = 0; e < kMost; e++)
-      if (e < each && base + e * 64 < n) pairs[counts[((p[e].key >> shift) & (kBins - 1)) * kWaves + wave] + rank[e]] = p[e];
+      if (e < each && base + e * 64 < n) pairs[counts[((p[e].key >> shift) & (n_bins - 1)) * kWaves + wave] + rank[e]] = p[e];
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kMost; e++)
@@ -779,7 +780,7 @@ hipError_t launch_embed_grad(const EmbedArgs& a, int table, int rows, void* work
   return by_type(table, [&](auto t) -> hipError_t {
     using T = decltype(t);
     if (p.one) {
-      hipLaunchKernelGGL(sort_one_kernel<T>, dim3((unsigned)(1 + clear)), dim3(kSortThreads), 0, stream, a, p.bits, pairs);
+      hipLaunchKernelGGL(sort_one_kernel<T>, dim3((unsigned)(1 + clear)), dim3(kSortThreads), 0, stream, a, p.bits, p.digit, pairs);
     } else {
       uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
       uint32_t* totals = reinterpret_cast<uint32_t*>(ws + p.totals);
