@@ -109,6 +109,7 @@ struct GradPlan {
   bool one;                 // one workgroup sorts
   uint32_t tiles;
   int lanes_shift;          // lanes of a group: 8 columns each
+  int join_shift;           // lanes a part, as a power of two, at four columns each
   int64_t col_tiles;        // groups a row takes
   uint32_t chunk, chunks;   // tokens of a chunk, number of chunks
   size_t pairs_a, pairs_b, counts, totals, parts, folds, bytes;  // offsets into the workspace
@@ -159,7 +160,10 @@ GradPlan grad_plan(const EmbedArgs& a, int num_cus) {
     p.totals = take((size_t)4 << p.digit);
   }
   if (p.chunks > 1) p.parts = take((size_t)p.chunks * 2 * (size_t)a.dim * 4);
-  if (p.chunks > 2 * (uint32_t)kFold) p.folds = take((size_t)(p.chunks / kFold) * (size_t)a.dim * 4);
+  while (p.join_shift < 6 && ((int64_t)4 << p.join_shift) < a.dim) p.join_shift++;
+  // Folding is a launch.  Without it the workgroup that joins a run of all chunks goes through them 64 at a time, times the
+  // parts that a wave takes at once.
+  if (p.chunks > (256u << (6 - p.join_shift))) p.folds = take((size_t)(p.chunks / kFold) * (size_t)a.dim * 4);
   p.bytes = n ? at : 0;
   return p;
 }
@@ -808,14 +812,12 @@ hipError_t launch_embed_grad(const EmbedArgs& a, int table, int rows, void* work
       return hipGetLastError();
     });
     if (e != hipSuccess || p.chunks < 2) return e;
-    int join_shift = 0;  // lanes a row at four columns each
-    while (join_shift < 6 && ((int64_t)4 << join_shift) < a.dim) join_shift++;
     const uint64_t join_tiles = (uint64_t)(a.dim + 255) / 256, units = (uint64_t)(p.chunks - 1) * join_tiles;
     float* folds = p.folds ? reinterpret_cast<float*>(ws + p.folds) : nullptr;
     if (folds)
-      hipLaunchKernelGGL(fold_kernel, dim3(capped((uint64_t)(p.chunks / kFold) * join_tiles)), dim3(64 * kJoinWaves), 0, stream, a, join_shift, p.chunk,
+      hipLaunchKernelGGL(fold_kernel, dim3(capped((uint64_t)(p.chunks / kFold) * join_tiles)), dim3(64 * kJoinWaves), 0, stream, a, p.join_shift, p.chunk,
                          p.chunks, pairs, parts, folds);
-    hipLaunchKernelGGL(join_kernel<T>, dim3(capped((units + kJoinWaves - 1) / kJoinWaves)), dim3(64 * kJoinWaves), 0, stream, a, join_shift,
+    hipLaunchKernelGGL(join_kernel<T>, dim3(capped((units + kJoinWaves - 1) / kJoinWaves)), dim3(64 * kJoinWaves), 0, stream, a, p.join_shift,
                        p.chunk, p.chunks, pairs, parts, folds);
     return hipGetLastError();
   });
