@@ -1229,25 +1229,39 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
 #pragma unroll 1
             for (int attempt = 0;; attempt++) {
               float x_lo = kInf, x_hi = kInf;  // nothing
-              int beside = 0;
+              int upper = b, lower = b;        // the bins that are listed
               if (found) {
                 // as many bins on either side as the list should hold; one, if it can
                 const float down = z_per > 0.0f ? (m - z_hi) + (float)b / z_per : (per > 0.0f ? (float)b / per : 0.0f);
                 const float one = __builtin_amdgcn_exp2f(guess_bits - down * per_t);  // a logit's weight there
                 auto in_bin = [&](int at) { return at >= 0 && at < BINS ? (float)sh.count[at] : 0.0f; };
                 float in_list = in_bin(b);
+                int beside = 0;
                 for (; beside < (z_per > 0.0f ? kZoom : 8); beside++) {
                   const float more = in_bin(b - beside - 1) + in_bin(b + beside + 1);
                   if (in_list + more > one * (float)(beside > 0 ? BLOCK * 5 / 8 : BLOCK * 7 / 8)) break;
                   in_list += more;
                 }
-                beside = uniform(beside);
+                upper = b - beside;
+                lower = b + beside;
+                // where the guess says that the border lies near the bin's end, the next bin with anything in it too (logits of
+                // 16 bits leave bins empty).  Without, 1 of 16 sets of 256 rows had a row that went through all this again: 122
+                // us, not 97
+                if (attempt == 0 && z_per == 0.0f) {
+                  const unsigned long long at = want_mass - sh.above_mass, sixteenth = sh.bin_mass >> 4;
+                  const int way = at < sixteenth ? -1 : (at > sh.bin_mass - sixteenth ? 1 : 0);
+                  int next = way < 0 ? upper - 1 : lower + 1;
+                  while (way && next >= 0 && next < BINS && !sh.count[next]) next += way;
+                  if (way && next >= 0 && next < BINS && in_list + in_bin(next) <= one * (float)(BLOCK * 7 / 8)) (way < 0 ? upper : lower) = next;
+                }
+                upper = uniform(upper);
+                lower = uniform(lower);
                 if (z_per > 0.0f) {
-                  x_lo = uniform(z_hi - (float)(b + beside + 1) / z_per);
-                  x_hi = uniform(fminf(m, z_hi - (float)(b - beside) / z_per));
+                  x_lo = uniform(z_hi - (float)(lower + 1) / z_per);
+                  x_hi = uniform(fminf(m, z_hi - (float)upper / z_per));
                 } else {
-                  x_lo = uniform(low_value(first_key_below(b + beside + 1)));
-                  x_hi = uniform(high_value(first_key_below(b - beside) - 1));
+                  x_lo = uniform(low_value(first_key_below(lower + 1)));
+                  x_hi = uniform(high_value(first_key_below(upper) - 1));
                 }
               }
               __syncthreads();
@@ -1309,7 +1323,7 @@ __global__ void __launch_bounds__(BLOCK) wide_kernel(SampleArgs a, int parts, in
                   // next to it then: the nearest bin with anything in it, once
                   const int way = target <= above ? -1 : 1;
                   above = 0.0;
-                  b = b + way * (beside + 1);
+                  b = way < 0 ? upper - 1 : lower + 1;
                   while (b >= 0 && b < BINS && !sh.count[b]) b += way;
                   if (attempt == 0 && b >= 0 && b < BINS) continue;
                 }
